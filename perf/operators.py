@@ -267,7 +267,8 @@ def _plain_route(s, out):
         j = torch.arange(nb, device="cuda")
         score = score.masked_fill((j < FIRST) | (j >= seen - LAST), math.inf).masked_fill(j >= seen, -math.inf)
         order = torch.sort(score, dim=-1, descending=True, stable=True)[1][..., :P]
-        probes = torch.where(torch.arange(order.shape[-1], device="cuda") < seen, order, -1)
+        order = order.masked_fill(order >= seen, nb).sort(-1)[0]                                    # in the order of the cache
+        probes = torch.where(order < nb, order, -1)
         out[b, :m, :, :probes.shape[-1]] = probes.transpose(0, 1).to(torch.int32)
     return out
 
@@ -486,7 +487,8 @@ def exact(case, seed):
                 near[(j < FIRST) | (at - j < LAST)] = math.inf
                 near[j.expand_as(near) > at] = -math.inf
                 best = near.argsort(dim=1, descending=True, stable=True)[:, :P].to(torch.int32)
-                best[torch.arange(best.shape[1], device=dev)[None] > at] = -1
+                best = torch.where(best > at, 1 << 30, best).sort(dim=1)[0]
+                best[best == 1 << 30] = -1
                 probes[b, :qlens[b], h, :best.shape[1]] = best
         return summary, probes
 
