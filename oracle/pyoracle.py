@@ -22,7 +22,7 @@ _u64p = C.POINTER(C.c_uint64)
 def build(force=False):
     """Compile liboracle.so / liboracle_refflags.so (and _ref/ref_core when /root/reference is present)."""
     targets = ["all"]
-    if os.path.isdir(os.environ.get("GPANN_REFERENCE", "/root/reference")):
+    if os.path.isfile(os.path.join(os.environ.get("GPANN_REFERENCE", "/root/reference"), "src", "defs.cpp")):   # (an empty mount is no checkout)
         targets.append("ref")
     if force:
         subprocess.check_call(["make", "-C", _HERE, "clean"])
