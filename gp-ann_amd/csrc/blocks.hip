@@ -1,0 +1,408 @@
+// blocks.hip — block operators: layout checks, centroids of the blocks, routing of query rows to blocks, eviction (include/gpann_blocks.h).
+#include "blocks.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace gpann {
+
+// ---- checks ---------------------------------------------------------------------------------------------------------------------------------
+// no two elements of an [n0][n1][n2][d] tensor share an address: ordered by stride, every dimension steps over the extent of those below it
+bool BlocksDisjoint(const int64_t stride[3], uint64_t n0, uint64_t n1, uint64_t n2, uint32_t d) {
+    std::pair<int64_t, uint64_t> dim[3] = {{stride[0], n0}, {stride[1], n1}, {stride[2], n2}};
+    std::sort(dim, dim + 3);
+    int64_t extent = d;
+    for (const auto& [s, n] : dim) {
+        if (n <= 1) continue;
+        if (s < extent) return false;
+        extent += s * (int64_t)(n - 1);
+    }
+    return true;
+}
+
+gpann_status BlocksCheckLayout(const gpann_blocks_layout* L) {
+    GPANN_REQUIRE(L != nullptr, "layout is null");
+    GPANN_REQUIRE(L->struct_bytes == sizeof(gpann_blocks_layout), "layout.struct_bytes is not sizeof(gpann_blocks_layout) of this library");
+    GPANN_REQUIRE(L->dtype == GPANN_BLOCKS_BF16 || L->dtype == GPANN_BLOCKS_FP16, "layout.dtype must be GPANN_BLOCKS_BF16 or GPANN_BLOCKS_FP16");
+    GPANN_REQUIRE((L->flags & ~(uint32_t)GPANN_BLOCKS_CAUSAL) == 0, "unknown bits in layout.flags");
+    GPANN_REQUIRE(L->batch <= 65535 && L->q_rows <= (1u << 24) && L->kv_rows <= (1u << 24), "batch above 65535 or more than 2^24 rows");
+    GPANN_REQUIRE(L->kv_heads > 0 && L->q_heads > 0 && L->q_heads % L->kv_heads == 0, "q_heads must be a positive multiple of kv_heads");
+    GPANN_REQUIRE(L->q_heads <= 1024, "more than 1024 query heads");
+    const uint32_t d = L->head_dim;
+    GPANN_REQUIRE(d == 64 || d == 96 || d == 128 || d == 192 || d == 256, "head_dim must be 64, 96, 128, 192 or 256");
+    GPANN_REQUIRE(L->block_rows >= 16 && L->block_rows <= 256 && L->block_rows % 16 == 0, "block_rows must be a multiple of 16 from 16 to 256");
+    GPANN_REQUIRE(BlocksPerSequence(L) <= GPANN_BLOCKS_MAX_BLOCKS, "more than GPANN_BLOCKS_MAX_BLOCKS blocks per sequence");
+    GPANN_REQUIRE(std::isfinite(L->scale), "layout.scale is not finite");
+    const int64_t* strides[4] = {L->q_stride, L->k_stride, L->v_stride, L->out_stride};
+    for (const int64_t* s : strides)
+        for (int i = 0; i < 3; ++i) {
+            GPANN_REQUIRE(s[i] >= 0 && s[i] % 8 == 0, "strides must be non-negative multiples of 8 elements");
+            GPANN_REQUIRE(s[i] <= (int64_t)1 << 40, "a stride above 2^40 elements");
+        }
+    if (L->page_table) {
+        GPANN_REQUIRE(L->page_stride >= BlocksPerSequence(L), "layout.page_stride is smaller than a sequence's blocks");
+        GPANN_REQUIRE(L->n_pages <= 0x7fffffffu, "more than 2^31 - 1 pages");
+    }
+    return GPANN_OK;
+}
+
+// a stream of another device would run the kernels where the tensors are not
+gpann_status BlocksCheckStream(const gpann_blocks_layout* L, void* stream) {
+    if (!stream) return GPANN_OK;
+    hipDevice_t dev = -1;
+    GPANN_HIP_TRY(hipStreamGetDevice(static_cast<hipStream_t>(stream), &dev));
+    GPANN_REQUIRE((int)dev == L->device, "the stream belongs to another device than the layout");
+    return GPANN_OK;
+}
+
+BlocksArgs BlocksMakeArgs(const gpann_blocks_layout* L, const void* q, const void* k, const void* v, const int32_t* probes, uint32_t nprobe) {
+    BlocksArgs a{};
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k);
+    a.v = static_cast<const uint16_t*>(v);
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = L->q_stride[i];
+        a.ks[i] = L->k_stride[i];
+        a.vs[i] = L->v_stride[i];
+        a.os[i] = L->out_stride[i];
+    }
+    a.q_len = L->q_len;
+    a.kv_len = L->kv_len;
+    a.table = L->page_table;
+    a.probes = probes;
+    a.B = L->batch;
+    a.Tq = L->q_rows;
+    a.Tk = L->kv_rows;
+    a.Hq = L->q_heads;
+    a.Hkv = L->kv_heads;
+    a.G = L->q_heads / L->kv_heads;
+    a.bs = L->block_rows;
+    a.nblk = BlocksPerSequence(L);
+    a.P = nprobe;
+    a.table_stride = L->page_stride;
+    a.n_pages = L->n_pages;
+    a.causal = (L->flags & GPANN_BLOCKS_CAUSAL) ? 1 : 0;
+    a.scale = L->scale;
+    a.scale2 = L->scale * kLog2e;
+    return a;
+}
+
+// ---- centroids ------------------------------------------------------------------------------------------------------------------------------
+// One workgroup per (block, head, sequence).  A thread adds eight dimensions of every (256 * 8 / d)-th row in binary64 — sums of 16-bit floats, exact but
+// for exponents that lie more than 2^40 apart — and the row groups are added in LDS, always in the same order.
+template <bool BF16>
+__global__ void __launch_bounds__(256) BlocksSummarizeKernel(BlocksArgs a, uint32_t d, uint32_t new_rows, float* __restrict__ summary) {
+    extern __shared__ double s_sum[];   // [row group][d]
+    const uint32_t b = blockIdx.z, h = blockIdx.y;
+    const int n = BlocksKvLen(a, b);
+    if (n == 0) return;
+    const int first = new_rows == 0 ? 0 : max(0, n - (int)min(new_rows, (uint32_t)n)) / (int)a.bs;
+    const int block = first + (int)blockIdx.x, row0 = block * (int)a.bs;
+    if (row0 >= n) return;
+    int64_t ko, vo;
+    const bool there = BlocksBase(a, b, block, ko, vo);
+    const int rows = there ? min((int)a.bs, n - row0) : 0;
+    const uint32_t chunks = d / 8, groups = 256 / chunks, chunk = threadIdx.x % chunks, group = threadIdx.x / chunks;
+    if (group < groups) {
+        double acc[8] = {};
+        const uint16_t* p = a.k + ko + h * a.ks[2] + chunk * 8;
+        for (int r = (int)group; r < rows; r += (int)groups) {
+            const uint4 x = *reinterpret_cast<const uint4*>(p + r * a.ks[1]);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[2 * i] += BlocksToDouble((uint16_t)w[i], BF16);
+                acc[2 * i + 1] += BlocksToDouble((uint16_t)(w[i] >> 16), BF16);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s_sum[group * d + chunk * 8 + i] = acc[i];
+    }
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < d; c += 256) {
+        double t = 0;
+        for (uint32_t g = 0; g < groups; ++g) t += s_sum[g * d + c];
+        summary[(((int64_t)b * a.Hkv + h) * a.nblk + block) * d + c] = rows > 0 ? (float)(t / rows) : 0.f;
+    }
+}
+
+// ---- routing --------------------------------------------------------------------------------------------------------------------------------
+// binary64 -> unsigned whose order is the numbers' order; NaN is the smallest, both zeros are equal
+__device__ __forceinline__ uint64_t BlocksScoreKey(double x) {
+    if (x != x) return 0;
+    const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
+    return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+}
+
+// One workgroup per (query row, key/value head, sequence).  Scores in binary64 because a selection has to come out the same whatever the order of a sum:
+// neighbouring scores differ by far more than 2^-50.  Sixteen lanes share a block's centroid.  The nprobe-th best key is found by bisection over the
+// 64 key bits — every thread counts the keys it wrote — and the blocks that reach it are written in block order.
+template <bool BF16>
+__global__ void __launch_bounds__(256) BlocksRouteKernel(BlocksArgs a, uint32_t d, const float* __restrict__ summary, uint32_t first, uint32_t last,
+                                                         int32_t* __restrict__ probes) {
+    extern __shared__ double s_route[];
+    double* s_q = s_route;                                            // [d]
+    uint64_t* s_key = reinterpret_cast<uint64_t*>(s_route + d);       // [blocks]
+    __shared__ uint32_t s_count[4];
+    const uint32_t b = blockIdx.z, h = blockIdx.y, t = blockIdx.x;
+    const int n = BlocksKvLen(a, b), m = BlocksQLen(a, b);
+    if ((int)t >= m) return;
+    const int visible = BlocksVisible(a, n, m, t);
+    const uint32_t nb = (uint32_t)(visible + (int)a.bs - 1) / a.bs;
+    int32_t* out = probes + (((int64_t)b * a.Tq + t) * a.Hkv + h) * a.P;
+    if (nb <= a.P) {
+        for (uint32_t j = threadIdx.x; j < a.P; j += 256) out[j] = j < nb ? (int32_t)j : -1;
+        return;
+    }
+    for (uint32_t c = threadIdx.x; c < d; c += 256) {
+        const uint16_t* p = a.q + b * a.qs[0] + t * a.qs[1] + (int64_t)h * a.G * a.qs[2] + c;
+        double x = 0;
+        for (uint32_t g = 0; g < a.G; ++g) x += BlocksToDouble(p[g * a.qs[2]], BF16);
+        s_q[c] = x;
+    }
+    __syncthreads();
+    const float* cen = summary + ((int64_t)b * a.Hkv + h) * a.nblk * d;
+    const uint32_t sub = threadIdx.x & 15;
+    for (uint32_t j0 = 0; j0 < nb; j0 += 16) {
+        const uint32_t j = j0 + threadIdx.x / 16;
+        double x = 0;
+        if (j < nb) {
+            const float* c = cen + (int64_t)j * d;
+            for (uint32_t i = sub * 4; i < d; i += 64) {
+                const float4 v = *reinterpret_cast<const float4*>(c + i);
+                const double* qq = s_q + i;
+                x = fma(qq[0], (double)v.x, x);
+                x = fma(qq[1], (double)v.y, x);
+                x = fma(qq[2], (double)v.z, x);
+                x = fma(qq[3], (double)v.w, x);
+            }
+        }
+        for (int s = 8; s > 0; s >>= 1) x += __shfl_xor(x, s);
+        if (sub == 0 && j < nb) s_key[j] = (j < first || j + last >= nb) ? ~0ull : BlocksScoreKey(x);
+    }
+    __syncthreads();
+    // largest key v with count(key >= v) >= P
+    uint64_t v = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+        const uint64_t trial = v | (1ull << bit);
+        uint32_t c = 0;
+        for (uint32_t j = threadIdx.x; j < nb; j += 256) c += s_key[j] >= trial;
+        for (int s = 32; s > 0; s >>= 1) c += __shfl_xor(c, s);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) s_count[threadIdx.x >> 6] = c;
+        __syncthreads();
+        c = s_count[0] + s_count[1] + s_count[2] + s_count[3];
+        if (c >= a.P) v = trial;
+        if (c == a.P) break;
+    }
+    // blocks above v all stay; of those equal to v the lowest.  One wavefront walks the blocks in order.
+    if (threadIdx.x < 64) {
+        const uint32_t lane = threadIdx.x;
+        uint32_t above = 0;
+        for (uint32_t j0 = 0; j0 < nb; j0 += 64) above += (uint32_t)__popcll(__ballot(j0 + lane < nb && s_key[min(j0 + lane, nb - 1)] > v));
+        uint32_t equal = a.P - above, at = 0;
+        for (uint32_t j0 = 0; j0 < nb && at < a.P; j0 += 64) {
+            const uint64_t key = s_key[min(j0 + lane, nb - 1)];
+            const bool in = j0 + lane < nb, gt = in && key > v, eq = in && key == v;
+            const uint64_t below = (1ull << lane) - 1, eqs = __ballot(eq);
+            const bool take = gt || (eq && (uint32_t)__popcll(eqs & below) < equal);
+            const uint64_t taken = __ballot(take);
+            if (take) out[at + (uint32_t)__popcll(taken & below)] = (int32_t)(j0 + lane);
+            at += (uint32_t)__popcll(taken);
+            equal -= min(equal, (uint32_t)__popcll(eqs));
+        }
+    }
+}
+
+// ---- eviction -------------------------------------------------------------------------------------------------------------------------------
+// binary32 -> unsigned whose order is the numbers' order; NaN is the smallest, both zeros are equal
+__device__ __forceinline__ uint32_t BlocksMassKey(float x) {
+    if (x != x) return 0;
+    return OrderedKey(x + 0.f);
+}
+
+// One workgroup per (head, sequence): bisection for the smallest key that stays, then one pass in row order.
+__global__ void __launch_bounds__(1024) BlocksEvictSelectKernel(BlocksArgs a, const float* __restrict__ mass, uint32_t keep, uint32_t first, uint32_t last,
+                                                                int32_t* __restrict__ rows, int32_t* __restrict__ count) {
+    __shared__ uint32_t s_count[16], s_eq[16];
+    const uint32_t h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const uint32_t n = (uint32_t)BlocksKvLen(a, b);
+    const uint32_t take = min(n, keep);
+    const int64_t pair = (int64_t)b * a.Hkv + h;
+    const float* ms = mass + pair * a.Tk;
+    int32_t* out = rows + pair * keep;
+    if (tid == 0) count[pair] = (int32_t)take;
+    if (n <= keep) {
+        for (uint32_t j = tid; j < n; j += 1024) out[j] = (int32_t)j;
+        return;
+    }
+    auto key = [&](uint32_t j) -> uint64_t { return (j < first || j + last >= n) ? 1ull << 32 : (uint64_t)BlocksMassKey(ms[j]); };
+    auto total = [&](uint32_t c) {
+        for (int s = 32; s > 0; s >>= 1) c += __shfl_xor(c, s);
+        __syncthreads();
+        if (lane == 0) s_count[wave] = c;
+        __syncthreads();
+        c = 0;
+        for (int w = 0; w < 16; ++w) c += s_count[w];
+        return c;
+    };
+    uint64_t v = 0;
+    for (int bit = 32; bit >= 0; --bit) {
+        const uint64_t trial = v | (1ull << bit);
+        uint32_t c = 0;
+        for (uint32_t j = tid; j < n; j += 1024) c += key(j) >= trial;
+        c = total(c);
+        if (c >= take) v = trial;
+        if (c == take) break;
+    }
+    uint32_t above = 0;
+    for (uint32_t j = tid; j < n; j += 1024) above += key(j) > v;
+    above = total(above);
+    uint32_t equal = take - above, at = 0;
+    const uint64_t below = (1ull << lane) - 1;
+    for (uint32_t j0 = 0; j0 < n && at < take; j0 += 1024) {
+        const uint32_t j = j0 + tid;
+        const uint64_t kk = j < n ? key(j) : 0;
+        const bool gt = j < n && kk > v, eq = j < n && kk == v;
+        const uint64_t gts = __ballot(gt), eqs = __ballot(eq);
+        __syncthreads();
+        if (lane == 0) {
+            s_count[wave] = (uint32_t)__popcll(gts);
+            s_eq[wave] = (uint32_t)__popcll(eqs);
+        }
+        __syncthreads();
+        uint32_t gt_before = 0, eq_before = 0, gt_all = 0, eq_all = 0;
+        for (uint32_t w = 0; w < 16; ++w) {
+            if (w < wave) {
+                gt_before += s_count[w];
+                eq_before += s_eq[w];
+            }
+            gt_all += s_count[w];
+            eq_all += s_eq[w];
+        }
+        const uint32_t g = gt_before + (uint32_t)__popcll(gts & below), e = eq_before + (uint32_t)__popcll(eqs & below);
+        if (gt || (eq && e < equal)) out[at + g + min(e, equal)] = (int32_t)j;
+        at += gt_all + min(equal, eq_all);
+        equal -= min(equal, eq_all);
+    }
+}
+
+// 16 bytes of a kept row per thread
+__global__ void __launch_bounds__(256) BlocksEvictCopyKernel(BlocksArgs a, uint32_t chunks, uint32_t keep, const int32_t* __restrict__ rows,
+                                                             const int32_t* __restrict__ count, const float* __restrict__ mass, uint16_t* __restrict__ k_out,
+                                                             uint16_t* __restrict__ v_out, int64_t os0, int64_t os1, int64_t os2, float* __restrict__ mass_out) {
+    const uint32_t b = blockIdx.y;
+    const uint64_t all = (uint64_t)keep * a.Hkv * chunks;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t c = (uint32_t)(i % chunks), h = (uint32_t)(i / chunks % a.Hkv), r = (uint32_t)(i / chunks / a.Hkv);
+        const int64_t pair = (int64_t)b * a.Hkv + h;
+        if ((int)r >= count[pair]) continue;
+        const int row = rows[pair * keep + r];
+        if (c == 0 && mass_out) mass_out[pair * keep + r] = mass[pair * a.Tk + row];
+        if (!k_out) continue;
+        int64_t ko, vo;
+        const int block = row / (int)a.bs, in = row % (int)a.bs;
+        uint4 x{}, y{};
+        if (BlocksBase(a, b, block, ko, vo)) {
+            x = *reinterpret_cast<const uint4*>(a.k + ko + in * a.ks[1] + h * a.ks[2] + c * 8);
+            y = *reinterpret_cast<const uint4*>(a.v + vo + in * a.vs[1] + h * a.vs[2] + c * 8);
+        }
+        const int64_t o = b * os0 + r * os1 + h * os2 + c * 8;
+        *reinterpret_cast<uint4*>(k_out + o) = x;
+        *reinterpret_cast<uint4*>(v_out + o) = y;
+    }
+}
+
+static bool Aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool Aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
+}  // namespace gpann
+
+using namespace gpann;
+
+extern "C" {
+
+gpann_status gpann_blocks_summarize(const gpann_blocks_layout* L, const void* k, uint32_t new_rows, float* summary, void* stream) {
+    GPANN_TRY(BlocksCheckLayout(L));
+    GPANN_REQUIRE(k && summary, "a tensor is null");
+    GPANN_REQUIRE(Aligned16(k) && Aligned16(summary), "tensors must be 16-byte aligned");
+    GPANN_BLOCKS_ENTER(L, stream);
+    const BlocksArgs a = BlocksMakeArgs(L, nullptr, k, nullptr, nullptr, 0);
+    if (a.B == 0 || a.nblk == 0) return GPANN_OK;
+    // the last new_rows rows start anywhere in a block
+    const uint32_t touched = new_rows == 0 ? a.nblk : std::min<uint32_t>(a.nblk, (uint32_t)(((uint64_t)new_rows + a.bs - 2) / a.bs + 1));
+    const uint32_t d = L->head_dim, groups = 256 / (d / 8);
+    const dim3 grid(touched, a.Hkv, a.B);
+    const size_t lds = (size_t)groups * d * sizeof(double);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (L->dtype == GPANN_BLOCKS_BF16)
+        hipLaunchKernelGGL(BlocksSummarizeKernel<true>, grid, dim3(256), lds, st, a, d, new_rows, summary);
+    else
+        hipLaunchKernelGGL(BlocksSummarizeKernel<false>, grid, dim3(256), lds, st, a, d, new_rows, summary);
+    GPANN_HIP_TRY(hipGetLastError());
+    return GPANN_OK;
+}
+
+gpann_status gpann_blocks_route(const gpann_blocks_layout* L, const void* q, const float* summary, uint32_t nprobe, uint32_t first, uint32_t last,
+                                int32_t* probes, void* workspace, size_t workspace_bytes, void* stream) {
+    (void)workspace;
+    (void)workspace_bytes;
+    GPANN_TRY(BlocksCheckLayout(L));
+    GPANN_REQUIRE(q && summary && probes, "a tensor is null");
+    GPANN_REQUIRE(Aligned16(q) && Aligned16(summary) && Aligned4(probes), "q and summary must be 16-byte aligned, probes 4-byte aligned");
+    GPANN_REQUIRE(nprobe >= 1 && nprobe <= GPANN_BLOCKS_MAX_PROBE, "nprobe must be 1 .. GPANN_BLOCKS_MAX_PROBE");
+    GPANN_REQUIRE(first <= nprobe && last <= nprobe - first, "first + last must not exceed nprobe");
+    GPANN_REQUIRE(last >= 1 || !(L->flags & GPANN_BLOCKS_CAUSAL), "a causal route needs last >= 1");
+    GPANN_BLOCKS_ENTER(L, stream);
+    const BlocksArgs a = BlocksMakeArgs(L, q, nullptr, nullptr, nullptr, nprobe);
+    if (a.B == 0 || a.Tq == 0) return GPANN_OK;
+    const uint32_t d = L->head_dim;
+    const dim3 grid(a.Tq, a.Hkv, a.B);
+    const size_t lds = (size_t)(d + a.nblk) * sizeof(double);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    auto kernel = L->dtype == GPANN_BLOCKS_BF16 ? BlocksRouteKernel<true> : BlocksRouteKernel<false>;
+    if (lds > 32 * 1024) GPANN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a, d, summary, first, last, probes);
+    GPANN_HIP_TRY(hipGetLastError());
+    return GPANN_OK;
+}
+
+gpann_status gpann_blocks_evict(const gpann_blocks_layout* L, const void* k, const void* v, const float* mass, uint32_t keep, uint32_t first, uint32_t last,
+                                int32_t* rows, int32_t* count, void* k_out, void* v_out, const int64_t out_kv_stride[3], float* mass_out, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+    (void)workspace;
+    (void)workspace_bytes;
+    GPANN_TRY(BlocksCheckLayout(L));
+    GPANN_REQUIRE(mass && rows && count, "a tensor is null");
+    GPANN_REQUIRE((k_out == nullptr) == (v_out == nullptr), "k_out and v_out must be given together");
+    GPANN_REQUIRE(k_out == nullptr || (k && v && out_kv_stride), "a tensor is null");
+    GPANN_REQUIRE(Aligned16(k) && Aligned16(v) && Aligned16(k_out) && Aligned16(v_out), "k, v, k_out and v_out must be 16-byte aligned");
+    GPANN_REQUIRE(Aligned4(mass) && Aligned4(rows) && Aligned4(count) && Aligned4(mass_out), "tensors must be 4-byte aligned");
+    GPANN_REQUIRE(keep >= 1 && keep <= (1u << 24), "keep must be 1 .. 2^24");
+    GPANN_REQUIRE(first <= keep && last <= keep - first, "first + last must not exceed keep");
+    GPANN_REQUIRE(mass_out == nullptr || mass_out != mass, "mass_out must not be mass");
+    if (k_out) {
+        GPANN_REQUIRE(k_out != k && v_out != v && k_out != v_out && k_out != v && v_out != k, "the outputs must not overlap the cache");
+        for (int i = 0; i < 3; ++i)
+            GPANN_REQUIRE(out_kv_stride[i] >= 0 && out_kv_stride[i] % 8 == 0 && out_kv_stride[i] <= (int64_t)1 << 40, "strides must be non-negative multiples of 8 elements");
+        GPANN_REQUIRE(BlocksDisjoint(out_kv_stride, L->batch, keep, L->kv_heads, L->head_dim), "an output tensor overlaps itself");
+    }
+    GPANN_BLOCKS_ENTER(L, stream);
+    const BlocksArgs a = BlocksMakeArgs(L, nullptr, k, v, nullptr, 0);
+    if (a.B == 0) return GPANN_OK;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(BlocksEvictSelectKernel, dim3(a.Hkv, a.B), dim3(1024), 0, st, a, mass, keep, first, last, rows, count);
+    GPANN_HIP_TRY(hipGetLastError());
+    if (!k_out && !mass_out) return GPANN_OK;
+    const uint32_t chunks = L->head_dim / 8, kept = std::min(keep, L->kv_rows);
+    if (kept == 0) return GPANN_OK;
+    const uint64_t threads = (uint64_t)kept * a.Hkv * chunks;
+    int64_t zero[3] = {0, 0, 0};
+    const int64_t* os = out_kv_stride ? out_kv_stride : zero;
+    hipLaunchKernelGGL(BlocksEvictCopyKernel, dim3((uint32_t)std::min<uint64_t>((threads + 255) / 256, 1u << 20), a.B), dim3(256), 0, st, a, chunks, keep, rows, count, mass,
+                       static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out), os[0], os[1], os[2], mass_out);
+    GPANN_HIP_TRY(hipGetLastError());
+    return GPANN_OK;
+}
+
+}  // extern "C"
