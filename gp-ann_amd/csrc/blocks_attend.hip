@@ -1,5 +1,5 @@
 // blocks_attend.hip — attention over probed cache blocks, its gradients, and the attention weights of the cache rows (include/gpann_blocks.h).
-#include "blocks_tile.h"
+#include "blocks_walk.h"
 
 #include <algorithm>
 
@@ -82,17 +82,18 @@ __device__ __forceinline__ void BlocksAttendStep(const BlocksArgs& a, int visibl
         }
     }
     float best = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-    best = fmaxf(top, BlocksMaxOver4(best));
-    const float from = best == -inf ? 0.f : best;   // nothing seen yet: 2^(-inf - 0) = 0
-    const float shrink = BlocksExp2(top - from);
-    if (__ballot(best != top)) {
+    best = BlocksMaxOver4(best);
+    if (__ballot(best > top + kBlocksSlack)) {
+        best = fmaxf(top, best);
+        const float shrink = top == best ? 1.f : BlocksExp2(top - best);   // (top = best = -inf: nothing seen yet)
+        top = best;
         sum *= shrink;
 #pragma unroll
         for (int d = 0; d < DC; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[d][i] *= shrink;
     }
-    top = best;
+    const float from = top == -inf ? 0.f : top;   // 2^(-inf - 0) = 0
 #pragma unroll
     for (int y = 0; y < 2; ++y)
 #pragma unroll
@@ -114,6 +115,50 @@ __device__ __forceinline__ void BlocksStoreColumns(uint16_t* p, const uint32_t (
 #pragma unroll
     for (int i = 0; i < N; ++i) t.x[i] = w[i];
     *reinterpret_cast<Dwords*>(p) = t;
+}
+
+// All of a query row's probed rows from tile `u` to `end`, 32 a step
+template <bool BF16, int DC, bool AHEAD>
+__device__ __forceinline__ void BlocksAttendRange(const BlocksArgs& a, uint32_t h, int visible, int block, int64_t ko, int64_t vo, uint32_t u, uint32_t end,
+                                                  uint32_t lane, const u32x4_t (&q)[DC / 2], f32x4_t (&o)[DC], float& top, float& sum) {
+    BlocksCursor c(u, a.bs / 16);
+    if constexpr (AHEAD && DC <= 8) {   // the next step's rows are on their way while this one is multiplied
+        BlocksStep<BF16, DC> s0, s1;
+        BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u, lane, s0);
+        for (;;) {
+            const bool more = u + 2 < end;
+            if (more) BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u - 2, lane, s1);
+            BlocksAttendStep(a, visible, lane, s0, q, o, top, sum);
+            if (!more) break;
+            u += 2;
+            const bool again = u + 2 < end;
+            if (again) BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u - 2, lane, s0);
+            BlocksAttendStep(a, visible, lane, s1, q, o, top, sum);
+            if (!again) break;
+            u += 2;
+        }
+    } else {
+        for (; u < end; u += 2) {
+            BlocksStep<BF16, DC> s;
+            BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u, lane, s);
+            BlocksAttendStep(a, visible, lane, s, q, o, top, sum);
+        }
+    }
+}
+
+// a wavefront's sums in the column layout (slot d of lane column: dimension (4 g + i) * DC + d) -> out and lse of its rows
+template <bool BF16, int DC>
+__device__ __forceinline__ void BlocksAttendStore(const BlocksArgs& a, uint32_t b, uint32_t t, uint32_t head, uint32_t g, const f32x4_t (&o)[DC], float top, float sum,
+                                                  uint16_t* out, float* lse) {
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);   // (a NaN sum stays one)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t w[DC / 2];
+#pragma unroll
+        for (int c = 0; c < DC / 2; ++c) w[c] = BlocksPack<BF16>(o[2 * c][i] * inv, o[2 * c + 1][i] * inv);
+        BlocksStoreColumns<BF16, DC / 2>(out + b * a.os[0] + (int64_t)t * a.os[1] + head * a.os[2] + (g * 4 + i) * DC, w);
+    }
+    if (lse && g == 0) lse[((int64_t)b * a.Tq + t) * a.Hq + head] = sum == 0.f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
 }
 
 template <bool BF16, int DC>
@@ -147,44 +192,12 @@ __global__ void __launch_bounds__(512) BlocksAttendKernel(BlocksArgs a, uint32_t
         if (u < end) {
             u32x4_t q[DC / 2];
             BlocksLoadRows<DC / 2>(a.q + b * a.qs[0] + t * a.qs[1] + head * a.qs[2] + g * 8, q);
-            BlocksCursor c(u, tpb);
-            if constexpr (DC <= 8) {   // the next step's rows are on their way while this one is multiplied
-                BlocksStep<BF16, DC> s0, s1;
-                BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u, lane, s0);
-                for (;;) {
-                    const bool more = u + 2 < end;
-                    if (more) BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u - 2, lane, s1);
-                    BlocksAttendStep(a, visible, lane, s0, q, o, top, sum);
-                    if (!more) break;
-                    u += 2;
-                    const bool again = u + 2 < end;
-                    if (again) BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u - 2, lane, s0);
-                    BlocksAttendStep(a, visible, lane, s1, q, o, top, sum);
-                    if (!again) break;
-                    u += 2;
-                }
-            } else {
-                for (; u < end; u += 2) {
-                    BlocksStep<BF16, DC> s;
-                    BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u, lane, s);
-                    BlocksAttendStep(a, visible, lane, s, q, o, top, sum);
-                }
-            }
+            BlocksAttendRange<BF16, DC, true>(a, h, visible, block, ko, vo, u, end, lane, q, o, top, sum);
         }
     }
     sum = BlocksSumOver4(sum);
-    uint16_t* dst = out + b * a.os[0] + (int64_t)t * a.os[1];
     if (waves == 1) {
-        if (!live || r >= heads) return;
-        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);   // (a NaN sum stays one)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t w[DC / 2];
-#pragma unroll
-            for (int c = 0; c < DC / 2; ++c) w[c] = BlocksPack<BF16>(o[2 * c][i] * inv, o[2 * c + 1][i] * inv);
-            BlocksStoreColumns<BF16, DC / 2>(dst + head * a.os[2] + (g * 4 + i) * DC, w);
-        }
-        if (lse && g == 0) lse[((int64_t)b * a.Tq + t) * a.Hq + head] = sum == 0.f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
+        if (live && r < heads) BlocksAttendStore<BF16, DC>(a, b, t, head, g, o, top, sum, out, lse);
         return;
     }
     float* s_ml = s_join + 8 * 16 * D;
@@ -221,6 +234,277 @@ __global__ void __launch_bounds__(512) BlocksAttendKernel(BlocksArgs a, uint32_t
         const uint32_t head2 = h * a.G + mt2 * 16 + row;
         *reinterpret_cast<uint32_t*>(out + b * a.os[0] + (int64_t)t2 * a.os[1] + head2 * a.os[2] + c) = BlocksPack<BF16>(x * inv, y * inv);
         if (lse && c == 0) lse[((int64_t)b * a.Tq + t2) * a.Hq + head2] = total == 0.f ? -__builtin_inff() : (best + __log2f(total)) * kLn2;
+    }
+}
+
+// ---- forward, neighbouring query rows together ----------------------------------------------------------------------------------------------------
+// LDS addresses of a lane's part of a stage's operands, relative to the stage
+template <int DC>
+struct BlocksWalkAddresses {
+    uint32_t rows[DC / 2], turned[DC];   // by rows: step s of row lane % 16; transposed: 16 dimensions d of rows 4 g ..
+    __device__ __forceinline__ explicit BlocksWalkAddresses(uint32_t lane) {
+        using S = BlocksWalkShape<DC>;
+        const uint32_t r = lane & 15, g = lane >> 4, row = g * 4 + r / 4;
+#pragma unroll
+        for (uint32_t s = 0; s < DC / 2; ++s) rows[s] = (r * S::CPR + S::Slot(s * 4 + g, r)) * 16;
+#pragma unroll
+        for (uint32_t d = 0; d < DC; ++d) turned[d] = (row * S::CPR + S::Slot(d * 2 + (r & 3) / 2, row)) * 16 + (r & 1) * 8;
+    }
+};
+
+// NT tiles of 16 keys of the stage at LDS byte `at` against a wavefront's CT x 16 columns; `mask`: which of its query rows look at them.  Operands are read in
+// batches ahead of the products that need them (the scheduling barriers keep the compiler from pairing every read with its use, a full LDS latency each).
+// scale2 >= 0 (the sign is the queries').
+template <bool BF16, int DC, int CT, int NT>
+__device__ __forceinline__ void BlocksWalkAttend(float scale2, uint32_t tile0, const BlocksWalkAddresses<DC>& ad, uint32_t at, const int (&start)[4],
+                                                 const uint32_t (&mask)[4], const BlocksWalkColumns<CT>& col, uint32_t g4, const u32x4_t (&q)[CT][DC / 2],
+                                                 f32x4_t (&o)[CT][DC], float (&top)[CT], float (&sum)[CT]) {
+    using S = BlocksWalkShape<DC>;
+    constexpr uint32_t TILE = S::D * 32;   // bytes of 16 rows
+    constexpr int KS = DC / 2, BATCH = DC * CT > 8 ? 2 : NT;
+    const float inf = __builtin_inff();
+    f32x4_t x[CT][NT];
+#pragma unroll
+    for (int y0 = 0; y0 < NT; y0 += BATCH) {
+        u32x4_t k[BATCH][KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int y = 0; y < BATCH; ++y) k[y][s] = BlocksReadRow(at + ad.rows[s] + (tile0 + y0 + y) * TILE);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int y = 0; y < BATCH; ++y) x[c][y0 + y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int y = 0; y < BATCH; ++y) x[c][y0 + y] = BlocksMfma<BF16>(k[y][s], q[c][s], x[c][y0 + y]);
+    }
+    u32x2_t v[DC][2];
+#pragma unroll
+    for (int d = 0; d < DC; ++d)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) v[d][y] = BlocksReadTransposed(at + ad.turned[d] + S::TENSOR + (tile0 + y) * TILE);
+    __builtin_amdgcn_sched_barrier(0);
+    bool plain = true;   // every column looks at every key
+#pragma unroll
+    for (int y = 0; y < NT; ++y) plain = plain && mask[tile0 + y] == col.full && start[tile0 + y] + 16 <= col.seen_by_all;
+    float from[CT][NT], best[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        best[c] = -inf;
+        if (plain) {
+#pragma unroll
+            for (int y = 0; y < NT; ++y) {
+                from[c][y] = 0.f;
+                best[c] = fmaxf(best[c], fmaxf(fmaxf(x[c][y][0], x[c][y][1]), fmaxf(x[c][y][2], x[c][y][3])));
+            }
+        } else {
+#pragma unroll
+            for (int y = 0; y < NT; ++y) {
+                const bool member = (mask[tile0 + y] >> col.in[c]) & 1;
+                if (start[tile0 + y] + 16 > col.seen_by_all) {
+                    const int limit = col.visible[c] - start[tile0 + y];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[c][y][i] = (int)g4 + i < limit ? x[c][y][i] : -inf;
+                }
+                from[c][y] = member ? 0.f : inf;
+                const float most = fmaxf(fmaxf(x[c][y][0], x[c][y][1]), fmaxf(x[c][y][2], x[c][y][3]));
+                best[c] = fmaxf(best[c], member ? most : -inf);
+            }
+        }
+        best[c] = BlocksMaxOver4(best[c]) * scale2;
+    }
+    bool raise = false;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) raise = raise || best[c] > top[c] + kBlocksSlack;
+    if (__ballot(raise)) {
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            best[c] = fmaxf(top[c], best[c]);
+            const float shrink = top[c] == best[c] ? 1.f : BlocksExp2(top[c] - best[c]);
+            top[c] = best[c];
+            sum[c] *= shrink;
+#pragma unroll
+            for (int d = 0; d < DC; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[c][d][i] *= shrink;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        const float base = top[c] == -inf ? 0.f : top[c];
+#pragma unroll
+        for (int y = 0; y < NT; ++y) {
+            const float less = -(from[c][y] + base);   // -inf: a tile that the column does not look at
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[c][y][i] = BlocksExp2(__builtin_fmaf(x[c][y][i], scale2, less));
+                sum[c] += x[c][y][i];
+            }
+        }
+    }
+#pragma unroll
+    for (int z = 0; z < NT / 2; ++z) {
+        u32x2_t next[DC][2];
+        if (z + 1 < NT / 2) {
+#pragma unroll
+            for (int d = 0; d < DC; ++d)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) next[d][y] = BlocksReadTransposed(at + ad.turned[d] + S::TENSOR + (tile0 + 2 * z + 2 + y) * TILE);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            const u32x4_t p = BlocksPackOperand<BF16>(x[c][2 * z], x[c][2 * z + 1]);
+#pragma unroll
+            for (int d = 0; d < DC; ++d) o[c][d] = BlocksMfma<BF16>(u32x4_t{v[d][0][0], v[d][0][1], v[d][1][0], v[d][1][1]}, p, o[c][d]);
+        }
+        if (z + 1 < NT / 2)
+#pragma unroll
+            for (int d = 0; d < DC; ++d)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) v[d][y] = next[d][y];
+    }
+}
+
+template <bool BF16, int DC, int CT>
+__global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint32_t tpw, uint32_t mtiles, uint32_t tiles, uint16_t* __restrict__ out,
+                                                              float* __restrict__ lse) {
+    TakeWholeRegisterFile();
+    using S = BlocksWalkShape<DC>;
+    constexpr int KS = DC / 2;
+    extern __shared__ __attribute__((aligned(16))) char s_walk[];   // stages, tables
+    __shared__ uint32_t s_count, s_scratch[8][64];
+    const BlocksWalkTables<DC> tab(s_walk);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    uint32_t pair, tile;
+    if (!BlocksPairOf(blockIdx.x, a.B * a.Hkv, tiles, pair, tile)) return;
+    BlocksWalkRows w;
+    w.b = pair / a.Hkv;
+    w.h = pair % a.Hkv;
+    w.wt0 = (tiles - 1 - tile) * 8;   // the rows with the longest walks first
+    w.tpw = tpw;
+    w.mtiles = mtiles;
+    w.n = BlocksKvLen(a, w.b);
+    w.m = BlocksQLen(a, w.b);
+    if ((int)w.FirstRow(w.wt0) >= w.m) return;
+    const BlocksWalkColumns<CT> col(a, w, wave, r);
+    const uint32_t blocks = ((uint32_t)BlocksVisible(a, w.n, w.m, (int)w.EndRow() - 1) + a.bs - 1) / a.bs, tpb = a.bs / 16;
+
+    // a negative scale is the queries' sign, a zero one makes them zero: the walk's own scale is positive
+    const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);
+    u32x4_t q[CT][KS];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        BlocksLoadRows<KS>(a.q + w.b * a.qs[0] + (int64_t)col.Row(w, c) * a.qs[1] + col.head[c] * a.qs[2] + g * 8, q[c]);
+        if (a.scale2 <= 0.f)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) q[c][s] = a.scale2 == 0.f ? u32x4_t{0u, 0u, 0u, 0u} : q[c][s] ^ 0x80008000u;
+    }
+    const BlocksWalkAddresses<DC> ad(lane);
+    f32x4_t o[CT][DC];
+    float top[CT], sum[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+#pragma unroll
+        for (int d = 0; d < DC; ++d) o[c][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        top[c] = -__builtin_inff();
+        sum[c] = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[c][s]));   // here, not in the loop, is where these loads are waited for
+    }
+    const BlocksWalker<DC> walk(a, wave, lane);
+    const uint32_t lds = BlocksLdsAddress(s_walk);
+
+    for (uint32_t window = 0; window < blocks; window += S::WINDOW) {
+        const uint32_t in_window = min(S::WINDOW, blocks - window);
+        const uint32_t units = BlocksWalkList<DC>(a, w, window, in_window, tab, &s_count) * tpb, stages = (units + 3) / 4;
+        BlocksWalkStage d[S::BUFFERS];   // of stages s, s + 1, ...
+#pragma unroll
+        for (uint32_t s = 0; s + 1 < S::BUFFERS; ++s)
+            if (s < stages) {
+                d[s] = walk.Describe(a, w, tab, window, s, units, col.seen_by_any);
+                walk.Load(d[s], lds + s * S::STAGE);
+            }
+        uint32_t buf = 0;
+        for (uint32_t s = 0; s < stages; ++s) {
+            const bool more = s + S::BUFFERS - 1 < stages;
+            if (more) d[S::BUFFERS - 1] = walk.Describe(a, w, tab, window, s + S::BUFFERS - 1, units, col.seen_by_any);
+            if (S::BUFFERS > 2 && s + 1 < stages)
+                BlocksDmaWait<(S::BUFFERS - 2) * S::LOADS>();
+            else
+                BlocksDmaWait<0>();
+            BlocksStageBarrier();   // stage s has landed, and nobody reads stage s - 1 any more
+            if (more) walk.Load(d[S::BUFFERS - 1], lds + (buf == 0 ? S::BUFFERS - 1 : buf - 1) * S::STAGE);
+            int start[4];
+            uint32_t mask[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                start[y] = __builtin_amdgcn_readlane(d[0].start, y);
+                mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)d[0].mask, y);
+            }
+            const uint32_t at = lds + buf * S::STAGE;
+            const bool first = mask[0] | mask[1], second = mask[2] | mask[3];
+            if (first && second)
+                BlocksWalkAttend<BF16, DC, CT, 4>(scale2, 0, ad, at, start, mask, col, g * 4, q, o, top, sum);
+            else if (first)
+                BlocksWalkAttend<BF16, DC, CT, 2>(scale2, 0, ad, at, start, mask, col, g * 4, q, o, top, sum);
+            else if (second)
+                BlocksWalkAttend<BF16, DC, CT, 2>(scale2, 2, ad, at, start, mask, col, g * 4, q, o, top, sum);
+#pragma unroll
+            for (uint32_t y = 0; y + 1 < S::BUFFERS; ++y) d[y] = d[y + 1];
+            buf = buf + 1 == S::BUFFERS ? 0 : buf + 1;
+        }
+        __syncthreads();
+    }
+    // A value that is not finite may have met the weight 0 of a row that does not look at it.  Such columns are rare: their query rows are done again one by
+    // one, where nothing but what a row sees takes part.
+    float bad = 0.f;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        sum[c] = BlocksSumOver4(sum[c]);
+        bad += sum[c] * 0.f;
+#pragma unroll
+        for (int d = 0; d < DC; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bad += o[c][d][i] * 0.f;
+    }
+    if (__ballot(bad != 0.f)) {
+        const uint32_t first_head = w.h * a.G + col.mt * 16 * CT, heads = mtiles > 1 ? col.cols : a.G;
+        for (uint32_t x = 0; x < col.rows * ((heads + 15) / 16); ++x) {
+            const uint32_t t = col.t0 + x % col.rows, h0 = x / col.rows * 16, some = min(16u, heads - h0), head = first_head + h0 + min(r, some - 1);
+            const int vis = BlocksVisible(a, w.n, w.m, (int)t);
+            top[0] = -__builtin_inff();
+            sum[0] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DC; ++d) o[0][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            int block;
+            int64_t ko, vo;
+            const uint32_t count = vis > 0 ? BlocksGatherProbes(a, a.probes + (((int64_t)w.b * a.Tq + t) * a.Hkv + w.h) * a.P, w.b, vis, s_scratch[wave], lane, block, ko, vo) : 0;
+            if (count) {
+                BlocksLoadRows<KS>(a.q + w.b * a.qs[0] + (int64_t)t * a.qs[1] + head * a.qs[2] + g * 8, q[0]);
+                BlocksAttendRange<BF16, DC, false>(a, w.h, vis, block, ko, vo, 0, count * tpb, lane, q[0], o[0], top[0], sum[0]);
+            }
+            sum[0] = BlocksSumOver4(sum[0]);
+            if (r < some) BlocksAttendStore<BF16, DC>(a, w.b, t, head, g, o[0], top[0], sum[0], out, lse);
+        }
+        return;
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        if (!col.live[c]) continue;
+        const float inv = sum[c] > 0.f ? 1.f / sum[c] : 0.f;
+        const uint32_t t = col.t0 + col.in[c];
+        uint16_t* dst = out + w.b * a.os[0] + (int64_t)t * a.os[1] + col.head[c] * a.os[2] + g * 4;
+#pragma unroll
+        for (int d = 0; d < DC; ++d)
+            *reinterpret_cast<u32x2_t*>(dst + d * 16) =
+                u32x2_t{BlocksPack<BF16>(o[c][d][0] * inv, o[c][d][1] * inv), BlocksPack<BF16>(o[c][d][2] * inv, o[c][d][3] * inv)};
+        if (lse && g == 0) lse[((int64_t)w.b * a.Tq + t) * a.Hq + col.head[c]] = sum[c] == 0.f ? -__builtin_inff() : (top[c] + __log2f(sum[c])) * kLn2;
     }
 }
 
@@ -697,10 +981,24 @@ static gpann_status Launch(K kernel, uint64_t grid, size_t lds, hipStream_t st, 
     return GPANN_OK;
 }
 
+template <bool BF16, int DC, int CT>
+static gpann_status AttendWalk(const BlocksArgs& a, uint16_t* out, float* lse, hipStream_t st) {
+    const uint32_t cols = 16 * CT, mtiles = (a.G + cols - 1) / cols, tpw = std::max(1u, cols / a.G);
+    const uint64_t waves = mtiles > 1 ? (uint64_t)a.Tq * mtiles : (a.Tq + tpw - 1) / tpw, tiles = (waves + 7) / 8;
+    return Launch(BlocksAttendWalkKernel<BF16, DC, CT>, BlocksPairGrid((uint64_t)a.B * a.Hkv, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, lse);
+}
+
 template <bool BF16, int DC>
 static gpann_status Attend(const BlocksArgs& a, uint16_t* out, float* lse, hipStream_t st) {
     const uint32_t mtiles = (a.G + 15) / 16;
     const uint64_t tasks = (uint64_t)a.Tq * mtiles, pairs = (uint64_t)a.B * a.Hkv;
+    if (a.Tq > 1) {
+        // 32 columns a wavefront read LDS half as often for each, but make half the workgroups (one per CU at a time) of a larger union: 8192 rows x 32 heads,
+        // 1024 workgroups of 32 columns, 536 us against 588; 777 rows x 12 heads, 120 workgroups, 152 us against 103.  (Wide heads have no registers for it.)
+        if constexpr (DC <= 8)
+            if (pairs * ((tasks * a.G / mtiles + 255) / 256) >= 512) return AttendWalk<BF16, DC, 2>(a, out, lse, st);
+        return AttendWalk<BF16, DC, 1>(a, out, lse, st);
+    }
     // few query rows: their keys are divided over wavefronts until the chip's 2048 have something to do
     uint32_t waves = 1;
     while (waves < 8 && pairs * tasks * waves < 2048) waves *= 2;

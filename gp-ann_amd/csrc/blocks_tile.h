@@ -72,14 +72,25 @@ __device__ __forceinline__ u32x4_t BlocksColumn(const uint32_t (&w)[8][N], int d
 }
 
 __device__ __forceinline__ float BlocksExp2(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32: 1 ulp, -inf -> 0
-__device__ __forceinline__ float BlocksMaxOver4(float x) {                                    // over the four lanes that hold a C column
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
+// over the four lanes that hold a C column: v_permlane32_swap / v_permlane16_swap of a register with itself put a lane's value and that of lane ^ 32 (^ 16)
+// side by side, without the trip through LDS of a shuffle
+__device__ __forceinline__ float BlocksMaxOver4(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto y = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])));
+    const auto z = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return fmaxf(__uint_as_float(z[0]), __uint_as_float(z[1]));
 }
 __device__ __forceinline__ float BlocksSumOver4(float x) {
-    x = x + __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+    const uint32_t u = __float_as_uint(x);
+    const auto y = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(__uint_as_float(y[0]) + __uint_as_float(y[1]));
+    const auto z = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return __uint_as_float(z[0]) + __uint_as_float(z[1]);
 }
+// The running maximum follows the true one only when that is more than this many powers of two ahead: weights then reach 2^8 instead of 1, which 16-bit
+// floats hold as exactly, and the accumulators are hardly ever rescaled.
+constexpr float kBlocksSlack = 8.f;
 __device__ __forceinline__ int64_t BlocksReadLane64(int64_t x, uint32_t lane) {
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, (int)lane);
     const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)x >> 32), (int)lane);

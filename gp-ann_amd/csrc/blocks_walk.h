@@ -1,0 +1,215 @@
+// blocks_walk.h — how a workgroup walks the blocks that neighbouring query rows probe (blocks_attend.hip, blocks_grad.hip).
+//
+// A wavefront's 16 CT matrix columns are the heads of a group of max(1, 16 CT / G) neighbouring query rows; a workgroup holds eight wavefronts.  The walk
+// goes over the UNION of the blocks its query rows probe, in block order: every row of K and V enters LDS once for the workgroup, and a wavefront multiplies
+// the blocks that one of its own query rows probes.  Neighbouring rows share most of their probes (their own block, the first one, what their text is about),
+// so the union is far smaller than the sum; a 16-column tile costs the same whether one or all of its rows want the block.
+//
+// Rows go to LDS by DMA (no registers, issued stages ahead), 64 rows of K and of V a stage.  The 16-byte chunks of a row are permuted by a function of the
+// row such that both ways of reading are free of bank conflicts: by rows (ds_read_b128: eight rows, one chunk) and transposed (ds_read_b64_tr_b16: four
+// rows, two neighbouring chunks per 16 lanes).
+#pragma once
+
+#include "blocks_tile.h"
+
+namespace gpann {
+
+template <int DC>
+struct BlocksWalkShape {
+    static constexpr uint32_t D = DC * 16, CPR = D / 8, ROWS = 64, TENSOR = ROWS * D * 2, STAGE = 2 * TENSOR;
+    static constexpr uint32_t BUFFERS = D <= 128 ? 3 : 2, LOADS = CPR / 4;   // LOADS: DMA instructions of a wavefront per stage
+    static constexpr uint32_t WINDOW = D <= 128 ? 1024 : 512;   // blocks that LDS has room for at a time
+    static constexpr size_t LDS = (size_t)BUFFERS * STAGE + WINDOW * (sizeof(uint4) + 32 + 4);
+
+    // Slot of a row's chunk.  LDS serves 256 bytes a cycle over 64 banks, so sixteen lanes' chunks (by rows: sixteen rows, one chunk) and thirty-two lanes'
+    // half chunks (transposed: eight rows, two neighbouring chunks) have to lie in sixteen different slots modulo 16; a row begins CPR slots after the one before.
+    static __device__ __forceinline__ uint32_t Turn(uint32_t row) {
+        if (CPR == 12) return ((row >> 2) & 1) * 2 + ((row >> 3) & 1);
+        if (CPR % 16 == 8) return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
+        return ((row & 7) << 1) | ((row >> 3) & 1);
+    }
+    static __device__ __forceinline__ uint32_t Slot(uint32_t chunk, uint32_t row) {
+        if ((CPR & (CPR - 1)) == 0) return chunk ^ Turn(row);
+        const uint32_t s = chunk + Turn(row);
+        return s >= CPR ? s - CPR : s;
+    }
+    static __device__ __forceinline__ uint32_t Chunk(uint32_t slot, uint32_t row) {
+        if ((CPR & (CPR - 1)) == 0) return slot ^ Turn(row);
+        const uint32_t t = Turn(row);
+        return slot >= t ? slot - t : slot + CPR - t;
+    }
+};
+
+// One LDS-DMA wave-instruction: 64 lanes x 16 bytes from base + offset to LDS bytes [lds, lds + 1024).  The compiler neither sees the bytes nor counts
+// it in vmcnt: BlocksDmaWait comes before the barrier that publishes them (waits of its own only get longer by it).
+__device__ __forceinline__ void BlocksDma(uint64_t base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "m0", "memory");
+}
+template <int LEFT>
+__device__ __forceinline__ void BlocksDmaWait() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LEFT) : "memory");
+}
+// every wavefront has its share of a stage in LDS and has read what it needs of the stage before
+__device__ __forceinline__ void BlocksStageBarrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+__device__ __forceinline__ uint32_t BlocksLdsAddress(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+// lane l of 16: address of (row l / 4, four elements l % 4) of a 4 x 16 tile -> column l of its four rows
+__device__ __forceinline__ u32x2_t BlocksReadTransposed(uint32_t lds) {
+    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)lds));
+}
+__device__ __forceinline__ u32x4_t BlocksReadRow(uint32_t lds) { return *(__attribute__((address_space(3))) const u32x4_t*)lds; }
+
+// What a workgroup's query rows are
+struct BlocksWalkRows {
+    uint32_t b, h, wt0, tpw, mtiles;   // wavefront w: column tile wt0 + w; tpw query rows each, or one of mtiles tiles of a row's heads
+    int n, m;
+    __device__ __forceinline__ uint32_t FirstRow(uint32_t wt) const { return mtiles > 1 ? wt / mtiles : wt * tpw; }
+    __device__ __forceinline__ uint32_t EndRow() const { return min((uint32_t)m, mtiles > 1 ? FirstRow(wt0 + 7) + 1 : FirstRow(wt0 + 8)); }
+};
+// ... a wavefront's
+template <int CT>
+struct BlocksWalkColumns {
+    uint32_t t0, rows, full;          // first query row, how many are live, a bit for each
+    int seen_by_all, seen_by_any;     // cache rows (a prefix) that its first and its last query row see
+    uint32_t cols, mt;                // columns in use
+    uint32_t in[CT], head[CT];        // this lane's columns: query row - t0, query head
+    int visible[CT];
+    bool live[CT];
+    __device__ __forceinline__ BlocksWalkColumns(const BlocksArgs& a, const BlocksWalkRows& w, uint32_t wave, uint32_t r) {
+        t0 = w.FirstRow(w.wt0 + wave);
+        mt = w.mtiles > 1 ? (w.wt0 + wave) % w.mtiles : 0;
+        cols = w.mtiles > 1 ? min(16u * CT, a.G - mt * 16 * CT) : w.tpw * a.G;
+        rows = (int)t0 < w.m ? min(w.tpw, (uint32_t)w.m - t0) : 0;
+        full = rows == 32 ? ~0u : (1u << rows) - 1;
+        seen_by_all = rows ? BlocksVisible(a, w.n, w.m, (int)t0) : 0;
+        seen_by_any = rows ? BlocksVisible(a, w.n, w.m, (int)(t0 + rows - 1)) : 0;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            const uint32_t col = min(c * 16 + r, cols - 1);
+            in[c] = w.mtiles > 1 ? 0 : col / a.G;
+            head[c] = w.h * a.G + (w.mtiles > 1 ? mt * 16 * CT + col : col % a.G);
+            live[c] = in[c] < rows && c * 16 + r < cols;
+            visible[c] = in[c] < rows ? BlocksVisible(a, w.n, w.m, (int)(t0 + in[c])) : 0;
+        }
+    }
+    __device__ __forceinline__ uint32_t Row(const BlocksWalkRows& w, int c) const { return min(t0 + in[c], (uint32_t)w.m - 1); }
+};
+
+// LDS of a walk behind the stages
+template <int DC>
+struct BlocksWalkTables {
+    uint4* address;    // [WINDOW] of the list's blocks: byte addresses of the first row of the head in K and V
+    uint32_t* masks;   // [WINDOW][8] which query rows of a wavefront probe a block
+    int* list;         // [WINDOW] the blocks with any, ascending
+    __device__ __forceinline__ explicit BlocksWalkTables(char* lds) {
+        using S = BlocksWalkShape<DC>;
+        address = reinterpret_cast<uint4*>(lds + S::BUFFERS * S::STAGE);
+        masks = reinterpret_cast<uint32_t*>(address + S::WINDOW);
+        list = reinterpret_cast<int*>(masks + S::WINDOW * 8);
+    }
+};
+
+// Fills the tables for the blocks [window, window + in_window) and returns the length of the list.  Ends with a barrier.
+template <int DC>
+__device__ __forceinline__ uint32_t BlocksWalkList(const BlocksArgs& a, const BlocksWalkRows& w, uint32_t window, uint32_t in_window, const BlocksWalkTables<DC>& tab,
+                                                   uint32_t* s_count) {
+    const uint32_t tid = threadIdx.x;
+    for (uint32_t i = tid; i < in_window * 8; i += 512) tab.masks[i] = 0;
+    __syncthreads();
+    const uint32_t t0 = w.FirstRow(w.wt0), t1 = w.EndRow();
+    const uint32_t entries = t1 > t0 ? (t1 - t0) * a.P : 0;
+    for (uint32_t i = tid; i < entries; i += 512) {
+        const uint32_t t = t0 + i / a.P;
+        const int p = a.probes[(((int64_t)w.b * a.Tq + t) * a.Hkv + w.h) * a.P + i % a.P];
+        if (p < (int)window || (uint32_t)p >= window + in_window || (int64_t)p * a.bs >= BlocksVisible(a, w.n, w.m, (int)t)) continue;
+        uint32_t* row = tab.masks + ((uint32_t)p - window) * 8;
+        if (w.mtiles > 1) {
+            for (uint32_t x = t * w.mtiles; x < (t + 1) * w.mtiles; ++x)
+                if (x >= w.wt0 && x < w.wt0 + 8) row[x - w.wt0] = 1;
+        } else {
+            atomicOr(row + (t - t0) / w.tpw, 1u << (t - t0) % w.tpw);
+        }
+    }
+    __syncthreads();
+    if (tid < 64) {
+        uint32_t at = 0;
+        for (uint32_t j0 = 0; j0 < in_window; j0 += 64) {
+            const uint32_t j = j0 + tid;
+            bool any = false;
+            int64_t ko = 0, vo = 0;
+            if (j < in_window) {
+                const uint4 x = *reinterpret_cast<const uint4*>(tab.masks + j * 8), y = *reinterpret_cast<const uint4*>(tab.masks + j * 8 + 4);
+                any = (x.x | x.y | x.z | x.w | y.x | y.y | y.z | y.w) != 0 && BlocksBase(a, w.b, (int)(window + j), ko, vo);
+            }
+            const uint64_t votes = __ballot(any);
+            if (any) {
+                const uint32_t e = at + (uint32_t)__popcll(votes & ((1ull << tid) - 1));
+                const uint64_t k = (uint64_t)(a.k + ko + w.h * a.ks[2]), v = (uint64_t)(a.v + vo + w.h * a.vs[2]);
+                tab.address[e] = uint4{(uint32_t)k, (uint32_t)(k >> 32), (uint32_t)v, (uint32_t)(v >> 32)};
+                tab.list[e] = (int)(window + j);
+            }
+            at += (uint32_t)__popcll(votes);
+        }
+        if (tid == 0) *s_count = at;
+    }
+    __syncthreads();
+    return *s_count;
+}
+
+// The four 16-row tiles of a stage, tile y in lane y
+struct BlocksWalkStage {
+    uint4 address;     // of its block
+    int row, last;     // its first row in the block; the last row of the block that the sequence has
+    int start;         // its position
+    uint32_t mask;     // which query rows of this wavefront look at it
+};
+
+// The walk's bookkeeping and its DMA side: which rows and chunks of a tile a lane loads is the same in every stage
+template <int DC>
+struct BlocksWalker {
+    using S = BlocksWalkShape<DC>;
+    uint32_t row[S::LOADS], chunk[S::LOADS];   // row in its tile, byte offset of the chunk in the row
+    uint32_t wave, lane, tpb, inverse, krow, vrow;
+    __device__ __forceinline__ BlocksWalker(const BlocksArgs& a, uint32_t wave_, uint32_t lane_) : wave(wave_), lane(lane_), tpb(a.bs / 16) {
+        inverse = tpb > 1 ? 0xFFFFFFFFu / tpb + 1 : 0;
+        krow = (uint32_t)a.ks[1] * 2;
+        vrow = (uint32_t)a.vs[1] * 2;
+#pragma unroll
+        for (uint32_t x = 0; x < S::LOADS; ++x) {
+            const uint32_t at = (wave + 8 * x) % S::CPR * 64 + lane, r = at / S::CPR;
+            row[x] = r % 16;
+            chunk[x] = S::Chunk(at % S::CPR, r) * 16;
+        }
+    }
+    // `seen`: rows that the last query row of this wavefront sees (a prefix)
+    __device__ __forceinline__ BlocksWalkStage Describe(const BlocksArgs& a, const BlocksWalkRows& w, const BlocksWalkTables<DC>& tab, uint32_t window, uint32_t s,
+                                                        uint32_t units, int seen) const {
+        BlocksWalkStage d;
+        const uint32_t unit = 4 * s + (lane & 3), in = min(unit, units - 1), e = inverse ? __umulhi(in, inverse) : in;   // in / tpb, exact below 2^16
+        const int block = tab.list[e];
+        d.address = tab.address[e];
+        d.row = (int)(in - e * tpb) * 16;
+        d.last = w.n - 1 - block * (int)a.bs;
+        d.start = block * (int)a.bs + d.row;
+        d.mask = tab.masks[(block - (int)window) * 8 + (int)wave];
+        if (unit >= units || d.start >= seen) d.mask = 0;
+        return d;
+    }
+    __device__ __forceinline__ void Load(const BlocksWalkStage& d, uint32_t to) const {
+#pragma unroll
+        for (uint32_t x = 0; x < S::LOADS; ++x) {
+            const uint32_t j = wave + 8 * x;
+            const bool value = j >= S::CPR;
+            const int tile = (int)(j % S::CPR / (S::CPR / 4));   // 16 rows are CPR / 4 instructions
+            const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(value ? d.address.z : d.address.x), tile);
+            const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(value ? d.address.w : d.address.y), tile);
+            const int first = __builtin_amdgcn_readlane(d.row, tile), last = __builtin_amdgcn_readlane(d.last, tile);
+            const uint32_t r = (uint32_t)min(first + (int)row[x], last);   // rows past the sequence's end are not read
+            BlocksDma(((uint64_t)hi << 32) | lo, r * (value ? vrow : krow) + chunk[x], to + (value ? S::TENSOR : 0) + j % S::CPR * 1024);
+        }
+    }
+};
+
+}  // namespace gpann
