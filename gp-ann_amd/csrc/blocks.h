@@ -97,6 +97,48 @@ __device__ __forceinline__ bool BlocksPairOf(uint32_t id, uint32_t pairs, uint32
     tile = rest % tiles;
     return pair < pairs;
 }
+// bits (and counts, may be null) of the probes of every block; both cleared first
+gpann_status BlocksMarkProbes(const BlocksArgs& a, uint32_t words, uint32_t* bits, uint32_t* counts, hipStream_t st);
+size_t BlocksBackwardSpace(const BlocksArgs& a, uint32_t d);
+
+inline bool BlocksAligned(uintptr_t n, const void* p) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+inline gpann_status BlocksCheckWorkspace(const void* p, size_t have, size_t need) {
+    if (need == 0) return GPANN_OK;
+    if (have < need) {
+        SetLastError("invalid argument: the workspace has %zu bytes, the call needs %zu", have, need);
+        return GPANN_ERR_INVALID;
+    }
+    GPANN_REQUIRE(p && BlocksAligned(16, p), "the workspace is null or not 16-byte aligned");
+    return GPANN_OK;
+}
+
+// workgroups of 512 threads
+template <typename K, typename... A>
+inline gpann_status BlocksLaunch(K kernel, uint64_t grid, size_t lds, hipStream_t st, A... args) {
+    if (grid > 0x7fffffffull / 512 * 2) {   // (a launch has fewer than 2^32 threads)
+        SetLastError("the call needs %llu workgroups of 512 threads", (unsigned long long)grid);
+        return GPANN_ERR_UNSUPPORTED;
+    }
+    if (lds > 32 * 1024) GPANN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(512), lds, st, args...);
+    GPANN_HIP_TRY(hipGetLastError());
+    return GPANN_OK;
+}
+
+// head_dim and element type -> template arguments
+#define GPANN_BLOCKS_DISPATCH(L, fn, ...)                                                                                                   \
+    do {                                                                                                                                    \
+        const bool bf16 = (L)->dtype == GPANN_BLOCKS_BF16;                                                                                  \
+        switch ((L)->head_dim) {                                                                                                            \
+            case 64: return bf16 ? fn<true, 4>(__VA_ARGS__) : fn<false, 4>(__VA_ARGS__);                                                    \
+            case 96: return bf16 ? fn<true, 6>(__VA_ARGS__) : fn<false, 6>(__VA_ARGS__);                                                    \
+            case 128: return bf16 ? fn<true, 8>(__VA_ARGS__) : fn<false, 8>(__VA_ARGS__);                                                   \
+            case 192: return bf16 ? fn<true, 12>(__VA_ARGS__) : fn<false, 12>(__VA_ARGS__);                                                 \
+            default: return bf16 ? fn<true, 16>(__VA_ARGS__) : fn<false, 16>(__VA_ARGS__);                                                  \
+        }                                                                                                                                   \
+    } while (0)
+
 inline uint64_t BlocksPairGrid(uint64_t pairs, uint64_t tiles) { return (pairs + 7) / 8 * 8 * tiles; }
 
 }  // namespace gpann

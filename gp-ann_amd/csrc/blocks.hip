@@ -313,9 +313,6 @@ __global__ void __launch_bounds__(256) BlocksEvictCopyKernel(BlocksArgs a, uint3
     }
 }
 
-static bool Aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-static bool Aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
-
 }  // namespace gpann
 
 using namespace gpann;
@@ -325,7 +322,7 @@ extern "C" {
 gpann_status gpann_blocks_summarize(const gpann_blocks_layout* L, const void* k, uint32_t new_rows, float* summary, void* stream) {
     GPANN_TRY(BlocksCheckLayout(L));
     GPANN_REQUIRE(k && summary, "a tensor is null");
-    GPANN_REQUIRE(Aligned16(k) && Aligned16(summary), "tensors must be 16-byte aligned");
+    GPANN_REQUIRE(BlocksAligned(16, k) && BlocksAligned(16, summary), "tensors must be 16-byte aligned");
     GPANN_BLOCKS_ENTER(L, stream);
     const BlocksArgs a = BlocksMakeArgs(L, nullptr, k, nullptr, nullptr, 0);
     if (a.B == 0 || a.nblk == 0) return GPANN_OK;
@@ -349,7 +346,7 @@ gpann_status gpann_blocks_route(const gpann_blocks_layout* L, const void* q, con
     (void)workspace_bytes;
     GPANN_TRY(BlocksCheckLayout(L));
     GPANN_REQUIRE(q && summary && probes, "a tensor is null");
-    GPANN_REQUIRE(Aligned16(q) && Aligned16(summary) && Aligned4(probes), "q and summary must be 16-byte aligned, probes 4-byte aligned");
+    GPANN_REQUIRE(BlocksAligned(16, q) && BlocksAligned(16, summary) && BlocksAligned(4, probes), "q and summary must be 16-byte aligned, probes 4-byte aligned");
     GPANN_REQUIRE(nprobe >= 1 && nprobe <= GPANN_BLOCKS_MAX_PROBE, "nprobe must be 1 .. GPANN_BLOCKS_MAX_PROBE");
     GPANN_REQUIRE(first <= nprobe && last <= nprobe - first, "first + last must not exceed nprobe");
     GPANN_REQUIRE(last >= 1 || !(L->flags & GPANN_BLOCKS_CAUSAL), "a causal route needs last >= 1");
@@ -376,8 +373,8 @@ gpann_status gpann_blocks_evict(const gpann_blocks_layout* L, const void* k, con
     GPANN_REQUIRE(mass && rows && count, "a tensor is null");
     GPANN_REQUIRE((k_out == nullptr) == (v_out == nullptr), "k_out and v_out must be given together");
     GPANN_REQUIRE(k_out == nullptr || (k && v && out_kv_stride), "a tensor is null");
-    GPANN_REQUIRE(Aligned16(k) && Aligned16(v) && Aligned16(k_out) && Aligned16(v_out), "k, v, k_out and v_out must be 16-byte aligned");
-    GPANN_REQUIRE(Aligned4(mass) && Aligned4(rows) && Aligned4(count) && Aligned4(mass_out), "tensors must be 4-byte aligned");
+    GPANN_REQUIRE(BlocksAligned(16, k) && BlocksAligned(16, v) && BlocksAligned(16, k_out) && BlocksAligned(16, v_out), "k, v, k_out and v_out must be 16-byte aligned");
+    GPANN_REQUIRE(BlocksAligned(4, mass) && BlocksAligned(4, rows) && BlocksAligned(4, count) && BlocksAligned(4, mass_out), "tensors must be 4-byte aligned");
     GPANN_REQUIRE(keep >= 1 && keep <= (1u << 24), "keep must be 1 .. 2^24");
     GPANN_REQUIRE(first <= keep && last <= keep - first, "first + last must not exceed keep");
     GPANN_REQUIRE(mass_out == nullptr || mass_out != mass, "mass_out must not be mass");

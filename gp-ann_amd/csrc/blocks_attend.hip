@@ -5,8 +5,6 @@
 
 namespace gpann {
 
-constexpr uint32_t kRange = 2048;   // query rows whose list a workgroup of a key-stationary kernel holds at a time
-
 // ---- forward --------------------------------------------------------------------------------------------------------------------------------
 // One pass over the probed rows with a running maximum and sum per query row, in powers of two (softmax(x) = 2^(x log2 e - max) / sum).  A wavefront works
 // on one query row's heads of a group (at most 16: the columns of the matrix tiles) and takes 32 keys a step: X^T = K Q^T, then O^T += V^T P^T, both
@@ -18,18 +16,6 @@ struct BlocksStep {
     uint32_t v[8][N];
     int start[2];     // position of the tiles' first rows
     bool second;      // the second tile is a tile of the range
-};
-
-// unit `u` of a query row's tiles: probed block u / tpb, tile u % tpb of it
-struct BlocksCursor {
-    uint32_t slot, sub, tpb;
-    __device__ __forceinline__ BlocksCursor(uint32_t u, uint32_t tiles_per_block) : slot(u / tiles_per_block), sub(u % tiles_per_block), tpb(tiles_per_block) {}
-    __device__ __forceinline__ void Next() {
-        if (++sub == tpb) {
-            sub = 0;
-            ++slot;
-        }
-    }
 };
 
 template <bool BF16, int DC>
@@ -107,16 +93,6 @@ __device__ __forceinline__ void BlocksAttendStep(const BlocksArgs& a, int visibl
     for (int d = 0; d < DC; ++d) o[d] = BlocksMfma<BF16>(BlocksColumn<DC / 2>(st.v, d), p, o[d]);
 }
 
-template <bool BF16, int N>
-__device__ __forceinline__ void BlocksStoreColumns(uint16_t* p, const uint32_t (&w)[N]) {
-    struct __attribute__((packed, aligned(4))) Dwords {
-        uint32_t x[N];
-    } t;
-#pragma unroll
-    for (int i = 0; i < N; ++i) t.x[i] = w[i];
-    *reinterpret_cast<Dwords*>(p) = t;
-}
-
 // All of a query row's probed rows from tile `u` to `end`, 32 a step
 template <bool BF16, int DC, bool AHEAD>
 __device__ __forceinline__ void BlocksAttendRange(const BlocksArgs& a, uint32_t h, int visible, int block, int64_t ko, int64_t vo, uint32_t u, uint32_t end,
@@ -156,7 +132,7 @@ __device__ __forceinline__ void BlocksAttendStore(const BlocksArgs& a, uint32_t 
         uint32_t w[DC / 2];
 #pragma unroll
         for (int c = 0; c < DC / 2; ++c) w[c] = BlocksPack<BF16>(o[2 * c][i] * inv, o[2 * c + 1][i] * inv);
-        BlocksStoreColumns<BF16, DC / 2>(out + b * a.os[0] + (int64_t)t * a.os[1] + head * a.os[2] + (g * 4 + i) * DC, w);
+        BlocksStoreColumns<DC / 2>(out + b * a.os[0] + (int64_t)t * a.os[1] + head * a.os[2] + (g * 4 + i) * DC, w);
     }
     if (lse && g == 0) lse[((int64_t)b * a.Tq + t) * a.Hq + head] = sum == 0.f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
 }
@@ -238,20 +214,6 @@ __global__ void __launch_bounds__(512) BlocksAttendKernel(BlocksArgs a, uint32_t
 }
 
 // ---- forward, neighbouring query rows together ----------------------------------------------------------------------------------------------------
-// LDS addresses of a lane's part of a stage's operands, relative to the stage
-template <int DC>
-struct BlocksWalkAddresses {
-    uint32_t rows[DC / 2], turned[DC];   // by rows: step s of row lane % 16; transposed: 16 dimensions d of rows 4 g ..
-    __device__ __forceinline__ explicit BlocksWalkAddresses(uint32_t lane) {
-        using S = BlocksWalkShape<DC>;
-        const uint32_t r = lane & 15, g = lane >> 4, row = g * 4 + r / 4;
-#pragma unroll
-        for (uint32_t s = 0; s < DC / 2; ++s) rows[s] = (r * S::CPR + S::Slot(s * 4 + g, r)) * 16;
-#pragma unroll
-        for (uint32_t d = 0; d < DC; ++d) turned[d] = (row * S::CPR + S::Slot(d * 2 + (r & 3) / 2, row)) * 16 + (r & 1) * 8;
-    }
-};
-
 // NT tiles of 16 keys of the stage at LDS byte `at` against a wavefront's CT x 16 columns; `mask`: which of its query rows look at them.  Operands are read in
 // batches ahead of the products that need them (the scheduling barriers keep the compiler from pairing every read with its use, a full LDS latency each).
 // scale2 >= 0 (the sign is the queries').
@@ -508,309 +470,6 @@ __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint
     }
 }
 
-// ---- gradient of the queries ----------------------------------------------------------------------------------------------------------------
-// The forward's walk again: X^T = K Q^T, dP^T = V dO^T, dS = P (dP - delta), dQ^T += K^T dS^T.  delta = <dout, out> of every row is left for the key side.
-template <bool BF16, int DC>
-__global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint32_t mtiles, uint32_t tiles, const uint16_t* __restrict__ out,
-                                                             const uint16_t* __restrict__ dout, const float* __restrict__ lse, uint16_t* __restrict__ dq,
-                                                             float* __restrict__ delta_out) {
-    TakeWholeRegisterFile();
-    constexpr int KS = DC / 2, N = DC / 2;
-    __shared__ uint32_t s_scratch[8][64];
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    uint32_t pair, tile;
-    if (!BlocksPairOf(blockIdx.x, a.B * a.Hkv, tiles, pair, tile)) return;
-    const uint32_t b = pair / a.Hkv, h = pair % a.Hkv;
-    const int n = BlocksKvLen(a, b), m = BlocksQLen(a, b);
-    const uint32_t task = tile * 8 + wave, t = task / mtiles, mt = task % mtiles;
-    if (t >= a.Tq) return;
-    const uint32_t heads = min(16u, a.G - mt * 16), head = h * a.G + mt * 16 + min(r, heads - 1);
-    const int visible = BlocksVisible(a, n, m, (int)t);
-    f32x4_t acc[DC];
-#pragma unroll
-    for (int d = 0; d < DC; ++d) acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    if (visible > 0) {
-        int block;
-        int64_t ko, vo;
-        const uint32_t count = BlocksGatherProbes(a, a.probes + (((int64_t)b * a.Tq + t) * a.Hkv + h) * a.P, b, visible, s_scratch[wave], lane, block, ko, vo);
-        u32x4_t q[KS], go[KS];
-        BlocksLoadRows<KS>(a.q + b * a.qs[0] + t * a.qs[1] + head * a.qs[2] + g * 8, q);
-        BlocksLoadRows<KS>(dout + b * a.os[0] + t * a.os[1] + head * a.os[2] + g * 8, go);
-        float delta = 0.f;
-        {
-            u32x4_t y[KS];
-            BlocksLoadRows<KS>(out + b * a.os[0] + t * a.os[1] + head * a.os[2] + g * 8, y);
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    delta += BlocksToFloat((uint16_t)y[s][i], BF16) * BlocksToFloat((uint16_t)go[s][i], BF16);
-                    delta += BlocksToFloat((uint16_t)(y[s][i] >> 16), BF16) * BlocksToFloat((uint16_t)(go[s][i] >> 16), BF16);
-                }
-            delta = BlocksSumOver4(delta);
-        }
-        const int64_t row = ((int64_t)b * a.Tq + t) * a.Hq + head;
-        const float l = lse[row], lse2 = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;   // an empty row weighs nothing
-        if (g == 0 && r < heads) delta_out[row] = delta;
-        const uint32_t tpb = a.bs / 16, units = count * tpb;
-        BlocksCursor c(0, tpb);
-        for (uint32_t u = 0; u < units; u += 2) {
-            u32x4_t kr[2][KS], vr[2][KS];
-            uint32_t kc[8][N];
-            int start[2];
-            const bool second = u + 1 < units;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int blk = __builtin_amdgcn_readlane(block, (int)c.slot);
-                const int64_t kb = BlocksReadLane64(ko, c.slot), vb = BlocksReadLane64(vo, c.slot);
-                const int base = (int)c.sub * 16, most = visible - 1 - blk * (int)a.bs;
-                start[x] = blk * (int)a.bs + base;
-                const uint16_t* k = a.k + kb + h * a.ks[2];
-                BlocksLoadRows<KS>(k + min(base + (int)r, most) * a.ks[1] + g * 8, kr[x]);
-                BlocksLoadRows<KS>(a.v + vb + h * a.vs[2] + min(base + (int)r, most) * a.vs[1] + g * 8, vr[x]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) BlocksLoadColumns<N>(k + min(base + (int)g * 4 + i, most) * a.ks[1] + r * DC, kc[x * 4 + i]);
-                if (x == 0 && second) c.Next();
-            }
-            c.Next();
-            f32x4_t s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, dp[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-#pragma unroll
-                for (int j = 0; j < KS; ++j) {
-                    s[x] = BlocksMfma<BF16>(kr[x][j], q[j], s[x]);
-                    dp[x] = BlocksMfma<BF16>(vr[x][j], go[j], dp[x]);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool ok = (x == 0 || second) && start[x] + (int)g * 4 + i < visible;
-                    const float p = BlocksExp2(s[x][i] * a.scale2 - lse2);
-                    s[x][i] = ok ? p * (dp[x][i] - delta) : 0.f;
-                    if (!ok) {
-#pragma unroll
-                        for (int w = 0; w < N; ++w) kc[x * 4 + i][w] = 0u;
-                    }
-                }
-            }
-            const u32x4_t ds = BlocksPackOperand<BF16>(s[0], s[1]);   // one rounding of dS, as of P in the forward
-#pragma unroll
-            for (int d = 0; d < DC; ++d) acc[d] = BlocksMfma<BF16>(BlocksColumn<N>(kc, d), ds, acc[d]);
-        }
-    }
-    if (r >= heads) return;
-    uint16_t* dst = dq + b * a.qs[0] + (int64_t)t * a.qs[1] + head * a.qs[2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t w[N];
-#pragma unroll
-        for (int c = 0; c < N; ++c) w[c] = BlocksPack<BF16>(acc[2 * c][i] * a.scale, acc[2 * c + 1][i] * a.scale);
-        BlocksStoreColumns<BF16, N>(dst + (g * 4 + i) * DC, w);
-    }
-}
-
-// ---- which query rows probe a block -------------------------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) BlocksClearKernel(uint32_t* __restrict__ p, uint64_t n) {
-    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) p[i] = 0;
-}
-// bits[sequence, head][block][query row]: set bits are the same whatever their order
-__global__ void __launch_bounds__(256) BlocksBitsKernel(BlocksArgs a, uint32_t words, uint32_t* __restrict__ bits) {
-    const uint64_t all = (uint64_t)a.B * a.Tq * a.Hkv * a.P;
-    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < all; i += gridDim.x * 256ull) {
-        const int p = a.probes[i];
-        const uint64_t row = i / a.P;
-        const uint32_t h = (uint32_t)(row % a.Hkv), t = (uint32_t)(row / a.Hkv % a.Tq), b = (uint32_t)(row / a.Hkv / a.Tq);
-        const int visible = BlocksVisible(a, BlocksKvLen(a, b), BlocksQLen(a, b), (int)t);
-        int64_t ko, vo;
-        if (p < 0 || (uint32_t)p >= a.nblk || (int64_t)p * a.bs >= visible || !BlocksBase(a, b, p, ko, vo)) continue;
-        atomicOr(bits + (((uint64_t)b * a.Hkv + h) * a.nblk + p) * words + t / 32, 1u << (t & 31));
-    }
-}
-// the set bits of words [first, first + kRange / 32) as a list of query rows, ascending; by the first wavefront
-__device__ __forceinline__ void BlocksListRows(const uint32_t* bits, uint32_t first, uint32_t words, uint32_t* s_list, uint32_t* s_count) {
-    if (threadIdx.x < 64) {
-        const uint32_t lane = threadIdx.x;
-        uint32_t w = first + lane < words ? bits[first + lane] : 0u;
-        const uint32_t c = (uint32_t)__popc(w);
-        uint32_t before = c;
-        for (int s = 1; s < 64; s <<= 1) {
-            const uint32_t x = __shfl_up(before, s);
-            if ((int)lane >= s) before += x;
-        }
-        if (lane == 63) *s_count = before;
-        before -= c;
-        while (w) {
-            s_list[before++] = (first + lane) * 32 + (uint32_t)__ffs(w) - 1;
-            w &= w - 1;
-        }
-    }
-}
-
-// What a wavefront of a key-stationary kernel knows of the 32 (query row, head) rows of a step
-struct BlocksRows {
-    int64_t q[32], o[32];
-    float lse2[32], delta[32];
-    int visible[32];
-};
-
-// ---- gradients of the keys and values -------------------------------------------------------------------------------------------------------
-// One workgroup per block (and per kRange query rows, `splits`): the rows that probe it, G heads each, stream past the block's keys.  X = Q K^T and
-// dP = dO V^T come out with a key per lane column, which makes P and dS the operands of dV += P^T dO and dK += dS^T Q as they are.  Wavefronts divide the
-// block's 16-key tiles (kt), halves of the dimensions where both accumulators would not fit (hd), and the rows (rg); row groups are added at the end.
-template <bool BF16, int DC>
-__global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_t words, uint32_t splits, uint32_t tile_groups, uint32_t blocks_x,
-                                                           const uint32_t* __restrict__ bits, const uint16_t* __restrict__ dout, const float* __restrict__ lse,
-                                                           const float* __restrict__ delta, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv,
-                                                           float* __restrict__ partial) {
-    TakeWholeRegisterFile();
-    constexpr int KS = DC / 2, D = DC * 16, ND = DC > 8 ? 2 : 1, OD = DC / ND, N = OD / 2;
-    extern __shared__ float s_add[];   // [8 / ND tiles][16 keys][D]
-    __shared__ uint32_t s_list[kRange], s_count;
-    __shared__ BlocksRows s_rows[8];
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    uint32_t pair, x;
-    if (!BlocksPairOf(blockIdx.x, a.B * a.Hkv, blocks_x, pair, x)) return;
-    const uint32_t split = x % splits, tg = x / splits % tile_groups, block = x / splits / tile_groups;
-    const uint32_t b = pair / a.Hkv, h = pair % a.Hkv;
-    const int n = BlocksKvLen(a, b), m = BlocksQLen(a, b);
-    const uint32_t most = 8 / ND, tpb = a.bs / 16, kts = min(most, tpb - tg * most), rgs = most / kts;
-    const uint32_t kt = wave % kts, hd = ND == 1 ? 0 : wave / kts % ND, rg = wave / (kts * ND);   // wavefronts beyond kts * ND * rgs idle
-    const bool works = rg < rgs;
-    const uint32_t in_block = (tg * most + kt) * 16;
-    const int key0 = (int)(block * a.bs + in_block);
-
-    f32x4_t ak[OD], av[OD];
-#pragma unroll
-    for (int d = 0; d < OD; ++d) ak[d] = av[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    BlocksListRows(bits + ((uint64_t)pair * a.nblk + block) * words, split * (kRange / 32), words, s_list, &s_count);
-    __syncthreads();
-    const uint32_t rows = s_count * a.G;
-    if (works && rows > 0) {
-        u32x4_t kf[KS], vf[KS];
-        {
-            int64_t ko, vo;
-            (void)BlocksBase(a, b, (int)block, ko, vo);
-            const int last = n - 1 - (int)(block * a.bs);   // >= 0: a listed block holds a visible row
-            const int row = min((int)(in_block + r), last);
-            BlocksLoadRows<KS>(a.k + ko + h * a.ks[2] + row * a.ks[1] + g * 8, kf);
-            BlocksLoadRows<KS>(a.v + vo + h * a.vs[2] + row * a.vs[1] + g * 8, vf);
-        }
-        BlocksRows& info = s_rows[wave];
-        for (uint32_t row0 = rg * 32; row0 < rows; row0 += rgs * 32) {
-            if (lane < 32) {
-                const uint32_t row = row0 + lane, rr = min(row, rows - 1), t = s_list[rr / a.G], head = h * a.G + rr % a.G;
-                const int64_t at = ((int64_t)b * a.Tq + t) * a.Hq + head;
-                const float l = lse[at];
-                info.q[lane] = b * a.qs[0] + t * a.qs[1] + head * a.qs[2];
-                info.o[lane] = b * a.os[0] + t * a.os[1] + head * a.os[2];
-                info.lse2[lane] = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;
-                info.delta[lane] = delta[at];
-                info.visible[lane] = row < rows ? BlocksVisible(a, n, m, (int)t) : 0;
-            }
-            BlocksWaveSync();
-            f32x4_t s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, dp[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const uint16_t* qp = a.q + info.q[y * 16 + r] + g * 8;
-                const uint16_t* op = dout + info.o[y * 16 + r] + g * 8;
-#pragma unroll
-                for (int j = 0; j < KS; ++j) {
-                    s[y] = BlocksMfma<BF16>(*reinterpret_cast<const u32x4_t*>(qp + j * 32), kf[j], s[y]);
-                    dp[y] = BlocksMfma<BF16>(*reinterpret_cast<const u32x4_t*>(op + j * 32), vf[j], dp[y]);
-                }
-            }
-            uint32_t qc[8][N], oc[8][N];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t row = (i >> 2) * 16 + g * 4 + (i & 3);
-                BlocksLoadColumns<N>(a.q + info.q[row] + r * DC + hd * OD, qc[i]);
-                BlocksLoadColumns<N>(dout + info.o[row] + r * DC + hd * OD, oc[i]);
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t row = y * 16 + g * 4 + i;
-                    const bool ok = key0 + (int)r < info.visible[row];
-                    const float p = ok ? BlocksExp2(s[y][i] * a.scale2 - info.lse2[row]) : 0.f;
-                    s[y][i] = p;
-                    dp[y][i] = ok ? p * (dp[y][i] - info.delta[row]) : 0.f;
-                }
-            const u32x4_t p = BlocksPackOperand<BF16>(s[0], s[1]), ds = BlocksPackOperand<BF16>(dp[0], dp[1]);
-#pragma unroll
-            for (int d = 0; d < OD; ++d) {
-                av[d] = BlocksMfma<BF16>(p, BlocksColumn<N>(oc, d), av[d]);
-                ak[d] = BlocksMfma<BF16>(ds, BlocksColumn<N>(qc, d), ak[d]);
-            }
-            BlocksWaveSync();
-        }
-    }
-    // row groups are added in their order, first the keys' sums, then the values'
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        f32x4_t(&acc)[OD] = which ? av : ak;
-        for (uint32_t from = 1; from < rgs; ++from) {
-            __syncthreads();
-            if (works && rg == from)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int d = 0; d < OD; ++d) s_add[(kt * 16 + g * 4 + i) * D + r * DC + hd * OD + d] = acc[d][i];
-            __syncthreads();
-            if (works && rg == 0)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int d = 0; d < OD; ++d) acc[d][i] += s_add[(kt * 16 + g * 4 + i) * D + r * DC + hd * OD + d];
-        }
-    }
-    if (!works || rg != 0) return;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t row = block * a.bs + in_block + g * 4 + i;
-        if (row >= a.Tk) continue;
-        if (splits > 1) {
-            float* pk = partial + ((((uint64_t)split * a.B * a.Hkv + pair) * a.Tk + row) * 2) * D + r * DC + hd * OD;
-#pragma unroll
-            for (int d = 0; d < OD; ++d) {
-                pk[d] = ak[d][i];
-                pk[D + d] = av[d][i];
-            }
-        } else {
-            uint32_t wk[N], wv[N];
-#pragma unroll
-            for (int c = 0; c < N; ++c) {
-                wk[c] = BlocksPack<BF16>(ak[2 * c][i] * a.scale, ak[2 * c + 1][i] * a.scale);
-                wv[c] = BlocksPack<BF16>(av[2 * c][i], av[2 * c + 1][i]);
-            }
-            BlocksStoreColumns<BF16, N>(dk + b * a.ks[0] + row * a.ks[1] + h * a.ks[2] + r * DC + hd * OD, wk);
-            BlocksStoreColumns<BF16, N>(dv + b * a.vs[0] + row * a.vs[1] + h * a.vs[2] + r * DC + hd * OD, wv);
-        }
-    }
-}
-
-// adds the splits' sums in their order; two dimensions a thread
-template <bool BF16>
-__global__ void __launch_bounds__(256) BlocksKeyGradJoinKernel(BlocksArgs a, uint32_t d, uint32_t splits, const float* __restrict__ partial,
-                                                               uint16_t* __restrict__ dk, uint16_t* __restrict__ dv) {
-    const uint64_t step = (uint64_t)a.B * a.Hkv * a.Tk * 2 * d, all = step / 2;
-    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < all; i += gridDim.x * 256ull) {
-        const uint64_t e = i * 2;
-        float x = 0.f, y = 0.f;
-        for (uint32_t s = 0; s < splits; ++s) {
-            const float2 p = *reinterpret_cast<const float2*>(partial + s * step + e);
-            x += p.x;
-            y += p.y;
-        }
-        const uint32_t c = (uint32_t)(e % d), value = (uint32_t)(e / d % 2);
-        const uint64_t pr = e / d / 2;
-        const uint32_t row = (uint32_t)(pr % a.Tk), pair = (uint32_t)(pr / a.Tk), b = pair / a.Hkv, h = pair % a.Hkv;
-        if (value)
-            *reinterpret_cast<uint32_t*>(dv + b * a.vs[0] + row * a.vs[1] + h * a.vs[2] + c) = BlocksPack<BF16>(x, y);
-        else
-            *reinterpret_cast<uint32_t*>(dk + b * a.ks[0] + row * a.ks[1] + h * a.ks[2] + c) = BlocksPack<BF16>(x * a.scale, y * a.scale);
-    }
-}
-
 // ---- attention weights of the cache rows ------------------------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) BlocksCopyKernel(const float* __restrict__ from, float* __restrict__ to, uint64_t n) {
     for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) to[i] = from[i];
@@ -857,14 +516,21 @@ __global__ void __launch_bounds__(512) BlocksWeighTokenKernel(BlocksArgs a, uint
     }
 }
 
-// many query rows: the key-stationary walk of the gradients, with the weights alone
+// What a wavefront of the kernel below knows of the 16 (query row, head) rows of a step
+struct BlocksWeighRows {
+    int64_t q[16];
+    float lse2[16];
+    int visible[16];
+};
+
+// many query rows: one workgroup per block, the rows that probe it stream past its keys; wavefronts divide the block's 16-key tiles and the rows
 template <bool BF16, int DC>
 __global__ void __launch_bounds__(512) BlocksWeighKernel(BlocksArgs a, uint32_t words, uint32_t tile_groups, uint32_t blocks_x, const uint32_t* __restrict__ bits,
                                                          const float* __restrict__ lse, const float* mass_in, float* mass_out) {
     TakeWholeRegisterFile();
     constexpr int KS = DC / 2;
     __shared__ uint32_t s_list[kRange], s_count;
-    __shared__ BlocksRows s_rows[8];
+    __shared__ BlocksWeighRows s_rows[8];
     __shared__ float s_sum[8][16];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     uint32_t pair, x;
@@ -890,7 +556,7 @@ __global__ void __launch_bounds__(512) BlocksWeighKernel(BlocksArgs a, uint32_t 
                 BlocksLoadRows<KS>(a.k + ko + h * a.ks[2] + min((int)(in_block + r), last) * a.ks[1] + g * 8, kf);
                 loaded = true;
             }
-            BlocksRows& info = s_rows[wave];
+            BlocksWeighRows& info = s_rows[wave];
             for (uint32_t row0 = rg * 16; row0 < rows; row0 += rgs * 16) {
                 if (lane < 16) {
                     const uint32_t row = row0 + lane, rr = min(row, rows - 1), t = s_list[rr / a.G], head = h * a.G + rr % a.G;
@@ -925,67 +591,13 @@ __global__ void __launch_bounds__(512) BlocksWeighKernel(BlocksArgs a, uint32_t 
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------------------
-static bool Aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-static bool Aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
-
-struct BackwardSpace {
-    size_t bits, delta, partial, total;
-    uint32_t words, splits;
-};
-static BackwardSpace BackwardLayout(const BlocksArgs& a, uint32_t d) {
-    BackwardSpace s{};
-    s.words = (a.Tq + 31) / 32;
-    s.splits = std::max(1u, (a.Tq + kRange - 1) / kRange);
-    size_t at = 0;
-    s.bits = at;
-    at += BlocksAlign((size_t)a.B * a.Hkv * a.nblk * s.words * 4);
-    s.delta = at;
-    at += BlocksAlign((size_t)a.B * a.Tq * a.Hq * 4);
-    s.partial = at;
-    if (s.splits > 1) at += BlocksAlign((size_t)s.splits * a.B * a.Hkv * a.Tk * 2 * d * 4);
-    s.total = at;
-    return s;
-}
 static size_t WeighSpace(const BlocksArgs& a) { return a.Tq <= 1 ? 0 : BlocksAlign((size_t)a.B * a.Hkv * a.nblk * ((a.Tq + 31) / 32) * 4); }
-
-static gpann_status CheckGrid(uint64_t n) {
-    if (n <= 0x7fffffffull) return GPANN_OK;
-    SetLastError("the call needs %llu workgroups, more than 2^31 - 1", (unsigned long long)n);
-    return GPANN_ERR_UNSUPPORTED;
-}
-static gpann_status CheckWorkspace(const void* p, size_t have, size_t need) {
-    if (need == 0) return GPANN_OK;
-    if (have < need) {
-        SetLastError("invalid argument: the workspace has %zu bytes, the call needs %zu", have, need);
-        return GPANN_ERR_INVALID;
-    }
-    GPANN_REQUIRE(p && Aligned16(p), "the workspace is null or not 16-byte aligned");
-    return GPANN_OK;
-}
-
-static gpann_status MarkProbes(const BlocksArgs& a, uint32_t words, uint32_t* bits, hipStream_t st) {
-    const uint64_t n = (uint64_t)a.B * a.Hkv * a.nblk * words, all = (uint64_t)a.B * a.Tq * a.Hkv * a.P;
-    hipLaunchKernelGGL(BlocksClearKernel, dim3((uint32_t)std::min<uint64_t>((n + 255) / 256, 8192)), dim3(256), 0, st, bits, n);
-    GPANN_HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(BlocksBitsKernel, dim3((uint32_t)std::min<uint64_t>((all + 255) / 256, 16384)), dim3(256), 0, st, a, words, bits);
-    GPANN_HIP_TRY(hipGetLastError());
-    return GPANN_OK;
-}
-
-template <typename K, typename... A>
-static gpann_status Launch(K kernel, uint64_t grid, size_t lds, hipStream_t st, A... args) {
-    GPANN_TRY(CheckGrid(grid));
-    if (lds > 32 * 1024) GPANN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(512), lds, st, args...);
-    GPANN_HIP_TRY(hipGetLastError());
-    return GPANN_OK;
-}
 
 template <bool BF16, int DC, int CT>
 static gpann_status AttendWalk(const BlocksArgs& a, uint16_t* out, float* lse, hipStream_t st) {
     const uint32_t cols = 16 * CT, mtiles = (a.G + cols - 1) / cols, tpw = std::max(1u, cols / a.G);
     const uint64_t waves = mtiles > 1 ? (uint64_t)a.Tq * mtiles : (a.Tq + tpw - 1) / tpw, tiles = (waves + 7) / 8;
-    return Launch(BlocksAttendWalkKernel<BF16, DC, CT>, BlocksPairGrid((uint64_t)a.B * a.Hkv, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, lse);
+    return BlocksLaunch(BlocksAttendWalkKernel<BF16, DC, CT>, BlocksPairGrid((uint64_t)a.B * a.Hkv, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, lse);
 }
 
 template <bool BF16, int DC>
@@ -996,7 +608,7 @@ static gpann_status Attend(const BlocksArgs& a, uint16_t* out, float* lse, hipSt
         // 32 columns a wavefront read LDS half as often for each, but make half the workgroups (one per CU at a time) of a larger union: 8192 rows x 32 heads,
         // 1024 workgroups of 32 columns, 536 us against 588; 777 rows x 12 heads, 120 workgroups, 152 us against 103.  (Wide heads have no registers for it.)
         if constexpr (DC <= 8)
-            if (pairs * ((tasks * a.G / mtiles + 255) / 256) >= 512) return AttendWalk<BF16, DC, 2>(a, out, lse, st);
+            if (pairs * (((uint64_t)a.Tq * a.G + 255) / 256) >= 512) return AttendWalk<BF16, DC, 2>(a, out, lse, st);
         return AttendWalk<BF16, DC, 1>(a, out, lse, st);
     }
     // few query rows: their keys are divided over wavefronts until the chip's 2048 have something to do
@@ -1004,35 +616,7 @@ static gpann_status Attend(const BlocksArgs& a, uint16_t* out, float* lse, hipSt
     while (waves < 8 && pairs * tasks * waves < 2048) waves *= 2;
     const uint64_t tiles = (tasks * waves + 7) / 8;
     const size_t lds = waves > 1 ? (size_t)8 * 16 * (DC * 16 + 2) * 4 : 0;
-    return Launch(BlocksAttendKernel<BF16, DC>, BlocksPairGrid(pairs, tiles), lds, st, a, waves, mtiles, (uint32_t)tiles, out, lse);
-}
-
-template <bool BF16, int DC>
-static gpann_status Backward(const BlocksArgs& a, const uint16_t* out, const float* lse, const uint16_t* dout, uint16_t* dq, uint16_t* dk, uint16_t* dv,
-                             char* ws, hipStream_t st) {
-    constexpr uint32_t D = DC * 16, most = DC > 8 ? 4 : 8;
-    const BackwardSpace s = BackwardLayout(a, D);
-    uint32_t* bits = reinterpret_cast<uint32_t*>(ws + s.bits);
-    float* delta = reinterpret_cast<float*>(ws + s.delta);
-    float* partial = reinterpret_cast<float*>(ws + s.partial);
-    const uint64_t pairs = (uint64_t)a.B * a.Hkv;
-    if (a.Tq > 0) {
-        const uint32_t mtiles = (a.G + 15) / 16;
-        const uint64_t tiles = ((uint64_t)a.Tq * mtiles + 7) / 8;
-        GPANN_TRY(Launch(BlocksQueryGradKernel<BF16, DC>, BlocksPairGrid(pairs, tiles), 0, st, a, mtiles, (uint32_t)tiles, out, dout, lse, dq, delta));
-        GPANN_TRY(MarkProbes(a, s.words, bits, st));
-    }
-    if (a.Tk == 0) return GPANN_OK;
-    const uint32_t tile_groups = (a.bs / 16 + most - 1) / most;
-    const uint64_t blocks_x = (uint64_t)a.nblk * tile_groups * s.splits;
-    GPANN_TRY(Launch(BlocksKeyGradKernel<BF16, DC>, BlocksPairGrid(pairs, blocks_x), (size_t)most * 16 * D * 4, st, a, s.words, s.splits, tile_groups,
-                     (uint32_t)blocks_x, bits, dout, lse, delta, dk, dv, partial));
-    if (s.splits > 1) {
-        const uint64_t all = pairs * a.Tk * D;
-        hipLaunchKernelGGL(BlocksKeyGradJoinKernel<BF16>, dim3((uint32_t)std::min<uint64_t>((all + 255) / 256, 65536)), dim3(256), 0, st, a, D, s.splits, partial, dk, dv);
-        GPANN_HIP_TRY(hipGetLastError());
-    }
-    return GPANN_OK;
+    return BlocksLaunch(BlocksAttendKernel<BF16, DC>, BlocksPairGrid(pairs, tiles), lds, st, a, waves, mtiles, (uint32_t)tiles, out, lse);
 }
 
 template <bool BF16, int DC>
@@ -1045,27 +629,14 @@ static gpann_status Weigh(const BlocksArgs& a, const float* lse, const float* ma
             GPANN_HIP_TRY(hipGetLastError());
         }
         if (a.Tq == 0) return GPANN_OK;
-        return Launch(BlocksWeighTokenKernel<BF16, DC>, pairs, 0, st, a, (a.G + 15) / 16, lse, mass_out);
+        return BlocksLaunch(BlocksWeighTokenKernel<BF16, DC>, pairs, 0, st, a, (a.G + 15) / 16, lse, mass_out);
     }
     const uint32_t words = (a.Tq + 31) / 32, tile_groups = (a.bs / 16 + 7) / 8;
     uint32_t* bits = reinterpret_cast<uint32_t*>(ws);
-    GPANN_TRY(MarkProbes(a, words, bits, st));
+    GPANN_TRY(BlocksMarkProbes(a, words, bits, nullptr, st));
     const uint64_t blocks_x = (uint64_t)a.nblk * tile_groups;
-    return Launch(BlocksWeighKernel<BF16, DC>, BlocksPairGrid(pairs, blocks_x), 0, st, a, words, tile_groups, (uint32_t)blocks_x, bits, lse, mass_in, mass_out);
+    return BlocksLaunch(BlocksWeighKernel<BF16, DC>, BlocksPairGrid(pairs, blocks_x), 0, st, a, words, tile_groups, (uint32_t)blocks_x, bits, lse, mass_in, mass_out);
 }
-
-// head_dim and element type -> template arguments
-#define GPANN_BLOCKS_DISPATCH(L, fn, ...)                                                                                                   \
-    do {                                                                                                                                    \
-        const bool bf16 = (L)->dtype == GPANN_BLOCKS_BF16;                                                                                  \
-        switch ((L)->head_dim) {                                                                                                            \
-            case 64: return bf16 ? fn<true, 4>(__VA_ARGS__) : fn<false, 4>(__VA_ARGS__);                                                    \
-            case 96: return bf16 ? fn<true, 6>(__VA_ARGS__) : fn<false, 6>(__VA_ARGS__);                                                    \
-            case 128: return bf16 ? fn<true, 8>(__VA_ARGS__) : fn<false, 8>(__VA_ARGS__);                                                   \
-            case 192: return bf16 ? fn<true, 12>(__VA_ARGS__) : fn<false, 12>(__VA_ARGS__);                                                 \
-            default: return bf16 ? fn<true, 16>(__VA_ARGS__) : fn<false, 16>(__VA_ARGS__);                                                  \
-        }                                                                                                                                   \
-    } while (0)
 
 }  // namespace gpann
 
@@ -1080,7 +651,7 @@ gpann_status gpann_blocks_workspace_bytes(const gpann_blocks_layout* L, uint32_t
     GPANN_REQUIRE((calls & ~31u) == 0, "unknown bits in calls");
     const BlocksArgs a = BlocksMakeArgs(L, nullptr, nullptr, nullptr, nullptr, nprobe);
     size_t need = 0;
-    if (calls & GPANN_BLOCKS_BACKWARD) need = std::max(need, BackwardLayout(a, L->head_dim).total);
+    if (calls & GPANN_BLOCKS_BACKWARD) need = std::max(need, BlocksBackwardSpace(a, L->head_dim));
     if (calls & GPANN_BLOCKS_WEIGH) need = std::max(need, WeighSpace(a));
     *out_bytes = need;
     return GPANN_OK;
@@ -1092,8 +663,8 @@ gpann_status gpann_blocks_attend(const gpann_blocks_layout* L, const void* q, co
     (void)workspace_bytes;
     GPANN_TRY(BlocksCheckLayout(L));
     GPANN_REQUIRE(q && k && v && probes && out, "a tensor is null");
-    GPANN_REQUIRE(Aligned16(q) && Aligned16(k) && Aligned16(v) && Aligned16(out), "q, k, v and out must be 16-byte aligned");
-    GPANN_REQUIRE(Aligned4(probes) && Aligned4(lse), "probes and lse must be 4-byte aligned");
+    GPANN_REQUIRE(BlocksAligned(16, q) && BlocksAligned(16, k) && BlocksAligned(16, v) && BlocksAligned(16, out), "q, k, v and out must be 16-byte aligned");
+    GPANN_REQUIRE(BlocksAligned(4, probes) && BlocksAligned(4, lse), "probes and lse must be 4-byte aligned");
     GPANN_REQUIRE(nprobe >= 1 && nprobe <= GPANN_BLOCKS_MAX_PROBE, "nprobe must be 1 .. GPANN_BLOCKS_MAX_PROBE");
     GPANN_REQUIRE(BlocksDisjoint(L->out_stride, L->batch, L->q_rows, L->q_heads, L->head_dim), "out overlaps itself");
     GPANN_BLOCKS_ENTER(L, stream);
@@ -1102,39 +673,15 @@ gpann_status gpann_blocks_attend(const gpann_blocks_layout* L, const void* q, co
     GPANN_BLOCKS_DISPATCH(L, Attend, a, static_cast<uint16_t*>(out), lse, static_cast<hipStream_t>(stream));
 }
 
-gpann_status gpann_blocks_attend_backward(const gpann_blocks_layout* L, const void* q, const void* k, const void* v, const int32_t* probes, uint32_t nprobe,
-                                          const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
-                                          size_t workspace_bytes, void* stream) {
-    GPANN_TRY(BlocksCheckLayout(L));
-    GPANN_REQUIRE(q && k && v && probes && out && lse && dout && dq && dk && dv, "a tensor is null");
-    GPANN_REQUIRE(Aligned16(q) && Aligned16(k) && Aligned16(v) && Aligned16(out) && Aligned16(dout) && Aligned16(dq) && Aligned16(dk) && Aligned16(dv),
-                  "q, k, v, out and the gradients must be 16-byte aligned");
-    GPANN_REQUIRE(Aligned4(probes) && Aligned4(lse), "probes and lse must be 4-byte aligned");
-    GPANN_REQUIRE(nprobe >= 1 && nprobe <= GPANN_BLOCKS_MAX_PROBE, "nprobe must be 1 .. GPANN_BLOCKS_MAX_PROBE");
-    if (L->page_table) {
-        SetLastError("gradients of a paged cache are not supported: pages may be shared between sequences");
-        return GPANN_ERR_UNSUPPORTED;
-    }
-    GPANN_REQUIRE(BlocksDisjoint(L->q_stride, L->batch, L->q_rows, L->q_heads, L->head_dim), "dq overlaps itself");
-    GPANN_REQUIRE(BlocksDisjoint(L->k_stride, L->batch, L->kv_rows, L->kv_heads, L->head_dim), "dk overlaps itself");
-    GPANN_REQUIRE(BlocksDisjoint(L->v_stride, L->batch, L->kv_rows, L->kv_heads, L->head_dim), "dv overlaps itself");
-    const BlocksArgs a = BlocksMakeArgs(L, q, k, v, probes, nprobe);
-    GPANN_TRY(CheckWorkspace(workspace, workspace_bytes, BackwardLayout(a, L->head_dim).total));
-    GPANN_BLOCKS_ENTER(L, stream);
-    if (a.B == 0) return GPANN_OK;
-    GPANN_BLOCKS_DISPATCH(L, Backward, a, static_cast<const uint16_t*>(out), lse, static_cast<const uint16_t*>(dout), static_cast<uint16_t*>(dq),
-                          static_cast<uint16_t*>(dk), static_cast<uint16_t*>(dv), static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
-}
-
 gpann_status gpann_blocks_weigh(const gpann_blocks_layout* L, const void* q, const void* k, const int32_t* probes, uint32_t nprobe, const float* lse,
                                 const float* mass_in, float* mass_out, void* workspace, size_t workspace_bytes, void* stream) {
     GPANN_TRY(BlocksCheckLayout(L));
     GPANN_REQUIRE(q && k && probes && lse && mass_in && mass_out, "a tensor is null");
-    GPANN_REQUIRE(Aligned16(q) && Aligned16(k), "q and k must be 16-byte aligned");
-    GPANN_REQUIRE(Aligned4(probes) && Aligned4(lse) && Aligned4(mass_in) && Aligned4(mass_out), "probes, lse and mass must be 4-byte aligned");
+    GPANN_REQUIRE(BlocksAligned(16, q) && BlocksAligned(16, k), "q and k must be 16-byte aligned");
+    GPANN_REQUIRE(BlocksAligned(4, probes) && BlocksAligned(4, lse) && BlocksAligned(4, mass_in) && BlocksAligned(4, mass_out), "probes, lse and mass must be 4-byte aligned");
     GPANN_REQUIRE(nprobe >= 1 && nprobe <= GPANN_BLOCKS_MAX_PROBE, "nprobe must be 1 .. GPANN_BLOCKS_MAX_PROBE");
     const BlocksArgs a = BlocksMakeArgs(L, q, k, nullptr, probes, nprobe);
-    GPANN_TRY(CheckWorkspace(workspace, workspace_bytes, WeighSpace(a)));
+    GPANN_TRY(BlocksCheckWorkspace(workspace, workspace_bytes, WeighSpace(a)));
     GPANN_BLOCKS_ENTER(L, stream);
     if (a.B == 0 || a.Tk == 0) return GPANN_OK;
     GPANN_BLOCKS_DISPATCH(L, Weigh, a, lse, mass_in, mass_out, static_cast<char*>(workspace), static_cast<hipStream_t>(stream));

@@ -62,6 +62,16 @@ __device__ __forceinline__ void BlocksLoadColumns(const uint16_t* p, uint32_t (&
 #pragma unroll
     for (int i = 0; i < N; ++i) w[i] = t.x[i];
 }
+template <int N>
+__device__ __forceinline__ void BlocksStoreColumns(uint16_t* p, const uint32_t (&w)[N]) {
+    struct __attribute__((packed, aligned(4))) Dwords {
+        uint32_t x[N];
+    } t;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t.x[i] = w[i];
+    *reinterpret_cast<Dwords*>(p) = t;
+}
+
 // operand for output slot dt from eight rows read by columns
 template <int N>
 __device__ __forceinline__ u32x4_t BlocksColumn(const uint32_t (&w)[8][N], int dt) {
@@ -101,6 +111,18 @@ __device__ __forceinline__ void BlocksWaveSync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
+
+// unit `u` of a query row's tiles: probed block u / tpb, tile u % tpb of it
+struct BlocksCursor {
+    uint32_t slot, sub, tpb;
+    __device__ __forceinline__ BlocksCursor(uint32_t u, uint32_t tiles_per_block) : slot(u / tiles_per_block), sub(u % tiles_per_block), tpb(tiles_per_block) {}
+    __device__ __forceinline__ void Next() {
+        if (++sub == tpb) {
+            sub = 0;
+            ++slot;
+        }
+    }
+};
 
 // The probed blocks of one query row, one per lane: those that exist and hold a visible row, each once, moved to the front.  Returns their number.
 // `scratch`: 64 words of LDS of this wavefront.

@@ -45,6 +45,10 @@ struct BlocksWalkShape {
 __device__ __forceinline__ void BlocksDma(uint64_t base, uint32_t offset, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(lds) : "m0", "memory");
 }
+// ... from an address per lane
+__device__ __forceinline__ void BlocksDmaFrom(const void* src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "m0", "memory");
+}
 template <int LEFT>
 __device__ __forceinline__ void BlocksDmaWait() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LEFT) : "memory");
@@ -211,5 +215,42 @@ struct BlocksWalker {
         }
     }
 };
+
+// LDS addresses of a lane's part of a stage's operands, relative to the stage
+template <int DC>
+struct BlocksWalkAddresses {
+    uint32_t rows[DC / 2], turned[DC];   // by rows: step s of row lane % 16; transposed: 16 dimensions d of rows 4 g ..
+    __device__ __forceinline__ explicit BlocksWalkAddresses(uint32_t lane) {
+        using S = BlocksWalkShape<DC>;
+        const uint32_t r = lane & 15, g = lane >> 4, row = g * 4 + r / 4;
+#pragma unroll
+        for (uint32_t s = 0; s < DC / 2; ++s) rows[s] = (r * S::CPR + S::Slot(s * 4 + g, r)) * 16;
+#pragma unroll
+        for (uint32_t d = 0; d < DC; ++d) turned[d] = (row * S::CPR + S::Slot(d * 2 + (r & 3) / 2, row)) * 16 + (r & 1) * 8;
+    }
+};
+
+// ---- which query rows probe a block: bits [sequence, head][block][query row] -----------------------------------------------------------------------
+constexpr uint32_t kRange = 2048;   // query rows whose list a workgroup holds at a time
+
+// the set bits of words [first, first + kRange / 32) as a list of query rows, ascending; by the first wavefront
+__device__ __forceinline__ void BlocksListRows(const uint32_t* bits, uint32_t first, uint32_t words, uint32_t* s_list, uint32_t* s_count) {
+    if (threadIdx.x < 64) {
+        const uint32_t lane = threadIdx.x;
+        uint32_t w = first + lane < words ? bits[first + lane] : 0u;
+        const uint32_t c = (uint32_t)__popc(w);
+        uint32_t before = c;
+        for (int s = 1; s < 64; s <<= 1) {
+            const uint32_t x = __shfl_up(before, s);
+            if ((int)lane >= s) before += x;
+        }
+        if (lane == 63) *s_count = before;
+        before -= c;
+        while (w) {
+            s_list[before++] = (first + lane) * 32 + (uint32_t)__ffs(w) - 1;
+            w &= w - 1;
+        }
+    }
+}
 
 }  // namespace gpann

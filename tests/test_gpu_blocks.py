@@ -149,6 +149,11 @@ SHAPES = [
     dict(q_len=[5, 0], kv_len=[150, 150]), dict(q_len=[3, 5], kv_len=[1, 31]), dict(q_len=[5, 4], kv_len=[0, 3]), dict(q_len=[99, -3], kv_len=[999, 20]),
     dict(q_len=[5, 4], kv_len=[0, 3], causal=False), dict(strength=3.0), dict(scale=-0.2), dict(scale=0.0), dict(batch=3, q_rows=33, kv_rows=97, kv_heads=1, q_heads=16),
     dict(q_rows=1, q_heads=24, kv_heads=8, batch=5, kv_len=[150, 7, 64, 65, 1]),
+    dict(batch=1, q_rows=1300, kv_rows=1300, q_heads=16, kv_heads=1, bs=64, nprobe=3),            # blocks that more rows probe than one workgroup takes
+    dict(batch=1, q_rows=1100, kv_rows=1200, q_heads=32, kv_heads=1, bs=16, nprobe=3, dtype="fp16"), dict(batch=1, q_rows=300, kv_rows=300, q_heads=24, kv_heads=1, bs=128, dim=192),
+    dict(batch=1, q_rows=20, kv_rows=20000, bs=16, nprobe=40, q_heads=3, kv_heads=1),             # more blocks than a walk holds at a time
+    dict(batch=1, q_rows=4, kv_rows=18000, bs=16, nprobe=64, q_heads=2, kv_heads=1, dim=192), dict(q_rows=260, kv_rows=260, q_heads=2, kv_heads=2, bs=96, batch=1),
+    dict(batch=8, q_rows=96, kv_rows=128, q_heads=64, kv_heads=8, dim=128, bs=32), dict(batch=8, q_rows=250, kv_rows=256, q_heads=24, kv_heads=8, dim=64, bs=16, causal=False),
 ]
 
 
