@@ -97,8 +97,8 @@ __device__ __forceinline__ bool BlocksPairOf(uint32_t id, uint32_t pairs, uint32
     tile = rest % tiles;
     return pair < pairs;
 }
-// bits (and counts, may be null) of the probes of every block; both cleared first
-gpann_status BlocksMarkProbes(const BlocksArgs& a, uint32_t words, uint32_t* bits, uint32_t* counts, hipStream_t st);
+// bits[sequence, head][block][query row / 32] of the rows that probe a block; every word is written
+gpann_status BlocksMarkProbes(const BlocksArgs& a, uint32_t words, uint32_t* bits, hipStream_t st);
 size_t BlocksBackwardSpace(const BlocksArgs& a, uint32_t d);
 
 inline bool BlocksAligned(uintptr_t n, const void* p) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }

@@ -37,7 +37,8 @@ gpann_status BlocksCheckLayout(const gpann_blocks_layout* L) {
     for (const int64_t* s : strides)
         for (int i = 0; i < 3; ++i) {
             GPANN_REQUIRE(s[i] >= 0 && s[i] % 8 == 0, "strides must be non-negative multiples of 8 elements");
-            GPANN_REQUIRE(s[i] <= (i == 1 ? (int64_t)1 << 22 : (int64_t)1 << 40), "a row stride above 2^22 elements or another above 2^40");
+            GPANN_REQUIRE(s[i] <= (i == 0 ? (int64_t)1 << 40 : i == 1 ? (int64_t)1 << 22 : (int64_t)1 << 31),
+                          "a stride above 2^40 (batch or page), 2^22 (row) or 2^31 (head) elements");
         }
     if (L->page_table) {
         GPANN_REQUIRE(L->page_stride >= BlocksPerSequence(L), "layout.page_stride is smaller than a sequence's blocks");

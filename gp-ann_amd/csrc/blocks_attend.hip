@@ -633,7 +633,7 @@ static gpann_status Weigh(const BlocksArgs& a, const float* lse, const float* ma
     }
     const uint32_t words = (a.Tq + 31) / 32, tile_groups = (a.bs / 16 + 7) / 8;
     uint32_t* bits = reinterpret_cast<uint32_t*>(ws);
-    GPANN_TRY(BlocksMarkProbes(a, words, bits, nullptr, st));
+    GPANN_TRY(BlocksMarkProbes(a, words, bits, st));
     const uint64_t blocks_x = (uint64_t)a.nblk * tile_groups;
     return BlocksLaunch(BlocksWeighKernel<BF16, DC>, BlocksPairGrid(pairs, blocks_x), 0, st, a, words, tile_groups, (uint32_t)blocks_x, bits, lse, mass_in, mass_out);
 }

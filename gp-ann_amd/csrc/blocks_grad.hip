@@ -13,10 +13,10 @@ namespace gpann {
 // delta = <dout, out> is what every dp is measured against; `out` was rounded, so it is off by e, the same for all of a row's keys.  The walk therefore sums
 // ds' = p (dp - delta'), which is e in all, and w = sum p k beside dq' = sum ds' k: the gradient at the true delta is dq' - e w (the weights sum to 1).
 
-// What a query row is to the key side
+// What the key side needs of a (query row, head) row: lse * log2 e (+inf: it weighs nothing) and delta.  Both arrays end with an entry of a row that weighs nothing.
 struct BlocksRowInfo {
-    float lse2, delta;
-    int visible, pad;
+    float* lse2;
+    float* delta;
 };
 
 template <bool BF16, int DC>
@@ -37,7 +37,7 @@ __device__ __forceinline__ float BlocksDelta(const uint16_t* out, const u32x4_t 
 // One query row's heads (columns r < heads), its probed rows straight from memory: the way out for rows whose neighbours' values are not finite.
 template <bool BF16, int DC>
 __device__ __forceinline__ void BlocksQueryGradRow(const BlocksArgs& a, uint32_t b, uint32_t h, uint32_t t, uint32_t head, bool live, int visible, uint32_t lane,
-                                                   uint32_t* scratch, const uint16_t* out, const uint16_t* dout, const float* lse, uint16_t* dq, BlocksRowInfo* rows) {
+                                                   uint32_t* scratch, const uint16_t* out, const uint16_t* dout, const float* lse, uint16_t* dq, BlocksRowInfo rows) {
     constexpr int KS = DC / 2, N = DC / 2;
     const uint32_t r = lane & 15, g = lane >> 4;
     int block;
@@ -97,7 +97,10 @@ __device__ __forceinline__ void BlocksQueryGradRow(const BlocksArgs& a, uint32_t
         for (int x = 0; x < N; ++x) w[x] = BlocksPack<BF16>(acc[2 * x][i] * a.scale, acc[2 * x + 1][i] * a.scale);
         BlocksStoreColumns<N>(dst + (g * 4 + i) * DC, w);
     }
-    if (g == 0) rows[row] = BlocksRowInfo{lse2, delta, visible, 0};
+    if (g == 0) {
+        rows.lse2[row] = lse2;
+        rows.delta[row] = delta;
+    }
 }
 
 // NT tiles of 16 keys of the stage at LDS byte `at` against a wavefront's 16 columns
@@ -170,7 +173,7 @@ __device__ __forceinline__ void BlocksWalkQueryGrad(float scale2, uint32_t tile0
 template <bool BF16, int DC>
 __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint32_t tpw, uint32_t mtiles, uint32_t tiles, const uint16_t* __restrict__ out,
                                                              const uint16_t* __restrict__ dout, const float* __restrict__ lse, uint16_t* __restrict__ dq,
-                                                             BlocksRowInfo* __restrict__ info) {
+                                                             BlocksRowInfo info) {
     TakeWholeRegisterFile();
     using S = BlocksWalkShape<DC>;
     constexpr int KS = DC / 2;
@@ -280,39 +283,43 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
     for (int d = 0; d < DC; ++d)
         *reinterpret_cast<u32x2_t*>(dst + d * 16) =
             u32x2_t{BlocksPack<BF16>(acc[d][0] * a.scale, acc[d][1] * a.scale), BlocksPack<BF16>(acc[d][2] * a.scale, acc[d][3] * a.scale)};
-    if (g == 0) info[row] = BlocksRowInfo{lse2, delta + off, col.visible[0], 0};
+    if (g == 0) {
+        info.lse2[row] = lse2;
+        info.delta[row] = delta + off;
+    }
 }
 
 // ---- which query rows probe a block -------------------------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) BlocksClearKernel(uint32_t* __restrict__ p, uint64_t n) {
-    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) p[i] = 0;
-}
-// set bits and counts are the same whatever their order
-__global__ void __launch_bounds__(256) BlocksBitsKernel(BlocksArgs a, uint32_t words, uint32_t* __restrict__ bits, uint32_t* __restrict__ counts) {
-    const uint64_t all = (uint64_t)a.B * a.Tq * a.Hkv * a.P;
-    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < all; i += gridDim.x * 256ull) {
-        const int p = a.probes[i];
-        const uint64_t row = i / a.P;
-        const uint32_t h = (uint32_t)(row % a.Hkv), t = (uint32_t)(row / a.Hkv % a.Tq), b = (uint32_t)(row / a.Hkv / a.Tq);
-        const int visible = BlocksVisible(a, BlocksKvLen(a, b), BlocksQLen(a, b), (int)t);
+constexpr uint32_t kMarkRows = 256, kMarkBlocks = 1024;   // query rows and blocks of a workgroup
+// One workgroup per pair, kMarkRows query rows and kMarkBlocks blocks: bits are set in LDS and every word is written, so nothing has to be cleared
+__global__ void __launch_bounds__(256) BlocksBitsKernel(BlocksArgs a, uint32_t words, uint32_t* __restrict__ bits) {
+    __shared__ uint32_t s_bits[kMarkBlocks * (kMarkRows / 32)];
+    constexpr uint32_t W = kMarkRows / 32;
+    const uint32_t pair = blockIdx.x, b = pair / a.Hkv, h = pair % a.Hkv, t0 = blockIdx.y * kMarkRows, window = blockIdx.z * kMarkBlocks, tid = threadIdx.x;
+    const uint32_t in_window = min(kMarkBlocks, a.nblk - window);
+    const int n = BlocksKvLen(a, b), m = BlocksQLen(a, b);
+    for (uint32_t i = tid; i < in_window * W; i += 256) s_bits[i] = 0;
+    __syncthreads();
+    const uint32_t rows = min(kMarkRows, a.Tq - t0);
+    for (uint32_t i = tid; i < rows * a.P; i += 256) {
+        const uint32_t in = i / a.P, t = t0 + in;
+        const int p = a.probes[(((int64_t)b * a.Tq + t) * a.Hkv + h) * a.P + i % a.P];
+        if (p < (int)window || (uint32_t)p >= window + in_window || (int64_t)p * a.bs >= BlocksVisible(a, n, m, (int)t)) continue;
+        atomicOr(s_bits + ((uint32_t)p - window) * W + in / 32, 1u << (in & 31));
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < in_window * W; i += 256) {
+        const uint32_t block = window + i / W, word = t0 / 32 + i % W;
+        uint32_t x = s_bits[i];
         int64_t ko, vo;
-        if (p < 0 || (uint32_t)p >= a.nblk || (int64_t)p * a.bs >= visible || !BlocksBase(a, b, p, ko, vo)) continue;
-        const uint64_t at = ((uint64_t)b * a.Hkv + h) * a.nblk + p;
-        const uint32_t bit = 1u << (t & 31);
-        if (counts && !(atomicOr(bits + at * words + t / 32, bit) & bit)) atomicAdd(counts + at, 1u);
-        if (!counts) atomicOr(bits + at * words + t / 32, bit);
+        if (x && a.table && !BlocksBase(a, b, (int)block, ko, vo)) x = 0;
+        if (word < words) bits[((uint64_t)pair * a.nblk + block) * words + word] = x;
     }
 }
 
-gpann_status BlocksMarkProbes(const BlocksArgs& a, uint32_t words, uint32_t* bits, uint32_t* counts, hipStream_t st) {
-    const uint64_t blocks = (uint64_t)a.B * a.Hkv * a.nblk, n = blocks * words, all = (uint64_t)a.B * a.Tq * a.Hkv * a.P;
-    hipLaunchKernelGGL(BlocksClearKernel, dim3((uint32_t)std::min<uint64_t>(n / 256 + 1, 8192)), dim3(256), 0, st, bits, n);
-    GPANN_HIP_TRY(hipGetLastError());
-    if (counts) {
-        hipLaunchKernelGGL(BlocksClearKernel, dim3((uint32_t)std::min<uint64_t>(blocks / 256 + 1, 8192)), dim3(256), 0, st, counts, blocks);
-        GPANN_HIP_TRY(hipGetLastError());
-    }
-    hipLaunchKernelGGL(BlocksBitsKernel, dim3((uint32_t)std::min<uint64_t>(all / 256 + 1, 16384)), dim3(256), 0, st, a, words, bits, counts);
+gpann_status BlocksMarkProbes(const BlocksArgs& a, uint32_t words, uint32_t* bits, hipStream_t st) {
+    const dim3 grid(a.B * a.Hkv, (a.Tq + kMarkRows - 1) / kMarkRows, (a.nblk + kMarkBlocks - 1) / kMarkBlocks);
+    hipLaunchKernelGGL(BlocksBitsKernel, grid, dim3(256), 0, st, a, words, bits);
     GPANN_HIP_TRY(hipGetLastError());
     return GPANN_OK;
 }
@@ -324,53 +331,78 @@ struct BlocksPart {
     uint32_t block, index;
     int slot;   // -1: the block's only part
 };
-// one workgroup per pair: parts[pair][capacity], used[pair], first_slot[pair][block]
-__global__ void __launch_bounds__(256) BlocksPartsKernel(BlocksArgs a, uint32_t part, uint32_t capacity, const uint32_t* __restrict__ counts, BlocksPart* __restrict__ parts,
-                                                         uint32_t* __restrict__ used, int* __restrict__ first_slot) {
-    __shared__ uint32_t s_sum[2][256];
-    const uint32_t pair = blockIdx.x, tid = threadIdx.x;
+// one workgroup per pair: counts[pair][block] of its query rows, parts[pair][capacity], used[pair], first_slot[pair][block]
+__global__ void __launch_bounds__(1024) BlocksPartsKernel(BlocksArgs a, uint32_t words, uint32_t part, uint32_t capacity, const uint32_t* __restrict__ bits,
+                                                          uint32_t* __restrict__ counts, BlocksPart* __restrict__ parts, uint32_t* __restrict__ used,
+                                                          int* __restrict__ first_slot, BlocksRowInfo info) {
+    __shared__ uint32_t s_n[1024], s_sum[16], s_slots[16];
+    const uint32_t pair = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     uint32_t base = 0, slots = 0;
-    for (uint32_t j0 = 0; j0 < a.nblk; j0 += 256) {
-        const uint32_t j = j0 + tid;
-        const uint32_t n = j < a.nblk ? max(1u, (counts[(uint64_t)pair * a.nblk + j] + part - 1) / part) : 0, m = n > 1 ? n : 0;
-        s_sum[0][tid] = n;
-        s_sum[1][tid] = m;
-        __syncthreads();
-        for (uint32_t s = 1; s < 256; s <<= 1) {
-            const uint32_t x = tid >= s ? s_sum[0][tid - s] : 0, y = tid >= s ? s_sum[1][tid - s] : 0;
-            __syncthreads();
-            s_sum[0][tid] += x;
-            s_sum[1][tid] += y;
-            __syncthreads();
+    for (uint32_t j0 = 0; j0 < a.nblk; j0 += 1024) {
+        const uint32_t in = min(1024u, a.nblk - j0);
+        for (uint32_t j = wave; j < in; j += 16) {
+            const uint32_t* row = bits + ((uint64_t)pair * a.nblk + j0 + j) * words;
+            uint32_t c = 0;
+            for (uint32_t w = lane; w < words; w += 64) c += (uint32_t)__popc(row[w]);
+            for (int s = 32; s > 0; s >>= 1) c += __shfl_xor(c, s);
+            if (lane == 0) s_n[j] = c;
         }
-        const uint32_t at = base + s_sum[0][tid] - n, slot = slots + s_sum[1][tid] - m;
+        __syncthreads();
+        const uint32_t j = j0 + tid, rows = tid < in ? s_n[tid] : 0, n = tid < in ? max(1u, (rows + part - 1) / part) : 0, m = n > 1 ? n : 0;
+        uint32_t x = n, y = m;   // inclusive sums over the wavefront, then over the workgroup
+        for (int s = 1; s < 64; s <<= 1) {
+            const uint32_t x1 = __shfl_up(x, s), y1 = __shfl_up(y, s);
+            if ((int)lane >= s) {
+                x += x1;
+                y += y1;
+            }
+        }
+        if (lane == 63) {
+            s_sum[wave] = x;
+            s_slots[wave] = y;
+        }
+        __syncthreads();
+        uint32_t at = base + x - n, slot = slots + y - m;
+        for (uint32_t w = 0; w < 16; ++w) {
+            if (w < wave) {
+                at += s_sum[w];
+                slot += s_slots[w];
+            }
+            base += s_sum[w];
+            slots += s_slots[w];
+        }
         for (uint32_t i = 0; i < n; ++i) parts[(uint64_t)pair * capacity + at + i] = BlocksPart{j, i, n > 1 ? (int)(slot + i) : -1};
-        if (j < a.nblk) first_slot[(uint64_t)pair * a.nblk + j] = n > 1 ? (int)slot : -1;
-        base += s_sum[0][255];
-        slots += s_sum[1][255];
+        if (tid < in) {
+            counts[(uint64_t)pair * a.nblk + j] = rows;
+            first_slot[(uint64_t)pair * a.nblk + j] = n > 1 ? (int)slot : -1;
+        }
         __syncthreads();
     }
     if (tid == 0) used[pair] = base;
+    if (tid == 0 && pair == 0) {
+        info.lse2[(uint64_t)a.B * a.Tq * a.Hq] = __builtin_inff();
+        info.delta[(uint64_t)a.B * a.Tq * a.Hq] = 0.f;
+    }
 }
 
-// Shape of the key side: a workgroup holds 64 keys (four 16-key tiles; halves of the dimensions apart where both sums would not fit a wavefront's
-// registers) and RGS groups of wavefronts take 32 of a stage's 32 RGS rows each.
+// Shape of the key side: a workgroup holds 64 keys (four 16-key tiles), ND wavefronts a tile each take 1 / ND of the dimensions of its sums (where both would
+// not fit a wavefront's registers, or a block has fewer tiles than there are wavefronts), and RGS groups of wavefronts take 32 of a stage's 32 RGS rows each.
+// Four stages: one being read transposed, the next by rows, one in flight, one being asked for.
 template <int DC, int RGS>
 struct BlocksKeyShape {
-    static constexpr uint32_t D = DC * 16, CPR = D / 8, ROWS = 32 * RGS, TENSOR = ROWS * D * 2, STAGE = 2 * TENSOR + ROWS * 16, LOADS = ROWS * D / 2048;
-    static constexpr uint32_t BUFFERS = 2 * TENSOR <= 32768 ? 3 : 2;
+    static constexpr uint32_t D = DC * 16, CPR = D / 8, ROWS = 32 * RGS, TENSOR = ROWS * D * 2, STAGE = 2 * TENSOR + 512, BUFFERS = 4;
 };
 
-template <bool BF16, int DC, int RGS>
+template <bool BF16, int DC, int ND, int RGS>
 __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_t words, uint32_t part_rows, uint32_t capacity, uint32_t slots, uint32_t groups,
                                                            uint32_t per_pair, const uint32_t* __restrict__ bits, const BlocksPart* __restrict__ parts,
-                                                           const uint32_t* __restrict__ used, const uint16_t* __restrict__ dout, const BlocksRowInfo* __restrict__ info,
+                                                           const uint32_t* __restrict__ used, const uint16_t* __restrict__ dout, BlocksRowInfo info,
                                                            uint16_t* __restrict__ dk, uint16_t* __restrict__ dv, float* __restrict__ partial) {
     TakeWholeRegisterFile();
     using W = BlocksWalkShape<DC>;
     using S = BlocksKeyShape<DC, RGS>;
-    constexpr int KS = DC / 2, D = DC * 16, ND = DC > 8 ? 2 : 1, OD = DC / ND;
-    extern __shared__ __attribute__((aligned(16))) char s_keys[];   // stages {Q rows, dO rows, row info}; afterwards the sums of the row groups; the row list behind
+    constexpr int KS = DC / 2, D = DC * 16, OD = DC / ND;
+    extern __shared__ __attribute__((aligned(16))) char s_keys[];   // stages {Q rows, dO rows, lse2, delta}; afterwards the sums of the row groups; the row list behind
     uint32_t* s_list = reinterpret_cast<uint32_t*>(s_keys + S::BUFFERS * S::STAGE);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     uint32_t pair, x;
@@ -379,51 +411,59 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
     if (item >= used[pair]) return;
     const BlocksPart part = parts[(uint64_t)pair * capacity + item];
     const uint32_t b = pair / a.Hkv, h = pair % a.Hkv, tpb = a.bs / 16, kts = min(4u, tpb - group * 4);
-    const int n = BlocksKvLen(a, b);
-    const uint32_t kt = wave % kts, hd = ND == 1 ? 0 : wave / kts % ND, rg = wave / (kts * ND);
-    const bool works = rg < RGS;   // wavefronts beyond kts * ND * RGS only load
+    const int n = BlocksKvLen(a, b), m = BlocksQLen(a, b);
+    const uint32_t kt = wave % kts, hd = wave / kts % ND, group_of = wave / (kts * ND);
+    const bool works = group_of < RGS;   // wavefronts beyond kts * ND * RGS load, and repeat another's products for nothing
+    const uint32_t rg = group_of % RGS;
     const uint32_t in_block = (group * 4 + kt) * 16;
     const int key = (int)(part.block * a.bs + in_block + r);
 
-    // the rows of this part: ranks [index * part_rows, ...) among the set bits; one wavefront counts its way there
-    __shared__ uint32_t s_rows;
-    if (threadIdx.x < 64) {
+    u32x4_t kf[KS], vf[KS];
+    const int last_row = n - 1 - (int)(part.block * a.bs);
+    if (last_row >= 0) {   // (a block behind the sequence's end has no query rows either)
+        int64_t ko, vo;
+        (void)BlocksBase(a, b, (int)part.block, ko, vo);
+        const int row = min((int)(in_block + r), last_row);
+        BlocksLoadRows<KS>(a.k + ko + h * a.ks[2] + row * a.ks[1] + g * 8, kf);
+        BlocksLoadRows<KS>(a.v + vo + h * a.vs[2] + row * a.vs[1] + g * 8, vf);
+    }
+    // the rows of this part: ranks [index * part_rows, ...) among the set bits, 512 words at a time
+    __shared__ uint32_t s_words[8];
+    uint32_t listed;
+    {
         const uint32_t* row_bits = bits + ((uint64_t)pair * a.nblk + part.block) * words;
         const uint32_t lo = part.index * part_rows, hi = lo + part_rows;
         uint32_t before = 0;
-        for (uint32_t w0 = 0; w0 < words && before < hi; w0 += 64) {
-            uint32_t w = w0 + lane < words ? row_bits[w0 + lane] : 0u;
+        for (uint32_t w0 = 0; w0 < words && before < hi; w0 += 512) {
+            uint32_t w = w0 + threadIdx.x < words ? row_bits[w0 + threadIdx.x] : 0u;
             const uint32_t c = (uint32_t)__popc(w);
             uint32_t sum = c;
             for (int s = 1; s < 64; s <<= 1) {
                 const uint32_t y = __shfl_up(sum, s);
                 if ((int)lane >= s) sum += y;
             }
+            if (lane == 63) s_words[wave] = sum;
+            __syncthreads();
             uint32_t rank = before + sum - c;
+            for (uint32_t y = 0; y < 8; ++y) {
+                if (y < wave) rank += s_words[y];
+                before += s_words[y];
+            }
             while (w) {
-                if (rank >= lo && rank < hi) s_list[rank - lo] = (w0 + lane) * 32 + (uint32_t)__ffs(w) - 1;
+                if (rank >= lo && rank < hi) s_list[rank - lo] = (w0 + threadIdx.x) * 32 + (uint32_t)__ffs(w) - 1;
                 ++rank;
                 w &= w - 1;
             }
-            before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+            __syncthreads();
         }
-        if (lane == 0) s_rows = before > lo ? min(before, hi) - lo : 0;
+        listed = before > lo ? min(before, hi) - lo : 0;
     }
-    __syncthreads();
-    const uint32_t rows = s_rows * a.G, stages = (rows + S::ROWS - 1) / S::ROWS;
+    const uint32_t rows = listed * a.G, stages = (rows + S::ROWS - 1) / S::ROWS;
 
     f32x4_t ak[OD], av[OD];
 #pragma unroll
     for (int d = 0; d < OD; ++d) ak[d] = av[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     if (stages > 0) {
-        u32x4_t kf[KS], vf[KS];
-        {
-            int64_t ko, vo;
-            (void)BlocksBase(a, b, (int)part.block, ko, vo);
-            const int row = min((int)(in_block + r), n - 1 - (int)(part.block * a.bs));   // a probed block holds a visible row
-            BlocksLoadRows<KS>(a.k + ko + h * a.ks[2] + row * a.ks[1] + g * 8, kf);
-            BlocksLoadRows<KS>(a.v + vo + h * a.vs[2] + row * a.vs[1] + g * 8, vf);
-        }
         const float scale2 = a.scale2 == 0.f ? 1.f : fabsf(a.scale2);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -432,120 +472,193 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
         }
         const BlocksWalkAddresses<DC> ad(lane);
         const uint32_t lds = BlocksLdsAddress(s_keys);
-        auto row_of = [&](uint32_t s, uint32_t row, uint32_t& t, uint32_t& head) {
-            const uint32_t rr = min(s * S::ROWS + row, rows - 1);
-            t = s_list[rr / a.G];
-            head = h * a.G + rr % a.G;
-        };
-        auto load = [&](uint32_t s, uint32_t to) {
+        // Row i of the part: query row list[i / G], head i % G of the group.  A wavefront asks for PER / 8 pieces of 64 / CPR rows of both tensors a stage,
+        // the last one for the rows' numbers too; `place`: what a lane adds to a row's address.
+        constexpr uint32_t PER = S::ROWS * S::CPR / 64, PIECES = (PER + 7) / 8;
+        const uint32_t inverse = a.G > 1 ? 0xFFFFFFFFu / a.G + 1 : 0;
+        const char* q0 = reinterpret_cast<const char*>(a.q + b * a.qs[0] + (int64_t)h * a.G * a.qs[2]);
+        const char* o0 = reinterpret_cast<const char*>(dout + b * a.os[0] + (int64_t)h * a.G * a.os[2]);
+        const uint32_t qrow = (uint32_t)a.qs[1] * 2, orow = (uint32_t)a.os[1] * 2, qhead = (uint32_t)a.qs[2] * 2, ohead = (uint32_t)a.os[2] * 2;
+        uint32_t piece_row[PIECES], place[PIECES];
 #pragma unroll
-            for (uint32_t y = 0; y < S::LOADS; ++y) {
-                const uint32_t j = wave + 8 * y, per = S::ROWS * S::CPR / 64, at = j % per * 64 + lane, row = at / S::CPR;
-                uint32_t t, head;
-                row_of(s, row, t, head);
-                const bool grad = j >= per;
-                const uint16_t* src = grad ? dout + b * a.os[0] + t * a.os[1] + head * a.os[2] : a.q + b * a.qs[0] + t * a.qs[1] + head * a.qs[2];
-                BlocksDmaFrom(src + W::Chunk(at % S::CPR, row % 16) * 8, to + (grad ? S::TENSOR : 0) + j % per * 1024);
-            }
-            if (wave < (S::ROWS + 63) / 64) {   // the rows' info, 16 bytes a lane
-                uint32_t t, head;
-                row_of(s, min(wave * 64 + lane, S::ROWS - 1), t, head);
-                if (S::ROWS >= 64 || lane < S::ROWS) BlocksDmaFrom(info + ((int64_t)b * a.Tq + t) * a.Hq + head, to + 2 * S::TENSOR + wave * 1024);
+        for (uint32_t y = 0; y < PIECES; ++y) {
+            const uint32_t at = (wave + 8 * y) * 64 + lane;
+            piece_row[y] = at / S::CPR;
+            place[y] = W::Chunk(at % S::CPR, piece_row[y] % 16) * 16;
+        }
+        auto row_of = [&](uint32_t i, uint32_t& t, uint32_t& head) {
+            const uint32_t in = inverse ? __umulhi(i, inverse) : i;   // i / G, exact below 2^16
+            t = s_list[in];
+            head = i - in * a.G;
+        };
+        auto load_rows = [&](uint32_t s, uint32_t y, uint32_t to) {
+            const uint32_t j = wave + 8 * y;
+            if (PER % 8 != 0 && j >= PER) return;
+            uint32_t t, head;
+            row_of(min(s * S::ROWS + piece_row[y], rows - 1), t, head);
+            const uint64_t dq_at = (uint64_t)head * qhead + place[y], do_at = (uint64_t)head * ohead + place[y];
+            BlocksDmaFrom(q0 + ((uint64_t)t * qrow + dq_at), to + j * 1024);
+            BlocksDmaFrom(o0 + ((uint64_t)t * orow + do_at), to + S::TENSOR + j * 1024);
+        };
+        auto load_info = [&](uint32_t s, uint32_t to) {
+            if (wave != 7) return;
+            const uint32_t i = s * S::ROWS + lane;
+            uint32_t t, head;
+            row_of(min(i, rows - 1), t, head);
+            const uint32_t at = i < rows ? ((b * a.Tq + t) * a.Hq + h * a.G + head) : a.B * a.Tq * a.Hq;   // a row that weighs nothing (checked: below 2^32)
+            if (lane < S::ROWS) {
+                BlocksDmaWordFrom(info.lse2 + at, to + 2 * S::TENSOR);
+                BlocksDmaWordFrom(info.delta + at, to + 2 * S::TENSOR + 256);
             }
         };
-        const bool extra = wave < (S::ROWS + 63) / 64;
-        for (uint32_t s = 0; s + 1 < S::BUFFERS && s < stages; ++s) load(s, lds + s * S::STAGE);
-        uint32_t buf = 0;
-        for (uint32_t s = 0; s < stages; ++s) {
-            if (S::BUFFERS > 2 && s + 1 < stages) {
-                if (extra)
-                    BlocksDmaWait<(S::BUFFERS - 2) * (S::LOADS + 1)>();
-                else
-                    BlocksDmaWait<(S::BUFFERS - 2) * S::LOADS>();
-            } else {
-                BlocksDmaWait<0>();
-            }
+        const uint32_t mine = 2 * (PER / 8 + (wave < PER % 8 ? 1 : 0)) + (wave == 7 ? 2 : 0);   // DMA instructions of this wavefront per stage
+        for (uint32_t s = 0; s + 1 < S::BUFFERS && s < stages; ++s) {
+            for (uint32_t y = 0; y < (PER + 7) / 8; ++y) load_rows(s, y, lds + s * S::STAGE);
+            load_info(s, lds + s * S::STAGE);
+        }
+        auto wait = [&](uint32_t s, uint32_t behind) {   // until stage s has landed, with `behind` stages after it in flight (if there are as many)
+            BlocksDmaWaitFor(mine * min(behind, stages - 1 - min(s, stages - 1)));
             BlocksStageBarrier();
-            if (s + S::BUFFERS - 1 < stages) load(s + S::BUFFERS - 1, lds + (buf == 0 ? S::BUFFERS - 1 : buf - 1) * S::STAGE);
-            if (works && s * S::ROWS + rg * 32 < rows) {
-                constexpr uint32_t TILE = D * 32;
-                const uint32_t at = lds + buf * S::STAGE + rg * 2 * TILE;
-                f32x4_t p[2], ds[2];
-                {
-                    u32x4_t qr[2][KS];
+        };
+        // LDS addresses of this lane's operands: everything but the stage is a constant offset
+        uint32_t by_rows[KS], turned[OD], by_info = lds + 2 * S::TENSOR + (rg * 32 + g * 4) * 4;
 #pragma unroll
-                    for (int j = 0; j < KS; ++j)
+        for (int j = 0; j < KS; ++j) by_rows[j] = lds + rg * 2 * D * 32 + ad.rows[j];
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) qr[y][j] = BlocksReadRow(at + ad.rows[j] + y * TILE);
-                    __builtin_amdgcn_sched_barrier(0);
+        for (int d = 0; d < OD; ++d) turned[d] = lds + rg * 2 * D * 32 + ad.turned[hd * OD + d];
+        auto rows_of = [&](uint32_t stage, uint32_t tensor, u32x4_t(&f)[2][KS]) {
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) p[y] = ds[y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < KS; ++j) {
+                uint32_t at = by_rows[j] + stage;
+                asm volatile("" : "+v"(at));
 #pragma unroll
-                    for (int j = 0; j < KS; ++j)
+                for (int y = 0; y < 2; ++y) f[y][j] = BlocksReadRow(at + tensor + y * D * 32);
+            }
+        };
+        auto turned_of = [&](uint32_t stage, uint32_t tensor, u32x2_t(&f)[OD][2]) {
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) p[y] = BlocksMfma<BF16>(qr[y][j], kf[j], p[y]);
+            for (int d = 0; d < OD; ++d) {
+                uint32_t at = turned[d] + stage;
+                asm volatile("" : "+v"(at));
 #pragma unroll
-                    for (int j = 0; j < KS; ++j)
+                for (int y = 0; y < 2; ++y) f[d][y] = BlocksReadTransposed(at + tensor + y * D * 32);
+            }
+        };
+        auto product = [&](const u32x4_t(&f)[2][KS], const u32x4_t(&keys)[KS], f32x4_t(&x)[2]) {
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) qr[y][j] = BlocksReadRow(at + ad.rows[j] + S::TENSOR + y * TILE);
-                    __builtin_amdgcn_sched_barrier(0);
+            for (int y = 0; y < 2; ++y) x[y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = 0; j < KS; ++j)
+            for (int j = 0; j < KS; ++j)
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) ds[y] = BlocksMfma<BF16>(qr[y][j], vf[j], ds[y]);
+                for (int y = 0; y < 2; ++y) x[y] = BlocksMfma<BF16>(f[y][j], keys[j], x[y]);
+        };
+        // The four products of a stage in a pipeline: while stage s's weights are computed, stage s + 1's logits are on the matrix cores.  LDS reads go out a
+        // phase before the products that use them; the scheduling barriers keep the phases, inside one the compiler interleaves.
+        // rows of this part that do not see the whole block: at most a block's query rows, the first of the list (and none but partly visible keys: the end)
+        const int block_end = min((int)((part.block + 1) * a.bs), n);
+        const bool tail = (int)((part.block + 1) * a.bs) > n;
+        uint32_t partly = tail ? rows : 0;
+        if (a.causal && !tail) partly = BlocksVisible(a, n, m, (int)s_list[0]) < block_end ? min(rows, a.bs * a.G) : 0;
+        f32x4_t p[2], ds[2];
+        u32x4_t dso = {0u, 0u, 0u, 0u};   // of the stage before: its part of the keys' sums is added behind the next barrier, while the first reads are on their way
+        u32x2_t qt[OD][2];
+#pragma unroll
+        for (int d = 0; d < OD; ++d) qt[d][0] = qt[d][1] = u32x2_t{0u, 0u};
+        auto add_keys = [&]() {
+#pragma unroll
+            for (int d = 0; d < OD; ++d) ak[d] = BlocksMfma<BF16>(dso, u32x4_t{qt[d][0][0], qt[d][0][1], qt[d][1][0], qt[d][1][1]}, ak[d]);
+        };
+        wait(0, 2);
+        {
+            u32x4_t f[2][KS];
+            rows_of(0, 0, f);
+            product(f, kf, p);
+            rows_of(0, S::TENSOR, f);
+            product(f, vf, ds);
+        }
+        for (uint32_t s = 0; s < stages; ++s) {
+            const uint32_t stage = (s & 3) * S::STAGE, next = ((s + 1) & 3) * S::STAGE, to = lds + ((s + 3) & 3) * S::STAGE;
+            const bool more = s + 3 < stages;
+            wait(s + 1, 1);   // (behind the last stage: rows of an earlier one, whose products nobody uses)
+            u32x4_t f[2][KS], f1[2][KS], about[2][2];   // lse2 and delta of the lane's eight rows
+            u32x2_t ot[OD][2];
+            f32x4_t p1[2], ds1[2];
+            rows_of(next, 0, f);
+            {
+                uint32_t at = by_info + stage;
+                asm volatile("" : "+v"(at));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) about[i >> 1][i & 1] = BlocksReadRow(at + (i >> 1) * 256 + (i & 1) * 64);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            add_keys();
+            __builtin_amdgcn_sched_barrier(0);
+            rows_of(next, S::TENSOR, f1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) load_rows(s + 3, 0, to);
+            __builtin_amdgcn_sched_barrier(0);
+            product(f, kf, p1);
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    p[y][i] = BlocksExp2(__builtin_fmaf(p[y][i], scale2, -__uint_as_float(about[0][y][i])));
+                    ds[y][i] = p[y][i] * (ds[y][i] - __uint_as_float(about[1][y][i]));
                 }
-                u32x4_t about[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) about[i] = BlocksReadRow(lds + buf * S::STAGE + 2 * S::TENSOR + (rg * 32 + (i >> 2) * 16 + g * 4 + (i & 3)) * 16);
-                u32x2_t ot[OD][2], qt[OD][2];
-#pragma unroll
-                for (int d = 0; d < OD; ++d)
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) ot[d][y] = BlocksReadTransposed(at + ad.turned[hd * OD + d] + S::TENSOR + y * TILE);
-                __builtin_amdgcn_sched_barrier(0);
+            // the first rows of the list may see only a part of the block
+            if (s * S::ROWS < partly) {
 #pragma unroll
                 for (int y = 0; y < 2; ++y)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const u32x4_t& row = about[y * 4 + i];
-                        const bool ok = key < (int)row[2] && s * S::ROWS + rg * 32 + y * 16 + g * 4 + i < rows;
-                        const float e = BlocksExp2(__builtin_fmaf(p[y][i], scale2, -__uint_as_float(row[0])));
-                        p[y][i] = ok ? e : 0.f;
-                        ds[y][i] = ok ? e * (ds[y][i] - __uint_as_float(row[1])) : 0.f;
+                        const uint32_t row = min(s * S::ROWS + rg * 32 + y * 16 + g * 4 + i, rows - 1), in = inverse ? __umulhi(row, inverse) : row;
+                        const bool ok = key < BlocksVisible(a, n, m, (int)s_list[in]);
+                        p[y][i] = ok ? p[y][i] : 0.f;
+                        ds[y][i] = ok ? ds[y][i] : 0.f;
                     }
-                const u32x4_t po = BlocksPackOperand<BF16>(p[0], p[1]), dso = BlocksPackOperand<BF16>(ds[0], ds[1]);
-#pragma unroll
-                for (int d = 0; d < OD; ++d)
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) qt[d][y] = BlocksReadTransposed(at + ad.turned[hd * OD + d] + y * TILE);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int d = 0; d < OD; ++d) av[d] = BlocksMfma<BF16>(po, u32x4_t{ot[d][0][0], ot[d][0][1], ot[d][1][0], ot[d][1][1]}, av[d]);
-#pragma unroll
-                for (int d = 0; d < OD; ++d) ak[d] = BlocksMfma<BF16>(dso, u32x4_t{qt[d][0][0], qt[d][0][1], qt[d][1][0], qt[d][1][1]}, ak[d]);
             }
-            buf = buf + 1 == S::BUFFERS ? 0 : buf + 1;
+            __builtin_amdgcn_sched_barrier(0);
+            turned_of(stage, S::TENSOR, ot);
+            __builtin_amdgcn_sched_barrier(0);
+            const u32x4_t po = BlocksPackOperand<BF16>(p[0], p[1]);
+            dso = BlocksPackOperand<BF16>(ds[0], ds[1]);
+            product(f1, vf, ds1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) {
+#pragma unroll
+                for (uint32_t y = 1; y < (PER + 7) / 8; ++y) load_rows(s + 3, y, to);
+                load_info(s + 3, to);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            turned_of(stage, 0, qt);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < OD; ++d) av[d] = BlocksMfma<BF16>(po, u32x4_t{ot[d][0][0], ot[d][0][1], ot[d][1][0], ot[d][1][1]}, av[d]);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                p[y] = p1[y];
+                ds[y] = ds1[y];
+            }
         }
+        add_keys();
     }
-    // row groups are added in their order, first the keys' sums, then the values'
-    float* s_add = reinterpret_cast<float*>(s_keys);
+    // the second row group's sums are added to the first's
+    if (RGS > 1) {
+        f32x4_t* s_add = reinterpret_cast<f32x4_t*>(s_keys) + (wave % (kts * ND)) * 2 * OD * 64 + lane;
+        __syncthreads();
+        if (works && rg == 1)
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        f32x4_t(&acc)[OD] = which ? av : ak;
-        for (uint32_t from = 1; from < RGS; ++from) {
-            __syncthreads();
-            if (works && rg == from)
+            for (int d = 0; d < OD; ++d) {
+                s_add[d * 64] = ak[d];
+                s_add[(OD + d) * 64] = av[d];
+            }
+        __syncthreads();
+        if (works && rg == 0)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int d = 0; d < OD; ++d) s_add[(kt * 16 + g * 4 + i) * D + (hd * OD + d) * 16 + r] = acc[d][i];
-            __syncthreads();
-            if (works && rg == 0)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int d = 0; d < OD; ++d) acc[d][i] += s_add[(kt * 16 + g * 4 + i) * D + (hd * OD + d) * 16 + r];
-        }
+            for (int d = 0; d < OD; ++d) {
+                ak[d] += s_add[d * 64];
+                av[d] += s_add[(OD + d) * 64];
+            }
     }
     if (!works || rg != 0) return;
 #pragma unroll
@@ -622,7 +735,7 @@ BackwardSpace BackwardLayout(const BlocksArgs& a, uint32_t d) {
     };
     s.bits = take(blocks * s.words * 4);
     s.counts = take(blocks * 4);
-    s.info = take((size_t)a.B * a.Tq * a.Hq * sizeof(BlocksRowInfo));
+    s.info = take(((size_t)a.B * a.Tq * a.Hq + 1) * 8);
     s.parts = take(pairs * s.capacity * sizeof(BlocksPart));
     s.used = take(pairs * 4);
     s.first_slot = take(blocks * 4);
@@ -631,15 +744,15 @@ BackwardSpace BackwardLayout(const BlocksArgs& a, uint32_t d) {
     return s;
 }
 
-template <bool BF16, int DC, int RGS>
-gpann_status KeyGrad(const BlocksArgs& a, const BackwardSpace& s, const uint16_t* dout, uint16_t* dk, uint16_t* dv, char* ws, hipStream_t st) {
+template <bool BF16, int DC, int ND, int RGS>
+gpann_status KeyGrad(const BlocksArgs& a, const BackwardSpace& s, const uint16_t* dout, BlocksRowInfo info, uint16_t* dk, uint16_t* dv, char* ws, hipStream_t st) {
     using S = BlocksKeyShape<DC, RGS>;
     const uint32_t groups = (a.bs / 16 + 3) / 4;
     const uint64_t per_pair = (uint64_t)s.capacity * groups;
-    const size_t lds = std::max<size_t>(S::BUFFERS * S::STAGE, 64 * S::D * 4) + (size_t)std::min(s.part_rows, a.Tq) * 4;
-    return BlocksLaunch(BlocksKeyGradKernel<BF16, DC, RGS>, BlocksPairGrid((uint64_t)a.B * a.Hkv, per_pair), lds, st, a, s.words, s.part_rows, s.capacity, s.slots, groups,
+    const size_t lds = std::max<size_t>(S::BUFFERS * S::STAGE, RGS > 1 ? (size_t)64 * S::D * 8 : 0) + (size_t)std::min(s.part_rows, a.Tq) * 4;
+    return BlocksLaunch(BlocksKeyGradKernel<BF16, DC, ND, RGS>, BlocksPairGrid((uint64_t)a.B * a.Hkv, per_pair), lds, st, a, s.words, s.part_rows, s.capacity, s.slots, groups,
                         (uint32_t)per_pair, reinterpret_cast<const uint32_t*>(ws + s.bits), reinterpret_cast<const BlocksPart*>(ws + s.parts),
-                        reinterpret_cast<const uint32_t*>(ws + s.used), dout, reinterpret_cast<const BlocksRowInfo*>(ws + s.info), dk, dv,
+                        reinterpret_cast<const uint32_t*>(ws + s.used), dout, info, dk, dv,
                         reinterpret_cast<float*>(ws + s.partial));
 }
 
@@ -650,23 +763,27 @@ gpann_status Backward(const BlocksArgs& a, const uint16_t* out, const float* lse
     uint32_t* counts = reinterpret_cast<uint32_t*>(ws + s.counts);
     int* first_slot = reinterpret_cast<int*>(ws + s.first_slot);
     const uint64_t pairs = (uint64_t)a.B * a.Hkv;
+    BlocksRowInfo info;
+    info.lse2 = reinterpret_cast<float*>(ws + s.info);
+    info.delta = info.lse2 + (uint64_t)a.B * a.Tq * a.Hq + 1;
     if (a.Tq > 0) {
         const uint32_t mtiles = (a.G + 15) / 16, tpw = std::max(1u, 16 / a.G);
         const uint64_t waves = mtiles > 1 ? (uint64_t)a.Tq * mtiles : (a.Tq + tpw - 1) / tpw, tiles = (waves + 7) / 8;
         GPANN_TRY(BlocksLaunch(BlocksQueryGradKernel<BF16, DC>, BlocksPairGrid(pairs, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, dout, lse,
-                               dq, reinterpret_cast<BlocksRowInfo*>(ws + s.info)));
+                               dq, info));
     }
     if (a.Tk == 0) return GPANN_OK;
-    GPANN_TRY(BlocksMarkProbes(a, s.words, reinterpret_cast<uint32_t*>(ws + s.bits), counts, st));
-    hipLaunchKernelGGL(BlocksPartsKernel, dim3((uint32_t)pairs), dim3(256), 0, st, a, s.part_rows, s.capacity, counts, reinterpret_cast<BlocksPart*>(ws + s.parts),
-                       reinterpret_cast<uint32_t*>(ws + s.used), first_slot);
+    uint32_t* bits = reinterpret_cast<uint32_t*>(ws + s.bits);
+    if (a.Tq > 0) GPANN_TRY(BlocksMarkProbes(a, s.words, bits, st));
+    hipLaunchKernelGGL(BlocksPartsKernel, dim3((uint32_t)pairs), dim3(1024), 0, st, a, s.words, s.part_rows, s.capacity, bits, counts,
+                       reinterpret_cast<BlocksPart*>(ws + s.parts), reinterpret_cast<uint32_t*>(ws + s.used), first_slot, info);
     GPANN_HIP_TRY(hipGetLastError());
-    // wavefronts beside the block's (up to four) 16-key tiles take more rows at a time
-    constexpr int most = DC > 8 ? 1 : 2;
-    if (a.bs <= 32)
-        GPANN_TRY((KeyGrad<BF16, DC, 2 * most>(a, s, dout, dk, dv, ws, st)));
+    if constexpr (DC > 8)
+        GPANN_TRY((KeyGrad<BF16, DC, 2, 1>(a, s, dout, info, dk, dv, ws, st)));
+    else if (a.bs <= 32)
+        GPANN_TRY((KeyGrad<BF16, DC, 2, 2>(a, s, dout, info, dk, dv, ws, st)));
     else
-        GPANN_TRY((KeyGrad<BF16, DC, most>(a, s, dout, dk, dv, ws, st)));
+        GPANN_TRY((KeyGrad<BF16, DC, 1, 2>(a, s, dout, info, dk, dv, ws, st)));
     if (s.slots > 0) {
         hipLaunchKernelGGL(BlocksKeyGradJoinKernel<BF16>, dim3(a.nblk, (uint32_t)pairs), dim3(256), 0, st, a, DC * 16, s.part_rows, s.slots, counts, first_slot,
                            reinterpret_cast<const float*>(ws + s.partial), dk, dv);
@@ -700,6 +817,7 @@ extern "C" gpann_status gpann_blocks_attend_backward(const gpann_blocks_layout* 
     GPANN_REQUIRE(BlocksDisjoint(L->k_stride, L->batch, L->kv_rows, L->kv_heads, L->head_dim), "dk overlaps itself");
     GPANN_REQUIRE(BlocksDisjoint(L->v_stride, L->batch, L->kv_rows, L->kv_heads, L->head_dim), "dv overlaps itself");
     GPANN_REQUIRE((uint64_t)L->batch * L->kv_heads <= 65535, "more than 65535 (sequence, head) pairs");
+    GPANN_REQUIRE((uint64_t)L->batch * L->q_rows * L->q_heads < 0xFFFFFFFFull, "2^32 - 1 (query row, head) rows or more");
     const BlocksArgs a = BlocksMakeArgs(L, q, k, v, probes, nprobe);
     GPANN_TRY(BlocksCheckWorkspace(workspace, workspace_bytes, BackwardLayout(a, L->head_dim).total));
     GPANN_BLOCKS_ENTER(L, stream);

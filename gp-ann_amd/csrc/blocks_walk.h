@@ -49,9 +49,24 @@ __device__ __forceinline__ void BlocksDma(uint64_t base, uint32_t offset, uint32
 __device__ __forceinline__ void BlocksDmaFrom(const void* src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "m0", "memory");
 }
+// ... 4 bytes a lane, to LDS bytes [lds, lds + 256)
+__device__ __forceinline__ void BlocksDmaWordFrom(const void* src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(src), "s"(lds) : "m0", "memory");
+}
 template <int LEFT>
 __device__ __forceinline__ void BlocksDmaWait() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LEFT) : "memory");
+}
+// the same for a number known at run time (at most 16: with more in flight than that, until 16 are)
+__device__ __forceinline__ void BlocksDmaWaitFor(uint32_t left) {
+    switch (left) {
+#define GPANN_WAIT(n) \
+    case n: BlocksDmaWait<n>(); break;
+        GPANN_WAIT(0) GPANN_WAIT(1) GPANN_WAIT(2) GPANN_WAIT(3) GPANN_WAIT(4) GPANN_WAIT(5) GPANN_WAIT(6) GPANN_WAIT(7) GPANN_WAIT(8) GPANN_WAIT(9)
+        GPANN_WAIT(10) GPANN_WAIT(11) GPANN_WAIT(12) GPANN_WAIT(13) GPANN_WAIT(14) GPANN_WAIT(15)
+        default: BlocksDmaWait<16>();
+#undef GPANN_WAIT
+    }
 }
 // every wavefront has its share of a stage in LDS and has read what it needs of the stage before
 __device__ __forceinline__ void BlocksStageBarrier() {
