@@ -135,84 +135,260 @@ __device__ __forceinline__ uint64_t BlocksScoreKey(double x) {
     return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
-// One workgroup per (query row, key/value head, sequence).  Scores in binary64 because a selection has to come out the same whatever the order of a sum:
-// neighbouring scores differ by far more than 2^-50.  Sixteen lanes share a block's centroid.  The nprobe-th best key is found by bisection over the
-// 64 key bits — every thread counts the keys it wrote — and the blocks that reach it are written in block order.
-template <bool BF16>
-__global__ void __launch_bounds__(256) BlocksRouteKernel(BlocksArgs a, uint32_t d, const float* __restrict__ summary, uint32_t first, uint32_t last,
-                                                         int32_t* __restrict__ probes) {
-    extern __shared__ double s_route[];
-    double* s_q = s_route;                                            // [d]
-    uint64_t* s_key = reinterpret_cast<uint64_t*>(s_route + d);       // [blocks]
-    __shared__ uint32_t s_count[4];
-    const uint32_t b = blockIdx.z, h = blockIdx.y, t = blockIdx.x;
-    const int n = BlocksKvLen(a, b), m = BlocksQLen(a, b);
-    if ((int)t >= m) return;
-    const int visible = BlocksVisible(a, n, m, t);
-    const uint32_t nb = (uint32_t)(visible + (int)a.bs - 1) / a.bs;
-    int32_t* out = probes + (((int64_t)b * a.Tq + t) * a.Hkv + h) * a.P;
-    if (nb <= a.P) {
-        for (uint32_t j = threadIdx.x; j < a.P; j += 256) out[j] = j < nb ? (int32_t)j : -1;
-        return;
-    }
-    for (uint32_t c = threadIdx.x; c < d; c += 256) {
-        const uint16_t* p = a.q + b * a.qs[0] + t * a.qs[1] + (int64_t)h * a.G * a.qs[2] + c;
-        double x = 0;
-        for (uint32_t g = 0; g < a.G; ++g) x += BlocksToDouble(p[g * a.qs[2]], BF16);
-        s_q[c] = x;
-    }
-    __syncthreads();
-    const float* cen = summary + ((int64_t)b * a.Hkv + h) * a.nblk * d;
-    const uint32_t sub = threadIdx.x & 15;
-    for (uint32_t j0 = 0; j0 < nb; j0 += 16) {
-        const uint32_t j = j0 + threadIdx.x / 16;
-        double x = 0;
-        if (j < nb) {
-            const float* c = cen + (int64_t)j * d;
-            for (uint32_t i = sub * 4; i < d; i += 64) {
-                const float4 v = *reinterpret_cast<const float4*>(c + i);
-                const double* qq = s_q + i;
-                x = fma(qq[0], (double)v.x, x);
-                x = fma(qq[1], (double)v.y, x);
-                x = fma(qq[2], (double)v.z, x);
-                x = fma(qq[3], (double)v.w, x);
+// The nprobe best of a query row's `nb` blocks, by one wavefront (REGS keys a lane, or from LDS): bisection over the upper 32 key bits — 32-bit comparisons,
+// counts on the scalar unit — until a threshold parts exactly P blocks from the rest; blocks that agree in those bits are told apart by the lower 32; of equal
+// keys the lowest blocks stay.  Probes come out in block order.
+template <int REGS>
+__device__ __forceinline__ void BlocksSelect(const uint64_t* s_key, uint32_t nb, uint32_t P, uint32_t first, uint32_t last, uint32_t lane, int32_t* out) {
+    constexpr int N = REGS > 0 ? REGS : 1;
+    uint32_t hi[N], lo[N];
+    auto key = [&](uint32_t j) -> uint64_t { return j >= nb ? 0 : (j < first || j + last >= nb) ? ~0ull : s_key[j]; };
+    if (REGS > 0)
+#pragma unroll
+        for (int i = 0; i < REGS; ++i) {
+            const uint64_t k = key(i * 64 + lane);
+            hi[i] = (uint32_t)(k >> 32);
+            lo[i] = (uint32_t)k;
+        }
+    const uint32_t rounds = REGS > 0 ? REGS : (nb + 63) / 64;
+    auto each = [&](auto&& f) {   // f(round, block, hi, lo) for all of a lane's keys
+        if (REGS > 0) {
+#pragma unroll
+            for (int i = 0; i < REGS; ++i) f(i, i * 64 + lane, hi[i], lo[i]);
+        } else {
+            for (uint32_t i = 0; i < rounds; ++i) {
+                const uint64_t k = key(i * 64 + lane);
+                f(i, i * 64 + lane, (uint32_t)(k >> 32), (uint32_t)k);
             }
         }
-        for (int s = 8; s > 0; s >>= 1) x += __shfl_xor(x, s);
-        if (sub == 0 && j < nb) s_key[j] = (j < first || j + last >= nb) ? ~0ull : BlocksScoreKey(x);
-    }
-    __syncthreads();
-    // largest key v with count(key >= v) >= P
-    uint64_t v = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-        const uint64_t trial = v | (1ull << bit);
+    };
+    uint32_t v = 0, w = 0;
+    bool exact = false;
+    for (uint32_t bit = 1u << 31; bit && !exact; bit >>= 1) {
+        const uint32_t trial = v | bit;
         uint32_t c = 0;
-        for (uint32_t j = threadIdx.x; j < nb; j += 256) c += s_key[j] >= trial;
-        for (int s = 32; s > 0; s >>= 1) c += __shfl_xor(c, s);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) s_count[threadIdx.x >> 6] = c;
-        __syncthreads();
-        c = s_count[0] + s_count[1] + s_count[2] + s_count[3];
-        if (c >= a.P) v = trial;
-        if (c == a.P) break;
+        each([&](int, uint32_t, uint32_t x, uint32_t) { c += (uint32_t)__popcll(__ballot(x >= trial)); });
+        if (c >= P) v = trial;
+        exact = c == P;
     }
-    // blocks above v all stay; of those equal to v the lowest.  One wavefront walks the blocks in order.
-    if (threadIdx.x < 64) {
-        const uint32_t lane = threadIdx.x;
-        uint32_t above = 0;
-        for (uint32_t j0 = 0; j0 < nb; j0 += 64) above += (uint32_t)__popcll(__ballot(j0 + lane < nb && s_key[min(j0 + lane, nb - 1)] > v));
-        uint32_t equal = a.P - above, at = 0;
-        for (uint32_t j0 = 0; j0 < nb && at < a.P; j0 += 64) {
-            const uint64_t key = s_key[min(j0 + lane, nb - 1)];
-            const bool in = j0 + lane < nb, gt = in && key > v, eq = in && key == v;
-            const uint64_t below = (1ull << lane) - 1, eqs = __ballot(eq);
-            const bool take = gt || (eq && (uint32_t)__popcll(eqs & below) < equal);
-            const uint64_t taken = __ballot(take);
-            if (take) out[at + (uint32_t)__popcll(taken & below)] = (int32_t)(j0 + lane);
-            at += (uint32_t)__popcll(taken);
-            equal -= min(equal, (uint32_t)__popcll(eqs));
+    if (!exact) {   // (v = 0: all keys reach it)
+        for (uint32_t bit = 1u << 31; bit && !exact; bit >>= 1) {
+            const uint32_t trial = w | bit;
+            uint32_t c = 0;
+            each([&](int, uint32_t j, uint32_t x, uint32_t y) { c += (uint32_t)__popcll(__ballot(j < nb && (x > v || (x == v && y >= trial)))); });
+            if (c >= P) w = trial;
+            exact = c == P;
         }
     }
+    const uint64_t below = (1ull << lane) - 1;
+    uint32_t at = 0, equal = 0;
+    if (!exact) {   // more than P reach the threshold: the lowest of those that equal it fill up
+        uint32_t above = 0;
+        each([&](int, uint32_t, uint32_t x, uint32_t y) { above += (uint32_t)__popcll(__ballot(x > v || (x == v && y > w))); });
+        equal = P - above;
+    }
+    each([&](int, uint32_t j, uint32_t x, uint32_t y) {
+        bool take = j < nb && (x > v || (x == v && y >= w));
+        if (!exact) {
+            const bool eq = j < nb && x == v && y == w;
+            const uint64_t eqs = __ballot(eq);
+            if (eq) take = (uint32_t)__popcll(eqs & below) < equal;
+            equal -= min(equal, (uint32_t)__popcll(eqs));
+        }
+        const uint64_t taken = __ballot(take);
+        if (take) out[at + (uint32_t)__popcll(taken & below)] = (int32_t)j;
+        at += (uint32_t)__popcll(taken);
+    });
+}
+
+// Scores in binary64, because a selection has to come out the same whatever the order of a sum: neighbouring scores differ by far more than 2^-50.  The
+// products run on the binary64 matrix instruction (16 x 16 x 4, the vector unit's rate without its operand traffic; C: column l % 16, rows 4 i + l / 16): a
+// wavefront holds the sums of `tokens` <= 16 query rows (lane: row l % 16, every fourth four dimensions) and takes 16 blocks' centroids at a time straight from
+// memory; keys wait in LDS until the wavefronts turn to selecting, a query row each.  A workgroup has `groups` sets of query rows, whose blocks 8 / groups
+// wavefronts divide.
+template <bool BF16, int DC>
+__global__ void __launch_bounds__(512) BlocksRouteKernel(BlocksArgs a, uint32_t groups, uint32_t tokens, uint32_t tiles, const float* __restrict__ summary,
+                                                         uint32_t first, uint32_t last, int32_t* __restrict__ probes) {
+    TakeWholeRegisterFile();
+    constexpr int D = DC * 16, K = D / 4;
+    typedef double f64x4_t __attribute__((ext_vector_type(4)));
+    extern __shared__ uint64_t s_key[];   // [query row of the workgroup][block]
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    uint32_t pair, tile;
+    if (!BlocksPairOf(blockIdx.x, a.B * a.Hkv, tiles, pair, tile)) return;
+    const uint32_t b = pair / a.Hkv, h = pair % a.Hkv, parts = 8 / groups, group = wave / parts, part = wave % parts;
+    const int n = BlocksKvLen(a, b), m = BlocksQLen(a, b);
+    const uint32_t row0 = (tiles - 1 - tile) * groups * tokens, t0 = row0 + group * tokens;
+    const uint32_t live = (int)t0 < m ? min(tokens, (uint32_t)m - t0) : 0;
+    const uint32_t blocks = live ? (uint32_t)(BlocksVisible(a, n, m, (int)(t0 + live - 1)) + (int)a.bs - 1) / a.bs : 0;
+    const float* cen = summary + (uint64_t)pair * a.nblk * D + g * 4;   // this lane's dimensions: 16 i + 4 g ..
+    if (part * 16 < blocks && blocks > a.P) {
+        double q[K];
+#pragma unroll
+        for (int i = 0; i < K; ++i) q[i] = 0;
+        if (r < live) {
+            const uint16_t* p = a.q + b * a.qs[0] + (int64_t)(t0 + r) * a.qs[1] + (int64_t)h * a.G * a.qs[2] + g * 4;
+            uint2 y[K / 4];
+#pragma unroll
+            for (int i = 0; i < K / 4; ++i) y[i] = *reinterpret_cast<const uint2*>(p + i * 16);
+            for (uint32_t x = 1;; ++x) {   // the next head's numbers are on their way while one's are added
+                uint2 z[K / 4];
+                const uint16_t* after = p + min(x, a.G - 1) * a.qs[2];
+#pragma unroll
+                for (int i = 0; i < K / 4; ++i) z[i] = *reinterpret_cast<const uint2*>(after + i * 16);
+#pragma unroll
+                for (int i = 0; i < K / 4; ++i) {
+                    q[4 * i] += BlocksToDouble((uint16_t)y[i].x, BF16);
+                    q[4 * i + 1] += BlocksToDouble((uint16_t)(y[i].x >> 16), BF16);
+                    q[4 * i + 2] += BlocksToDouble((uint16_t)y[i].y, BF16);
+                    q[4 * i + 3] += BlocksToDouble((uint16_t)(y[i].y >> 16), BF16);
+                    y[i] = z[i];
+                }
+                if (x >= a.G) break;
+            }
+        }
+        float4 c[K / 4], next[K / 4];
+        auto load = [&](uint32_t j0, float4(&to)[K / 4]) {
+            const float* p = cen + (uint64_t)min(j0 + r, blocks - 1) * D;
+#pragma unroll
+            for (int i = 0; i < K / 4; ++i) to[i] = *reinterpret_cast<const float4*>(p + i * 16);
+        };
+        load(part * 16, c);
+        for (uint32_t j0 = part * 16; j0 < blocks; j0 += parts * 16) {
+            load(j0 + parts * 16, next);   // (of no use behind the last blocks; a load under a branch would be waited for at once)
+            f64x4_t x = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < K / 4; ++i) {
+                x = __builtin_amdgcn_mfma_f64_16x16x4f64(q[4 * i], (double)c[i].x, x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f64_16x16x4f64(q[4 * i + 1], (double)c[i].y, x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f64_16x16x4f64(q[4 * i + 2], (double)c[i].z, x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f64_16x16x4f64(q[4 * i + 3], (double)c[i].w, x, 0, 0, 0);
+            }
+            if (j0 + r < blocks)
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+                    if (i * 4 + g < live) s_key[(uint64_t)(group * tokens + i * 4 + g) * a.nblk + j0 + r] = BlocksScoreKey(x[i]);
+#pragma unroll
+            for (int i = 0; i < K / 4; ++i) c[i] = next[i];
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = wave; i < groups * tokens; i += 8) {
+        const uint32_t t = row0 + i;
+        if ((int)t >= m) break;
+        const uint32_t nb = (uint32_t)(BlocksVisible(a, n, m, (int)t) + (int)a.bs - 1) / a.bs;
+        int32_t* out = probes + (((int64_t)b * a.Tq + t) * a.Hkv + h) * a.P;
+        if (nb <= a.P) {
+            if (lane < a.P) out[lane] = lane < nb ? (int32_t)lane : -1;
+        } else if (nb <= 128) {
+            BlocksSelect<2>(s_key + (uint64_t)i * a.nblk, nb, a.P, first, last, lane, out);
+        } else if (nb <= 512) {
+            BlocksSelect<8>(s_key + (uint64_t)i * a.nblk, nb, a.P, first, last, lane, out);
+        } else {
+            BlocksSelect<0>(s_key + (uint64_t)i * a.nblk, nb, a.P, first, last, lane, out);
+        }
+    }
+}
+
+// lane ^ 1, ^ 2, and the mirrors of 8 and 16 lanes: a sum over 16 lanes on the vector unit
+template <int CTRL>
+__device__ __forceinline__ double BlocksAddLane(double x) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+    return x + __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+}
+__device__ __forceinline__ double BlocksSumOver16(double x) {
+    x = BlocksAddLane<0xB1>(x);    // quad_perm 1 0 3 2
+    x = BlocksAddLane<0x4E>(x);    // quad_perm 2 3 0 1
+    x = BlocksAddLane<0x141>(x);   // row_half_mirror
+    return BlocksAddLane<0x140>(x);   // row_mirror
+}
+
+// One query row per (sequence, head): a workgroup reads all its blocks' centroids once — bound by that read, so by what is in flight: 64 groups of 16 lanes,
+// four blocks each — and one wavefront selects.
+template <bool BF16, int DC>
+__global__ void __launch_bounds__(1024) BlocksRouteRowKernel(BlocksArgs a, const float* __restrict__ summary, uint32_t first, uint32_t last,
+                                                             int32_t* __restrict__ probes) {
+    constexpr uint32_t D = DC * 16, N = (D + 63) / 64;   // float4 a lane of a 16-lane group: dimensions 64 i + 4 l
+    extern __shared__ uint64_t s_key[];
+    const uint32_t t = blockIdx.x, pair = blockIdx.y, b = pair / a.Hkv, h = pair % a.Hkv, sub = threadIdx.x & 15, group = threadIdx.x >> 4;
+    const int n = BlocksKvLen(a, b), m = BlocksQLen(a, b);
+    if ((int)t >= m) return;
+    const uint32_t nb = (uint32_t)(BlocksVisible(a, n, m, (int)t) + (int)a.bs - 1) / a.bs;
+    int32_t* out = probes + (((int64_t)b * a.Tq + t) * a.Hkv + h) * a.P;
+    if (nb <= a.P) {
+        if (threadIdx.x < a.P) out[threadIdx.x] = threadIdx.x < nb ? (int32_t)threadIdx.x : -1;
+        return;
+    }
+    const float* cen = summary + (uint64_t)pair * a.nblk * D;
+    const uint16_t* p = a.q + b * a.qs[0] + (int64_t)t * a.qs[1] + (int64_t)h * a.G * a.qs[2];
+    double q[N][4];
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) q[i][0] = q[i][1] = q[i][2] = q[i][3] = 0;
+    for (uint32_t j0 = 0; j0 < nb; j0 += 256) {
+        float4 c[4][N];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i)
+                c[u][i] = *reinterpret_cast<const float4*>(cen + (uint64_t)min(j0 + u * 64 + group, nb - 1) * D + min(i * 64 + sub * 4, D - 4));
+        if (j0 == 0)
+            for (uint32_t x = 0; x < a.G; ++x)
+#pragma unroll
+                for (uint32_t i = 0; i < N; ++i) {
+                    if (i * 64 + sub * 4 >= D) continue;
+                    const uint2 y = *reinterpret_cast<const uint2*>(p + x * a.qs[2] + i * 64 + sub * 4);
+                    q[i][0] += BlocksToDouble((uint16_t)y.x, BF16);
+                    q[i][1] += BlocksToDouble((uint16_t)(y.x >> 16), BF16);
+                    q[i][2] += BlocksToDouble((uint16_t)y.y, BF16);
+                    q[i][3] += BlocksToDouble((uint16_t)(y.y >> 16), BF16);
+                }
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+            double x = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i)
+                if (i * 64 + sub * 4 < D) {
+                    x = fma(q[i][0], (double)c[u][i].x, x);
+                    x = fma(q[i][1], (double)c[u][i].y, x);
+                    x = fma(q[i][2], (double)c[u][i].z, x);
+                    x = fma(q[i][3], (double)c[u][i].w, x);
+                }
+            x = BlocksSumOver16(x);
+            const uint32_t j = j0 + u * 64 + group;
+            if (sub == 0 && j < nb) s_key[j] = BlocksScoreKey(x);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    if (nb <= 128)
+        BlocksSelect<2>(s_key, nb, a.P, first, last, threadIdx.x, out);
+    else if (nb <= 512)
+        BlocksSelect<8>(s_key, nb, a.P, first, last, threadIdx.x, out);
+    else
+        BlocksSelect<0>(s_key, nb, a.P, first, last, threadIdx.x, out);
+}
+
+template <bool BF16, int DC>
+static gpann_status Route(const BlocksArgs& a, const float* summary, uint32_t first, uint32_t last, int32_t* probes, hipStream_t st) {
+    // keys of a workgroup's query rows in 128 KB; groups are given up while there are not two workgroups per CU
+    const uint64_t pairs = (uint64_t)a.B * a.Hkv, room = 128 * 1024 / 8;
+    if (a.Tq < 16 || a.nblk > room / 4) {   // the matrix tiles would hold fewer than four query rows
+        const size_t lds = (size_t)a.nblk * 8;
+        auto kernel = BlocksRouteRowKernel<BF16, DC>;
+        GPANN_REQUIRE(pairs <= 65535, "more than 65535 (sequence, head) pairs");
+        if (lds > 32 * 1024) GPANN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        hipLaunchKernelGGL(kernel, dim3(a.Tq, (uint32_t)pairs), dim3(1024), lds, st, a, summary, first, last, probes);
+        GPANN_HIP_TRY(hipGetLastError());
+        return GPANN_OK;
+    }
+    const uint32_t tokens = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(16, a.Tq), std::max<uint64_t>(1, room / std::max(1u, a.nblk)));
+    uint32_t groups = 8;
+    while (groups > 1 && ((uint64_t)groups * tokens * a.nblk > room || pairs * ((a.Tq + groups * tokens - 1) / (groups * tokens)) < 512)) groups /= 2;
+    const uint64_t tiles = ((uint64_t)a.Tq + groups * tokens - 1) / (groups * tokens);
+    const size_t lds = std::max<size_t>(8, (size_t)groups * tokens * a.nblk * 8);
+    return BlocksLaunch(BlocksRouteKernel<BF16, DC>, BlocksPairGrid(pairs, tiles), lds, st, a, groups, tokens, (uint32_t)tiles, summary, first, last, probes);
 }
 
 // ---- eviction -------------------------------------------------------------------------------------------------------------------------------
@@ -354,15 +530,7 @@ gpann_status gpann_blocks_route(const gpann_blocks_layout* L, const void* q, con
     GPANN_BLOCKS_ENTER(L, stream);
     const BlocksArgs a = BlocksMakeArgs(L, q, nullptr, nullptr, nullptr, nprobe);
     if (a.B == 0 || a.Tq == 0) return GPANN_OK;
-    const uint32_t d = L->head_dim;
-    const dim3 grid(a.Tq, a.Hkv, a.B);
-    const size_t lds = (size_t)(d + a.nblk) * sizeof(double);
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    auto kernel = L->dtype == GPANN_BLOCKS_BF16 ? BlocksRouteKernel<true> : BlocksRouteKernel<false>;
-    if (lds > 32 * 1024) GPANN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a, d, summary, first, last, probes);
-    GPANN_HIP_TRY(hipGetLastError());
-    return GPANN_OK;
+    GPANN_BLOCKS_DISPATCH(L, Route, a, summary, first, last, probes, static_cast<hipStream_t>(stream));
 }
 
 gpann_status gpann_blocks_evict(const gpann_blocks_layout* L, const void* k, const void* v, const float* mass, uint32_t keep, uint32_t first, uint32_t last,
