@@ -57,11 +57,13 @@ struct BlocksDevice {
     GPANN_TRY(::gpann::BlocksCheckStream(L, stream))
 
 // ---- device helpers -----------------------------------------------------------------------------------------------------------------------
+// (constant address space: nothing writes the lengths while a kernel runs, and a scalar load does not queue behind the vector loads in flight)
+__device__ __forceinline__ int BlocksLength(const int32_t* p, uint32_t b) { return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)p)[b]; }
 __device__ __forceinline__ int BlocksKvLen(const BlocksArgs& a, uint32_t b) {
-    return a.kv_len ? min(max(a.kv_len[b], 0), (int)a.Tk) : (int)a.Tk;
+    return a.kv_len ? min(max(BlocksLength(a.kv_len, b), 0), (int)a.Tk) : (int)a.Tk;
 }
 __device__ __forceinline__ int BlocksQLen(const BlocksArgs& a, uint32_t b) {
-    return a.q_len ? min(max(a.q_len[b], 0), (int)a.Tq) : (int)a.Tq;
+    return a.q_len ? min(max(BlocksLength(a.q_len, b), 0), (int)a.Tq) : (int)a.Tq;
 }
 // how many cache rows (a prefix) query row t sees; n, m: lengths of the sequence
 __device__ __forceinline__ int BlocksVisible(const BlocksArgs& a, int n, int m, int t) {

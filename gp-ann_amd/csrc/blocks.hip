@@ -1,5 +1,5 @@
 // blocks.hip — block operators: layout checks, centroids of the blocks, routing of query rows to blocks, eviction (include/gpann_blocks.h).
-#include "blocks.h"
+#include "blocks_tile.h"
 
 #include <algorithm>
 #include <cmath>
@@ -272,8 +272,13 @@ __global__ void __launch_bounds__(512) BlocksRouteKernel(BlocksArgs a, uint32_t 
             for (int i = 0; i < K / 4; ++i) c[i] = next[i];
         }
     }
-    __syncthreads();
-    for (uint32_t i = wave; i < groups * tokens; i += 8) {
+    // a wavefront that has all the blocks of its query rows to itself goes on with them; else the workgroup's query rows are divided
+    const bool own = parts == 1;
+    if (own)
+        BlocksWaveSync();
+    else
+        __syncthreads();
+    for (uint32_t i = own ? group * tokens : wave, end = own ? i + tokens : groups * tokens; i < end; i += own ? 1 : 8) {
         const uint32_t t = row0 + i;
         if ((int)t >= m) break;
         const uint32_t nb = (uint32_t)(BlocksVisible(a, n, m, (int)t) + (int)a.bs - 1) / a.bs;
@@ -398,10 +403,13 @@ __device__ __forceinline__ uint32_t BlocksMassKey(float x) {
     return OrderedKey(x + 0.f);
 }
 
-// One workgroup per (head, sequence): bisection for the smallest key that stays, then one pass in row order.
+constexpr uint32_t kEvictKeys = 32;   // keys a thread holds in registers: sequences up to 32768 rows are read once
+// One workgroup per (head, sequence).  The smallest key that stays is found eleven, eleven and ten bits at a time: a histogram of the keys that agree with the
+// bits found so far, summed from its top.  Then one pass in row order: keys above it stay, and of those equal to it the lowest rows.
+template <bool HELD>
 __global__ void __launch_bounds__(1024) BlocksEvictSelectKernel(BlocksArgs a, const float* __restrict__ mass, uint32_t keep, uint32_t first, uint32_t last,
                                                                 int32_t* __restrict__ rows, int32_t* __restrict__ count) {
-    __shared__ uint32_t s_count[16], s_eq[16];
+    __shared__ uint32_t s_bins[2048], s_gt[16], s_eq[16], s_found[2];
     const uint32_t h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const uint32_t n = (uint32_t)BlocksKvLen(a, b);
     const uint32_t take = min(n, keep);
@@ -413,55 +421,88 @@ __global__ void __launch_bounds__(1024) BlocksEvictSelectKernel(BlocksArgs a, co
         for (uint32_t j = tid; j < n; j += 1024) out[j] = (int32_t)j;
         return;
     }
-    auto key = [&](uint32_t j) -> uint64_t { return (j < first || j + last >= n) ? 1ull << 32 : (uint64_t)BlocksMassKey(ms[j]); };
-    auto total = [&](uint32_t c) {
-        for (int s = 32; s > 0; s >>= 1) c += __shfl_xor(c, s);
-        __syncthreads();
-        if (lane == 0) s_count[wave] = c;
-        __syncthreads();
-        c = 0;
-        for (int w = 0; w < 16; ++w) c += s_count[w];
-        return c;
+    // rows first .. n - last compete for what the others leave
+    const uint32_t lo_row = first, hi_row = n - last, want = take - first - last;
+    uint32_t held[HELD ? kEvictKeys : 1];
+    if (HELD)
+#pragma unroll
+        for (uint32_t i = 0; i < kEvictKeys; ++i) {
+            const uint32_t j = i * 1024 + tid;
+            held[i] = j < n ? __float_as_uint(ms[j]) : 0u;
+        }
+    if (HELD)
+#pragma unroll
+        for (uint32_t i = 0; i < kEvictKeys; ++i) held[i] = BlocksMassKey(__uint_as_float(held[i]));
+    auto each = [&](auto&& f) {   // f(row, key), a thread's rows in order
+        if (HELD) {
+#pragma unroll
+            for (uint32_t i = 0; i < kEvictKeys; ++i)
+                if (i * 1024 < n) f(i * 1024 + tid, held[i]);
+        } else {
+            for (uint32_t j0 = 0; j0 < n; j0 += 1024) f(j0 + tid, j0 + tid < n ? BlocksMassKey(ms[j0 + tid]) : 0u);
+        }
     };
-    uint64_t v = 0;
-    for (int bit = 32; bit >= 0; --bit) {
-        const uint64_t trial = v | (1ull << bit);
-        uint32_t c = 0;
-        for (uint32_t j = tid; j < n; j += 1024) c += key(j) >= trial;
-        c = total(c);
-        if (c >= take) v = trial;
-        if (c == take) break;
-    }
-    uint32_t above = 0;
-    for (uint32_t j = tid; j < n; j += 1024) above += key(j) > v;
-    above = total(above);
-    uint32_t equal = take - above, at = 0;
+    uint32_t v = 0, left = want;   // key bits found; how many of the keys that agree with them stay
+    if (want > 0)
+        for (int digit = 0; digit < 3; ++digit) {
+            const uint32_t shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bins = digit == 2 ? 1024 : 2048;
+            const uint32_t above = digit == 0 ? 0 : digit == 1 ? 0xFFE00000u : 0xFFFFFC00u;
+            for (uint32_t i = tid; i < bins; i += 1024) s_bins[i] = 0;
+            __syncthreads();
+            each([&](uint32_t j, uint32_t k) {
+                if (j >= lo_row && j < hi_row && (k & above) == v) atomicAdd(&s_bins[(k >> shift) & (bins - 1)], 1u);
+            });
+            __syncthreads();
+            // thread t: bins top - 2 t and top - 2 t - 1 (or one each); sums from the top
+            const uint32_t per = bins / 1024, bin = bins - 1 - tid * per;
+            const uint32_t c0 = s_bins[bin], c1 = per == 2 ? s_bins[bin - 1] : 0;
+            uint32_t sum = c0 + c1;
+            for (int s = 1; s < 64; s <<= 1) {
+                const uint32_t x = __shfl_up(sum, s);
+                if ((int)lane >= s) sum += x;
+            }
+            if (lane == 63) s_gt[wave] = sum;
+            __syncthreads();
+            uint32_t before = sum - c0 - c1;
+            for (uint32_t w = 0; w < wave; ++w) before += s_gt[w];
+            if (before < left && before + c0 + c1 >= left) {
+                const bool upper = before + c0 >= left;
+                s_found[0] = upper ? bin : bin - 1;
+                s_found[1] = upper ? before : before + c0;
+            }
+            __syncthreads();
+            v |= s_found[0] << shift;
+            left -= s_found[1];
+            __syncthreads();
+        }
+    // `left` of the rows whose key is v stay
+    uint32_t at = 0, equal = left;
     const uint64_t below = (1ull << lane) - 1;
-    for (uint32_t j0 = 0; j0 < n && at < take; j0 += 1024) {
-        const uint32_t j = j0 + tid;
-        const uint64_t kk = j < n ? key(j) : 0;
-        const bool gt = j < n && kk > v, eq = j < n && kk == v;
+    each([&](uint32_t j, uint32_t k) {
+        const bool forced = j < lo_row || (j >= hi_row && j < n), free = j >= lo_row && j < hi_row && want > 0;
+        const bool gt = forced || (free && k > v), eq = free && k == v;
         const uint64_t gts = __ballot(gt), eqs = __ballot(eq);
-        __syncthreads();
         if (lane == 0) {
-            s_count[wave] = (uint32_t)__popcll(gts);
+            s_gt[wave] = (uint32_t)__popcll(gts);
             s_eq[wave] = (uint32_t)__popcll(eqs);
         }
         __syncthreads();
         uint32_t gt_before = 0, eq_before = 0, gt_all = 0, eq_all = 0;
         for (uint32_t w = 0; w < 16; ++w) {
+            const uint32_t x = s_gt[w], y = s_eq[w];
             if (w < wave) {
-                gt_before += s_count[w];
-                eq_before += s_eq[w];
+                gt_before += x;
+                eq_before += y;
             }
-            gt_all += s_count[w];
-            eq_all += s_eq[w];
+            gt_all += x;
+            eq_all += y;
         }
         const uint32_t g = gt_before + (uint32_t)__popcll(gts & below), e = eq_before + (uint32_t)__popcll(eqs & below);
         if (gt || (eq && e < equal)) out[at + g + min(e, equal)] = (int32_t)j;
         at += gt_all + min(equal, eq_all);
         equal -= min(equal, eq_all);
-    }
+        __syncthreads();
+    });
 }
 
 // 16 bytes of a kept row per thread
@@ -557,7 +598,10 @@ gpann_status gpann_blocks_evict(const gpann_blocks_layout* L, const void* k, con
     const BlocksArgs a = BlocksMakeArgs(L, nullptr, k, v, nullptr, 0);
     if (a.B == 0) return GPANN_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(BlocksEvictSelectKernel, dim3(a.Hkv, a.B), dim3(1024), 0, st, a, mass, keep, first, last, rows, count);
+    if (a.Tk <= kEvictKeys * 1024)
+        hipLaunchKernelGGL(BlocksEvictSelectKernel<true>, dim3(a.Hkv, a.B), dim3(1024), 0, st, a, mass, keep, first, last, rows, count);
+    else
+        hipLaunchKernelGGL(BlocksEvictSelectKernel<false>, dim3(a.Hkv, a.B), dim3(1024), 0, st, a, mass, keep, first, last, rows, count);
     GPANN_HIP_TRY(hipGetLastError());
     if (!k_out && !mass_out) return GPANN_OK;
     const uint32_t chunks = L->head_dim / 8, kept = std::min(keep, L->kv_rows);

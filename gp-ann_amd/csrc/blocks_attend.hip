@@ -489,104 +489,145 @@ __global__ void __launch_bounds__(512) BlocksWeighTokenKernel(BlocksArgs a, uint
     int64_t ko, vo;
     const uint32_t count = BlocksGatherProbes(a, a.probes + (int64_t)pair * a.P, b, visible, s_scratch[wave], lane, block, ko, vo);
     const uint32_t tpb = a.bs / 16, units = count * tpb;
+    auto load = [&](uint32_t u, u32x4_t(&to)[KS], int& start) {   // (clamped behind the last unit: of no use there)
+        const uint32_t unit = min(u, units - 1), slot = unit / tpb, base = unit % tpb * 16;
+        const int blk = __builtin_amdgcn_readlane(block, (int)slot), last = visible - 1 - blk * (int)a.bs;
+        start = blk * (int)a.bs + (int)base;
+        BlocksLoadRows<KS>(a.k + BlocksReadLane64(ko, slot) + h * a.ks[2] + min((int)(base + r), last) * a.ks[1] + g * 8, to);
+    };
+    if (units == 0) return;
+    u32x4_t kr[KS], q[KS];
+    int start;
+    load(wave, kr, start);
+    const uint32_t heads0 = min(16u, a.G);
+    BlocksLoadRows<KS>(a.q + b * a.qs[0] + (h * a.G + min(r, heads0 - 1)) * a.qs[2] + g * 8, q);
+    const float l0 = lse[(int64_t)b * a.Hq + h * a.G + min(r, heads0 - 1)];
     for (uint32_t u = wave; u < units; u += 8) {
-        const uint32_t slot = u / tpb, base = u % tpb * 16;
-        const int blk = __builtin_amdgcn_readlane(block, (int)slot), last = visible - 1 - blk * (int)a.bs, start = blk * (int)a.bs + (int)base;
-        if (start >= visible) continue;
-        u32x4_t kr[KS];
-        BlocksLoadRows<KS>(a.k + BlocksReadLane64(ko, slot) + h * a.ks[2] + min((int)(base + r), last) * a.ks[1] + g * 8, kr);
+        u32x4_t next[KS];
+        int next_start;
+        load(u + 8, next, next_start);
         f32x4_t w = {0.f, 0.f, 0.f, 0.f};
         for (uint32_t mt = 0; mt < mtiles; ++mt) {
             const uint32_t heads = min(16u, a.G - mt * 16), head = h * a.G + mt * 16 + min(r, heads - 1);
-            const float l = lse[(int64_t)b * a.Hq + head], lse2 = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;
-            const uint16_t* q = a.q + b * a.qs[0] + head * a.qs[2] + g * 8;
+            if (mtiles > 1) BlocksLoadRows<KS>(a.q + b * a.qs[0] + head * a.qs[2] + g * 8, q);
+            const float l = mtiles > 1 ? lse[(int64_t)b * a.Hq + head] : l0, lse2 = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;
             f32x4_t s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < KS; ++j) s = BlocksMfma<BF16>(kr[j], *reinterpret_cast<const u32x4_t*>(q + j * 32), s);
+            for (int j = 0; j < KS; ++j) s = BlocksMfma<BF16>(kr[j], q[j], s);
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] += r < heads ? BlocksExp2(s[i] * a.scale2 - lse2) : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int x = 8; x > 0; x >>= 1) w[i] += __shfl_xor(w[i], x);
+            w[i] = BlocksSumRow16(w[i]);
             const int key = start + (int)g * 4 + i;
             if ((int)r == i && key < visible) mass[(int64_t)pair * a.Tk + key] += w[i];
         }
+        start = next_start;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) kr[j] = next[j];
     }
 }
 
-// What a wavefront of the kernel below knows of the 16 (query row, head) rows of a step
-struct BlocksWeighRows {
-    int64_t q[16];
-    float lse2[16];
-    int visible[16];
-};
-
-// many query rows: one workgroup per block, the rows that probe it stream past its keys; wavefronts divide the block's 16-key tiles and the rows
+// Many query rows: a wavefront takes a 64-key piece of a block, lists the query rows that probe it and lets their heads stream past the keys, 16 rows a
+// product with a key per lane column; what a key gets is added in one lane group's registers.  Wavefronts share nothing and go from piece to piece (those of a
+// pair on one die): a piece is two or three dependent trips to memory, so what counts is that eight are always under way on a CU.
 template <bool BF16, int DC>
-__global__ void __launch_bounds__(512) BlocksWeighKernel(BlocksArgs a, uint32_t words, uint32_t tile_groups, uint32_t blocks_x, const uint32_t* __restrict__ bits,
-                                                         const float* __restrict__ lse, const float* mass_in, float* mass_out) {
+__global__ void __launch_bounds__(512) BlocksWeighKernel(BlocksArgs a, uint32_t words, uint32_t pieces, const uint32_t* __restrict__ bits, const float* __restrict__ lse,
+                                                         const float* mass_in, float* mass_out) {
     TakeWholeRegisterFile();
     constexpr int KS = DC / 2;
-    __shared__ uint32_t s_list[kRange], s_count;
-    __shared__ BlocksWeighRows s_rows[8];
-    __shared__ float s_sum[8][16];
+    struct About {
+        float lse2;
+        int visible;
+    };
+    __shared__ uint16_t s_list[8][kRange];
+    __shared__ About s_about[8][16];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    uint32_t pair, x;
-    if (!BlocksPairOf(blockIdx.x, a.B * a.Hkv, blocks_x, pair, x)) return;
-    const uint32_t tg = x % tile_groups, block = x / tile_groups, b = pair / a.Hkv, h = pair % a.Hkv;
-    const int n = BlocksKvLen(a, b), m = BlocksQLen(a, b);
-    const uint32_t tpb = a.bs / 16, kts = min(8u, tpb - tg * 8), rgs = 8 / kts, kt = wave % kts, rg = wave / kts;
-    const bool works = rg < rgs;
-    const uint32_t in_block = (tg * 8 + kt) * 16;
-    const int key = (int)(block * a.bs + in_block + r);
-    float w = 0.f;
-    u32x4_t kf[KS];
-    bool loaded = false;
-    for (uint32_t first = 0; first < words; first += kRange / 32) {
-        BlocksListRows(bits + ((uint64_t)pair * a.nblk + block) * words, first, words, s_list, &s_count);
-        __syncthreads();
-        const uint32_t rows = s_count * a.G;
-        if (works && rows > 0) {
-            if (!loaded) {
+    const uint32_t die = blockIdx.x & 7, pairs = a.B * a.Hkv, per_pair = a.nblk * pieces, waves = (gridDim.x >> 3) * 8;
+    const uint64_t tasks = (uint64_t)((pairs + 7 - die) / 8) * per_pair;   // of the pairs that are `die` modulo 8
+    const uint32_t inverse = a.G > 1 ? 0xFFFFFFFFu / a.G + 1 : 0;
+    auto first_words = [&](uint64_t task) -> uint32_t {
+        if (task >= tasks) return 0u;
+        const uint64_t block = (uint64_t)((uint32_t)(task / per_pair) * 8 + die) * a.nblk + (uint32_t)(task % per_pair) / pieces;
+        return lane < words ? bits[block * words + lane] : 0u;
+    };
+    uint64_t task = (blockIdx.x >> 3) * 8 + wave;
+    uint32_t ahead = first_words(task);
+    for (; task < tasks; task += waves) {
+        const uint32_t pair = (uint32_t)(task / per_pair) * 8 + die, x = (uint32_t)(task % per_pair), block = x / pieces, in_block = x % pieces * 64;
+        const uint32_t b = pair / a.Hkv, h = pair % a.Hkv, tiles = min(4u, (a.bs - in_block) / 16);
+        const int key0 = (int)(block * a.bs + in_block), mine = key0 + (int)lane;
+        const bool writes = lane < tiles * 16 && mine < (int)a.Tk;
+        const float before = writes ? mass_in[(uint64_t)pair * a.Tk + mine] : 0.f;
+        uint32_t word = ahead;
+        ahead = first_words(task + waves);
+        const int n = BlocksKvLen(a, b), m = BlocksQLen(a, b);
+        float w[4] = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t first = 0;;) {
+            const uint32_t c = (uint32_t)__popc(word);
+            uint32_t at = c;
+            for (int s = 1; s < 64; s <<= 1) {
+                const uint32_t y = __shfl_up(at, s);
+                if ((int)lane >= s) at += y;
+            }
+            const uint32_t rows = (uint32_t)__builtin_amdgcn_readlane((int)at, 63) * a.G;
+            at -= c;
+            while (word) {
+                s_list[wave][at++] = (uint16_t)(lane * 32 + (uint32_t)__ffs(word) - 1);
+                word &= word - 1;
+            }
+            BlocksWaveSync();
+            if (rows > 0) {
+                u32x4_t kf[4][KS], q[KS];
                 int64_t ko, vo;
                 (void)BlocksBase(a, b, (int)block, ko, vo);
-                const int last = n - 1 - (int)(block * a.bs);
-                BlocksLoadRows<KS>(a.k + ko + h * a.ks[2] + min((int)(in_block + r), last) * a.ks[1] + g * 8, kf);
-                loaded = true;
-            }
-            BlocksWeighRows& info = s_rows[wave];
-            for (uint32_t row0 = rg * 16; row0 < rows; row0 += rgs * 16) {
-                if (lane < 16) {
-                    const uint32_t row = row0 + lane, rr = min(row, rows - 1), t = s_list[rr / a.G], head = h * a.G + rr % a.G;
-                    const float l = lse[((int64_t)b * a.Tq + t) * a.Hq + head];
-                    info.q[lane] = b * a.qs[0] + t * a.qs[1] + head * a.qs[2];
-                    info.lse2[lane] = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;
-                    info.visible[lane] = row < rows ? BlocksVisible(a, n, m, (int)t) : 0;
-                }
-                BlocksWaveSync();
-                const uint16_t* q = a.q + info.q[r] + g * 8;
-                f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+                const int last = n - 1 - (int)(block * a.bs);   // >= 0: a listed block holds a visible row
+                const uint16_t* k = a.k + ko + h * a.ks[2] + g * 8;
 #pragma unroll
-                for (int j = 0; j < KS; ++j) s = BlocksMfma<BF16>(*reinterpret_cast<const u32x4_t*>(q + j * 32), kf[j], s);
+                for (uint32_t y = 0; y < 4; ++y) BlocksLoadRows<KS>(k + min((int)(in_block + min(y, tiles - 1) * 16 + r), last) * a.ks[1], kf[y]);
+                float l;
+                int t;
+                auto load = [&](uint32_t row0, u32x4_t(&to)[KS]) {   // (clamped behind the last row: of no use there)
+                    const uint32_t i = min(row0 + r, rows - 1), in = inverse ? __umulhi(i, inverse) : i, head = h * a.G + i - in * a.G;
+                    t = (int)(first * 32 + s_list[wave][in]);
+                    BlocksLoadRows<KS>(a.q + b * a.qs[0] + t * a.qs[1] + head * a.qs[2] + g * 8, to);
+                    l = lse[((int64_t)b * a.Tq + t) * a.Hq + head];
+                };
+                load(0, q);
+                for (uint32_t row0 = 0; row0 < rows; row0 += 16) {
+                    if (g == 0) s_about[wave][r] = About{l == -__builtin_inff() ? __builtin_inff() : l * kLog2e, row0 + r < rows ? BlocksVisible(a, n, m, t) : 0};
+                    u32x4_t next[KS];
+                    load(row0 + 16, next);
+                    BlocksWaveSync();
+                    About about[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t row = g * 4 + i;
-                    w += key < info.visible[row] ? BlocksExp2(s[i] * a.scale2 - info.lse2[row]) : 0.f;
+                    for (int j = 0; j < 4; ++j) about[j] = s_about[wave][g * 4 + j];
+                    BlocksWaveSync();
+                    f32x4_t s[4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) s[y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int j = 0; j < KS; ++j)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) s[y] = BlocksMfma<BF16>(q[j], kf[y][j], s[y]);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            w[y] += key0 + y * 16 + (int)r < about[j].visible ? BlocksExp2(s[y][j] * a.scale2 - about[j].lse2) : 0.f;
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) q[j] = next[j];
                 }
-                BlocksWaveSync();
             }
+            first += kRange / 32;
+            if (first >= words) break;
+            word = first + lane < words ? bits[((uint64_t)pair * a.nblk + block) * words + first + lane] : 0u;
         }
-        __syncthreads();
-    }
-    w = BlocksSumOver4(w);
-    if (g == 0) s_sum[wave][r] = w;
-    __syncthreads();
-    if (works && rg == 0 && g == 0 && key < (int)a.Tk) {
-        float total = mass_in[(int64_t)pair * a.Tk + key];
-        for (uint32_t y = 0; y < rgs; ++y) total += s_sum[y * kts + kt][r];
-        mass_out[(int64_t)pair * a.Tk + key] = total;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) w[y] = BlocksSumOver4(w[y]);
+        const float more = g == 0 ? w[0] : g == 1 ? w[1] : g == 2 ? w[2] : w[3];   // lane = key of the piece
+        if (writes) mass_out[(uint64_t)pair * a.Tk + mine] = before + more;
     }
 }
 
@@ -631,11 +672,12 @@ static gpann_status Weigh(const BlocksArgs& a, const float* lse, const float* ma
         if (a.Tq == 0) return GPANN_OK;
         return BlocksLaunch(BlocksWeighTokenKernel<BF16, DC>, pairs, 0, st, a, (a.G + 15) / 16, lse, mass_out);
     }
-    const uint32_t words = (a.Tq + 31) / 32, tile_groups = (a.bs / 16 + 7) / 8;
+    const uint32_t words = (a.Tq + 31) / 32, pieces = (a.bs + 63) / 64;
     uint32_t* bits = reinterpret_cast<uint32_t*>(ws);
     GPANN_TRY(BlocksMarkProbes(a, words, bits, st));
-    const uint64_t blocks_x = (uint64_t)a.nblk * tile_groups;
-    return BlocksLaunch(BlocksWeighKernel<BF16, DC>, BlocksPairGrid(pairs, blocks_x), 0, st, a, words, tile_groups, (uint32_t)blocks_x, bits, lse, mass_in, mass_out);
+    const uint64_t tasks = pairs * a.nblk * pieces;   // one workgroup per CU, fewer where there is less to do; a multiple of the eight dies
+    const uint64_t grid = std::min<uint64_t>(256, (tasks + 63) / 64 * 8);
+    return BlocksLaunch(BlocksWeighKernel<BF16, DC>, grid, 0, st, a, words, pieces, bits, lse, mass_in, mass_out);
 }
 
 }  // namespace gpann

@@ -98,6 +98,12 @@ __device__ __forceinline__ float BlocksSumOver4(float x) {
     const auto z = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     return __uint_as_float(z[0]) + __uint_as_float(z[1]);
 }
+// over 16 neighbouring lanes: ^ 1, ^ 2, mirror of 8, mirror of 16 lanes
+template <int CTRL>
+__device__ __forceinline__ float BlocksAddLane(float x) {
+    return x + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float BlocksSumRow16(float x) { return BlocksAddLane<0x140>(BlocksAddLane<0x141>(BlocksAddLane<0x4E>(BlocksAddLane<0xB1>(x)))); }
 // The running maximum follows the true one only when that is more than this many powers of two ahead: weights then reach 2^8 instead of 1, which 16-bit
 // floats hold as exactly, and the accumulators are hardly ever rescaled.
 constexpr float kBlocksSlack = 8.f;

@@ -246,26 +246,6 @@ struct BlocksWalkAddresses {
 };
 
 // ---- which query rows probe a block: bits [sequence, head][block][query row] -----------------------------------------------------------------------
-constexpr uint32_t kRange = 2048;   // query rows whose list a workgroup holds at a time
-
-// the set bits of words [first, first + kRange / 32) as a list of query rows, ascending; by the first wavefront
-__device__ __forceinline__ void BlocksListRows(const uint32_t* bits, uint32_t first, uint32_t words, uint32_t* s_list, uint32_t* s_count) {
-    if (threadIdx.x < 64) {
-        const uint32_t lane = threadIdx.x;
-        uint32_t w = first + lane < words ? bits[first + lane] : 0u;
-        const uint32_t c = (uint32_t)__popc(w);
-        uint32_t before = c;
-        for (int s = 1; s < 64; s <<= 1) {
-            const uint32_t x = __shfl_up(before, s);
-            if ((int)lane >= s) before += x;
-        }
-        if (lane == 63) *s_count = before;
-        before -= c;
-        while (w) {
-            s_list[before++] = (first + lane) * 32 + (uint32_t)__ffs(w) - 1;
-            w &= w - 1;
-        }
-    }
-}
+constexpr uint32_t kRange = 2048;   // query rows a wavefront lists at a time: 64 words
 
 }  // namespace gpann
