@@ -423,23 +423,28 @@ __global__ void __launch_bounds__(1024) BlocksEvictSelectKernel(BlocksArgs a, co
     }
     // rows first .. n - last compete for what the others leave
     const uint32_t lo_row = first, hi_row = n - last, want = take - first - last;
+    // a wavefront has the rows chunk * wave .., 64 at a time: what it keeps lies together in the output
+    const uint32_t chunk = (n + 1023) / 1024 * 64, row0 = wave * chunk;
     uint32_t held[HELD ? kEvictKeys : 1];
     if (HELD)
 #pragma unroll
         for (uint32_t i = 0; i < kEvictKeys; ++i) {
-            const uint32_t j = i * 1024 + tid;
-            held[i] = j < n ? __float_as_uint(ms[j]) : 0u;
+            const uint32_t j = row0 + i * 64 + lane;
+            held[i] = i * 64 < chunk && j < n ? __float_as_uint(ms[j]) : 0u;
         }
     if (HELD)
 #pragma unroll
         for (uint32_t i = 0; i < kEvictKeys; ++i) held[i] = BlocksMassKey(__uint_as_float(held[i]));
-    auto each = [&](auto&& f) {   // f(row, key), a thread's rows in order
+    auto each = [&](auto&& f) {   // f(row, key) of the wavefront's rows, in their order
         if (HELD) {
 #pragma unroll
             for (uint32_t i = 0; i < kEvictKeys; ++i)
-                if (i * 1024 < n) f(i * 1024 + tid, held[i]);
+                if (i * 64 < chunk) f(row0 + i * 64 + lane, held[i]);
         } else {
-            for (uint32_t j0 = 0; j0 < n; j0 += 1024) f(j0 + tid, j0 + tid < n ? BlocksMassKey(ms[j0 + tid]) : 0u);
+            for (uint32_t i = 0; i < chunk; i += 64) {
+                const uint32_t j = row0 + i + lane;
+                f(j, j < n ? BlocksMassKey(ms[j]) : 0u);
+            }
         }
     };
     uint32_t v = 0, left = want;   // key bits found; how many of the keys that agree with them stay
@@ -475,33 +480,38 @@ __global__ void __launch_bounds__(1024) BlocksEvictSelectKernel(BlocksArgs a, co
             left -= s_found[1];
             __syncthreads();
         }
-    // `left` of the rows whose key is v stay
-    uint32_t at = 0, equal = left;
+    // `left` of the rows whose key is v stay: how many of either kind the wavefronts before this one have, then where each row goes
     const uint64_t below = (1ull << lane) - 1;
+    auto kind = [&](uint32_t j, uint32_t k, bool& gt, bool& eq) {
+        const bool free = j >= lo_row && j < hi_row && want > 0;
+        gt = (j < n && !(j >= lo_row && j < hi_row)) || (free && k > v);
+        eq = free && k == v;
+    };
+    uint32_t gts = 0, eqs = 0;
     each([&](uint32_t j, uint32_t k) {
-        const bool forced = j < lo_row || (j >= hi_row && j < n), free = j >= lo_row && j < hi_row && want > 0;
-        const bool gt = forced || (free && k > v), eq = free && k == v;
-        const uint64_t gts = __ballot(gt), eqs = __ballot(eq);
-        if (lane == 0) {
-            s_gt[wave] = (uint32_t)__popcll(gts);
-            s_eq[wave] = (uint32_t)__popcll(eqs);
-        }
-        __syncthreads();
-        uint32_t gt_before = 0, eq_before = 0, gt_all = 0, eq_all = 0;
-        for (uint32_t w = 0; w < 16; ++w) {
-            const uint32_t x = s_gt[w], y = s_eq[w];
-            if (w < wave) {
-                gt_before += x;
-                eq_before += y;
-            }
-            gt_all += x;
-            eq_all += y;
-        }
-        const uint32_t g = gt_before + (uint32_t)__popcll(gts & below), e = eq_before + (uint32_t)__popcll(eqs & below);
-        if (gt || (eq && e < equal)) out[at + g + min(e, equal)] = (int32_t)j;
-        at += gt_all + min(equal, eq_all);
-        equal -= min(equal, eq_all);
-        __syncthreads();
+        bool gt, eq;
+        kind(j, k, gt, eq);
+        gts += (uint32_t)__popcll(__ballot(gt));
+        eqs += (uint32_t)__popcll(__ballot(eq));
+    });
+    if (lane == 0) {
+        s_gt[wave] = gts;
+        s_eq[wave] = eqs;
+    }
+    __syncthreads();
+    uint32_t gt_at = 0, eq_at = 0;
+    for (uint32_t w = 0; w < wave; ++w) {
+        gt_at += s_gt[w];
+        eq_at += s_eq[w];
+    }
+    each([&](uint32_t j, uint32_t k) {
+        bool gt, eq;
+        kind(j, k, gt, eq);
+        const uint64_t g = __ballot(gt), e = __ballot(eq);
+        const uint32_t before = gt_at + (uint32_t)__popcll(g & below), same = eq_at + (uint32_t)__popcll(e & below);
+        if (gt || (eq && same < left)) out[before + min(same, left)] = (int32_t)j;
+        gt_at += (uint32_t)__popcll(g);
+        eq_at += (uint32_t)__popcll(e);
     });
 }
 

@@ -471,41 +471,50 @@ __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint
 }
 
 // ---- attention weights of the cache rows ------------------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) BlocksCopyKernel(const float* __restrict__ from, float* __restrict__ to, uint64_t n) {
-    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) to[i] = from[i];
-}
-
-// one query row per sequence: a cache row gets the weights of one group's heads, from one wavefront
+// One query row per sequence: a cache row gets the weights of one group's heads, from one wavefront of the workgroup that copies the pair's masses.
 template <bool BF16, int DC>
-__global__ void __launch_bounds__(512) BlocksWeighTokenKernel(BlocksArgs a, uint32_t mtiles, const float* __restrict__ lse, float* __restrict__ mass) {
+__global__ void __launch_bounds__(512) BlocksWeighTokenKernel(BlocksArgs a, uint32_t mtiles, uint32_t vector, const float* __restrict__ lse, const float* mass_in,
+                                                              float* mass_out) {
     TakeWholeRegisterFile();
     constexpr int KS = DC / 2;
     __shared__ uint32_t s_scratch[8][64];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const uint32_t pair = blockIdx.x, b = pair / a.Hkv, h = pair % a.Hkv;
-    const int n = BlocksKvLen(a, b), visible = BlocksVisible(a, n, BlocksQLen(a, b), 0);
+    const int n = BlocksKvLen(a, b), visible = a.Tq ? BlocksVisible(a, n, BlocksQLen(a, b), 0) : 0;
+    const float* from = mass_in + (uint64_t)pair * a.Tk;
+    float* to = mass_out + (uint64_t)pair * a.Tk;
+    if (mass_in != mass_out) {
+        if (vector)
+            for (uint32_t i = threadIdx.x * 4; i < a.Tk; i += 2048) *reinterpret_cast<float4*>(to + i) = *reinterpret_cast<const float4*>(from + i);
+        else
+            for (uint32_t i = threadIdx.x; i < a.Tk; i += 512) to[i] = from[i];
+        __syncthreads();
+    }
     if (visible == 0) return;
     int block;
     int64_t ko, vo;
     const uint32_t count = BlocksGatherProbes(a, a.probes + (int64_t)pair * a.P, b, visible, s_scratch[wave], lane, block, ko, vo);
     const uint32_t tpb = a.bs / 16, units = count * tpb;
-    auto load = [&](uint32_t u, u32x4_t(&to)[KS], int& start) {   // (clamped behind the last unit: of no use there)
+    auto load = [&](uint32_t u, u32x4_t(&rows)[KS], int& start, float& before) {   // (clamped behind the last unit: of no use there)
         const uint32_t unit = min(u, units - 1), slot = unit / tpb, base = unit % tpb * 16;
         const int blk = __builtin_amdgcn_readlane(block, (int)slot), last = visible - 1 - blk * (int)a.bs;
         start = blk * (int)a.bs + (int)base;
-        BlocksLoadRows<KS>(a.k + BlocksReadLane64(ko, slot) + h * a.ks[2] + min((int)(base + r), last) * a.ks[1] + g * 8, to);
+        BlocksLoadRows<KS>(a.k + BlocksReadLane64(ko, slot) + h * a.ks[2] + min((int)(base + r), last) * a.ks[1] + g * 8, rows);
+        before = from[min(start + (int)(g * 4 + (r & 3)), visible - 1)];
     };
     if (units == 0) return;
     u32x4_t kr[KS], q[KS];
     int start;
-    load(wave, kr, start);
+    float before;
+    load(wave, kr, start, before);
     const uint32_t heads0 = min(16u, a.G);
     BlocksLoadRows<KS>(a.q + b * a.qs[0] + (h * a.G + min(r, heads0 - 1)) * a.qs[2] + g * 8, q);
     const float l0 = lse[(int64_t)b * a.Hq + h * a.G + min(r, heads0 - 1)];
     for (uint32_t u = wave; u < units; u += 8) {
         u32x4_t next[KS];
         int next_start;
-        load(u + 8, next, next_start);
+        float next_before;
+        load(u + 8, next, next_start, next_before);
         f32x4_t w = {0.f, 0.f, 0.f, 0.f};
         for (uint32_t mt = 0; mt < mtiles; ++mt) {
             const uint32_t heads = min(16u, a.G - mt * 16), head = h * a.G + mt * 16 + min(r, heads - 1);
@@ -521,9 +530,10 @@ __global__ void __launch_bounds__(512) BlocksWeighTokenKernel(BlocksArgs a, uint
         for (int i = 0; i < 4; ++i) {
             w[i] = BlocksSumRow16(w[i]);
             const int key = start + (int)g * 4 + i;
-            if ((int)r == i && key < visible) mass[(int64_t)pair * a.Tk + key] += w[i];
+            if ((int)r == i && key < visible) to[key] = before + w[i];
         }
         start = next_start;
+        before = next_before;
 #pragma unroll
         for (int j = 0; j < KS; ++j) kr[j] = next[j];
     }
@@ -664,13 +674,8 @@ template <bool BF16, int DC>
 static gpann_status Weigh(const BlocksArgs& a, const float* lse, const float* mass_in, float* mass_out, char* ws, hipStream_t st) {
     const uint64_t pairs = (uint64_t)a.B * a.Hkv;
     if (a.Tq <= 1) {
-        if (mass_in != mass_out) {
-            const uint64_t n = pairs * a.Tk;
-            hipLaunchKernelGGL(BlocksCopyKernel, dim3((uint32_t)std::min<uint64_t>((n + 255) / 256, 16384)), dim3(256), 0, st, mass_in, mass_out, n);
-            GPANN_HIP_TRY(hipGetLastError());
-        }
-        if (a.Tq == 0) return GPANN_OK;
-        return BlocksLaunch(BlocksWeighTokenKernel<BF16, DC>, pairs, 0, st, a, (a.G + 15) / 16, lse, mass_out);
+        const uint32_t vector = a.Tk % 4 == 0 && BlocksAligned(16, mass_in) && BlocksAligned(16, mass_out) ? 1 : 0;
+        return BlocksLaunch(BlocksWeighTokenKernel<BF16, DC>, pairs, 0, st, a, (a.G + 15) / 16, vector, lse, mass_in, mass_out);
     }
     const uint32_t words = (a.Tq + 31) / 32, pieces = (a.bs + 63) / 64;
     uint32_t* bits = reinterpret_cast<uint32_t*>(ws);
