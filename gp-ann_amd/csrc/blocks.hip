@@ -403,7 +403,7 @@ __device__ __forceinline__ uint32_t BlocksMassKey(float x) {
     return OrderedKey(x + 0.f);
 }
 
-constexpr uint32_t kEvictKeys = 32;   // keys a thread holds in registers: sequences up to 32768 rows are read once
+constexpr uint32_t kEvictKeys = 32768;   // keys that fit LDS: sequences up to that length are read once
 // One workgroup per (head, sequence).  The smallest key that stays is found eleven, eleven and ten bits at a time: a histogram of the keys that agree with the
 // bits found so far, summed from its top.  Then one pass in row order: keys above it stay, and of those equal to it the lowest rows.
 template <bool HELD>
@@ -425,26 +425,18 @@ __global__ void __launch_bounds__(1024) BlocksEvictSelectKernel(BlocksArgs a, co
     const uint32_t lo_row = first, hi_row = n - last, want = take - first - last;
     // a wavefront has the rows chunk * wave .., 64 at a time: what it keeps lies together in the output
     const uint32_t chunk = (n + 1023) / 1024 * 64, row0 = wave * chunk;
-    uint32_t held[HELD ? kEvictKeys : 1];
+    extern __shared__ uint32_t s_keys[];
     if (HELD)
-#pragma unroll
-        for (uint32_t i = 0; i < kEvictKeys; ++i) {
-            const uint32_t j = row0 + i * 64 + lane;
-            held[i] = i * 64 < chunk && j < n ? __float_as_uint(ms[j]) : 0u;
+#pragma unroll 4
+        for (uint32_t i = 0; i < chunk; i += 64) {
+            const uint32_t j = row0 + i + lane;
+            if (j < n) s_keys[j] = BlocksMassKey(ms[j]);
         }
-    if (HELD)
-#pragma unroll
-        for (uint32_t i = 0; i < kEvictKeys; ++i) held[i] = BlocksMassKey(__uint_as_float(held[i]));
     auto each = [&](auto&& f) {   // f(row, key) of the wavefront's rows, in their order
-        if (HELD) {
-#pragma unroll
-            for (uint32_t i = 0; i < kEvictKeys; ++i)
-                if (i * 64 < chunk) f(row0 + i * 64 + lane, held[i]);
-        } else {
-            for (uint32_t i = 0; i < chunk; i += 64) {
-                const uint32_t j = row0 + i + lane;
-                f(j, j < n ? BlocksMassKey(ms[j]) : 0u);
-            }
+#pragma unroll 4
+        for (uint32_t i = 0; i < chunk; i += 64) {
+            const uint32_t j = row0 + i + lane, at = min(j, n - 1);
+            f(j, HELD ? s_keys[at] : BlocksMassKey(ms[at]));
         }
     };
     uint32_t v = 0, left = want;   // key bits found; how many of the keys that agree with them stay
@@ -608,8 +600,10 @@ gpann_status gpann_blocks_evict(const gpann_blocks_layout* L, const void* k, con
     const BlocksArgs a = BlocksMakeArgs(L, nullptr, k, v, nullptr, 0);
     if (a.B == 0) return GPANN_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a.Tk <= kEvictKeys * 1024)
-        hipLaunchKernelGGL(BlocksEvictSelectKernel<true>, dim3(a.Hkv, a.B), dim3(1024), 0, st, a, mass, keep, first, last, rows, count);
+    const size_t lds = ((size_t)a.Tk + 64) * 4;
+    if (a.Tk <= kEvictKeys) GPANN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(BlocksEvictSelectKernel<true>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    if (a.Tk <= kEvictKeys)
+        hipLaunchKernelGGL(BlocksEvictSelectKernel<true>, dim3(a.Hkv, a.B), dim3(1024), lds, st, a, mass, keep, first, last, rows, count);
     else
         hipLaunchKernelGGL(BlocksEvictSelectKernel<false>, dim3(a.Hkv, a.B), dim3(1024), 0, st, a, mass, keep, first, last, rows, count);
     GPANN_HIP_TRY(hipGetLastError());

@@ -557,15 +557,24 @@ __global__ void __launch_bounds__(512) BlocksWeighKernel(BlocksArgs a, uint32_t 
     const uint32_t die = blockIdx.x & 7, pairs = a.B * a.Hkv, per_pair = a.nblk * pieces, waves = (gridDim.x >> 3) * 8;
     const uint64_t tasks = (uint64_t)((pairs + 7 - die) / 8) * per_pair;   // of the pairs that are `die` modulo 8
     const uint32_t inverse = a.G > 1 ? 0xFFFFFFFFu / a.G + 1 : 0;
+    // a pair's pieces are dealt to the wavefronts in an order of its own: the first block, which most query rows probe, would else always fall to the same one
+    auto piece_of = [&](uint64_t task, uint32_t& pair) -> uint32_t {
+        const uint32_t which = (uint32_t)(task / per_pair);
+        pair = which * 8 + die;
+        return (uint32_t)((task % per_pair + (uint64_t)which * 61) % per_pair);
+    };
     auto first_words = [&](uint64_t task) -> uint32_t {
         if (task >= tasks) return 0u;
-        const uint64_t block = (uint64_t)((uint32_t)(task / per_pair) * 8 + die) * a.nblk + (uint32_t)(task % per_pair) / pieces;
+        uint32_t pair;
+        const uint32_t x = piece_of(task, pair);
+        const uint64_t block = (uint64_t)pair * a.nblk + x / pieces;
         return lane < words ? bits[block * words + lane] : 0u;
     };
     uint64_t task = (blockIdx.x >> 3) * 8 + wave;
     uint32_t ahead = first_words(task);
     for (; task < tasks; task += waves) {
-        const uint32_t pair = (uint32_t)(task / per_pair) * 8 + die, x = (uint32_t)(task % per_pair), block = x / pieces, in_block = x % pieces * 64;
+        uint32_t pair;
+        const uint32_t x = piece_of(task, pair), block = x / pieces, in_block = x % pieces * 64;
         const uint32_t b = pair / a.Hkv, h = pair % a.Hkv, tiles = min(4u, (a.bs - in_block) / 16);
         const int key0 = (int)(block * a.bs + in_block), mine = key0 + (int)lane;
         const bool writes = lane < tiles * 16 && mine < (int)a.Tk;

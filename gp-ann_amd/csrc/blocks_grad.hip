@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
 }
 
 // ---- which query rows probe a block -------------------------------------------------------------------------------------------------------------
-constexpr uint32_t kMarkRows = 256, kMarkBlocks = 1024;   // query rows and blocks of a workgroup
+constexpr uint32_t kMarkRows = 128, kMarkBlocks = 512;   // query rows and blocks of a workgroup
 // One workgroup per pair, kMarkRows query rows and kMarkBlocks blocks: bits are set in LDS and every word is written, so nothing has to be cleared
 __global__ void __launch_bounds__(256) BlocksBitsKernel(BlocksArgs a, uint32_t words, uint32_t* __restrict__ bits) {
     __shared__ uint32_t s_bits[kMarkBlocks * (kMarkRows / 32)];
