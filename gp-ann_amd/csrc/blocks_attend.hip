@@ -214,13 +214,13 @@ __global__ void __launch_bounds__(512) BlocksAttendKernel(BlocksArgs a, uint32_t
 }
 
 // ---- forward, neighbouring query rows together ----------------------------------------------------------------------------------------------------
-// NT tiles of 16 keys of the stage at LDS byte `at` against a wavefront's CT x 16 columns; `mask`: which of its query rows look at them.  Operands are read in
+// NT tiles of 16 keys, the first at LDS byte `at`, against a wavefront's CT x 16 columns; `mask`: which of its query rows look at them.  Operands are read in
 // batches ahead of the products that need them (the scheduling barriers keep the compiler from pairing every read with its use, a full LDS latency each).
 // scale2 >= 0 (the sign is the queries').
-template <bool BF16, int DC, int CT, int NT>
-__device__ __forceinline__ void BlocksWalkAttend(float scale2, uint32_t tile0, const BlocksWalkAddresses<DC>& ad, uint32_t at, const int (&start)[4],
-                                                 const uint32_t (&mask)[4], const BlocksWalkColumns<CT>& col, uint32_t g4, const u32x4_t (&q)[CT][DC / 2],
-                                                 f32x4_t (&o)[CT][DC], float (&top)[CT], float (&sum)[CT]) {
+template <bool BF16, int DC, int CT, int NT, typename F>
+__device__ __forceinline__ void BlocksWalkAttend(float scale2, const BlocksWalkAddresses<DC>& ad, uint32_t at, const int (&start)[NT],
+                                                 const uint32_t (&mask)[NT], const BlocksWalkColumns<CT>& col, uint32_t g4, const u32x4_t (&q)[CT][DC / 2],
+                                                 f32x4_t (&o)[CT][DC], float (&top)[CT], float (&sum)[CT], F&& meanwhile) {
     using S = BlocksWalkShape<DC>;
     constexpr uint32_t TILE = S::D * 32;   // bytes of 16 rows
     constexpr int KS = DC / 2, BATCH = DC * CT > 8 ? 2 : NT;
@@ -229,10 +229,10 @@ __device__ __forceinline__ void BlocksWalkAttend(float scale2, uint32_t tile0, c
 #pragma unroll
     for (int y0 = 0; y0 < NT; y0 += BATCH) {
         u32x4_t k[BATCH][KS];
+        ad.EachRowStep(at, [&](int s, uint32_t x) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int y = 0; y < BATCH; ++y) k[y][s] = BlocksReadRow(at + ad.rows[s] + (tile0 + y0 + y) * TILE);
+            for (int y = 0; y < BATCH; ++y) k[y][s] = BlocksReadRow(x + (y0 + y) * TILE);
+        });
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < CT; ++c)
@@ -245,15 +245,17 @@ __device__ __forceinline__ void BlocksWalkAttend(float scale2, uint32_t tile0, c
 #pragma unroll
                 for (int y = 0; y < BATCH; ++y) x[c][y0 + y] = BlocksMfma<BF16>(k[y][s], q[c][s], x[c][y0 + y]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    meanwhile();   // the next stage is asked for under the products' cover: asked for by all wavefronts right behind a barrier, it would hold them all up
     u32x2_t v[DC][2];
+    ad.template EachDimension<DC>(at, [&](int d, uint32_t x) {
 #pragma unroll
-    for (int d = 0; d < DC; ++d)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) v[d][y] = BlocksReadTransposed(at + ad.turned[d] + S::TENSOR + (tile0 + y) * TILE);
+        for (int y = 0; y < 2; ++y) v[d][y] = BlocksReadTransposed(x + S::TENSOR + y * TILE);
+    });
     __builtin_amdgcn_sched_barrier(0);
     bool plain = true;   // every column looks at every key
 #pragma unroll
-    for (int y = 0; y < NT; ++y) plain = plain && mask[tile0 + y] == col.full && start[tile0 + y] + 16 <= col.seen_by_all;
+    for (int y = 0; y < NT; ++y) plain = plain && mask[y] == col.full && start[y] + 16 <= col.seen_by_all;
     float from[CT][NT], best[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -267,9 +269,9 @@ __device__ __forceinline__ void BlocksWalkAttend(float scale2, uint32_t tile0, c
         } else {
 #pragma unroll
             for (int y = 0; y < NT; ++y) {
-                const bool member = (mask[tile0 + y] >> col.in[c]) & 1;
-                if (start[tile0 + y] + 16 > col.seen_by_all) {
-                    const int limit = col.visible[c] - start[tile0 + y];
+                const bool member = (mask[y] >> col.in[c]) & 1;
+                if (start[y] + 16 > col.seen_by_all) {
+                    const int limit = col.visible[c] - start[y];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[c][y][i] = (int)g4 + i < limit ? x[c][y][i] : -inf;
                 }
@@ -313,10 +315,10 @@ __device__ __forceinline__ void BlocksWalkAttend(float scale2, uint32_t tile0, c
     for (int z = 0; z < NT / 2; ++z) {
         u32x2_t next[DC][2];
         if (z + 1 < NT / 2) {
+            ad.template EachDimension<DC>(at, [&](int d, uint32_t x) {
 #pragma unroll
-            for (int d = 0; d < DC; ++d)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) next[d][y] = BlocksReadTransposed(at + ad.turned[d] + S::TENSOR + (tile0 + 2 * z + 2 + y) * TILE);
+                for (int y = 0; y < 2; ++y) next[d][y] = BlocksReadTransposed(x + S::TENSOR + (2 * z + 2 + y) * TILE);
+            });
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -333,13 +335,14 @@ __device__ __forceinline__ void BlocksWalkAttend(float scale2, uint32_t tile0, c
     }
 }
 
-template <bool BF16, int DC, int CT>
+// NT: tiles taken at a time, 4 where a block is a multiple of them
+template <bool BF16, int DC, int CT, int NT>
 __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint32_t tpw, uint32_t mtiles, uint32_t tiles, uint16_t* __restrict__ out,
                                                               float* __restrict__ lse) {
     TakeWholeRegisterFile();
     using S = BlocksWalkShape<DC>;
     constexpr int KS = DC / 2;
-    extern __shared__ __attribute__((aligned(16))) char s_walk[];   // stages, tables
+    extern __shared__ __attribute__((aligned(1024))) char s_walk[];   // stages, tables
     __shared__ uint32_t s_count, s_scratch[8][64];
     const BlocksWalkTables<DC> tab(s_walk);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -389,34 +392,36 @@ __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint
 #pragma unroll
         for (uint32_t s = 0; s + 1 < S::BUFFERS; ++s)
             if (s < stages) {
-                d[s] = walk.Describe(a, w, tab, window, s, units, col.seen_by_any);
-                walk.Load(d[s], lds + s * S::STAGE);
+                const BlocksWalkSource from = walk.Describe(a, w, tab, window, s, units, col.seen_by_any, d[s]);
+                walk.Load(from, lds + s * S::STAGE);
             }
         uint32_t buf = 0;
         for (uint32_t s = 0; s < stages; ++s) {
             const bool more = s + S::BUFFERS - 1 < stages;
-            if (more) d[S::BUFFERS - 1] = walk.Describe(a, w, tab, window, s + S::BUFFERS - 1, units, col.seen_by_any);
+            const BlocksWalkSource from = walk.Describe(a, w, tab, window, s + S::BUFFERS - 1, units, col.seen_by_any, d[S::BUFFERS - 1]);
             if (S::BUFFERS > 2 && s + 1 < stages)
                 BlocksDmaWait<(S::BUFFERS - 2) * S::LOADS>();
             else
                 BlocksDmaWait<0>();
             BlocksStageBarrier();   // stage s has landed, and nobody reads stage s - 1 any more
-            if (more) walk.Load(d[S::BUFFERS - 1], lds + (buf == 0 ? S::BUFFERS - 1 : buf - 1) * S::STAGE);
-            int start[4];
-            uint32_t mask[4];
+            bool asked = false;
+            auto load = [&]() {
+                if (more && !asked) walk.Load(from, lds + (buf == 0 ? S::BUFFERS - 1 : buf - 1) * S::STAGE);
+                asked = true;
+            };
+#pragma unroll 1
+            for (uint32_t z = 0; z < 4; z += NT) {
+                int start[NT];
+                uint32_t mask[NT], any = 0;
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                start[y] = __builtin_amdgcn_readlane(d[0].start, y);
-                mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)d[0].mask, y);
+                for (uint32_t y = 0; y < NT; ++y) {
+                    start[y] = __builtin_amdgcn_readlane(d[0].start, (int)(z + y));
+                    mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)d[0].mask, (int)(z + y));
+                    any |= mask[y];
+                }
+                if (any) BlocksWalkAttend<BF16, DC, CT, NT>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, o, top, sum, load);
             }
-            const uint32_t at = lds + buf * S::STAGE;
-            const bool first = mask[0] | mask[1], second = mask[2] | mask[3];
-            if (first && second)
-                BlocksWalkAttend<BF16, DC, CT, 4>(scale2, 0, ad, at, start, mask, col, g * 4, q, o, top, sum);
-            else if (first)
-                BlocksWalkAttend<BF16, DC, CT, 2>(scale2, 0, ad, at, start, mask, col, g * 4, q, o, top, sum);
-            else if (second)
-                BlocksWalkAttend<BF16, DC, CT, 2>(scale2, 2, ad, at, start, mask, col, g * 4, q, o, top, sum);
+            load();
 #pragma unroll
             for (uint32_t y = 0; y + 1 < S::BUFFERS; ++y) d[y] = d[y + 1];
             buf = buf + 1 == S::BUFFERS ? 0 : buf + 1;
@@ -653,11 +658,11 @@ __global__ void __launch_bounds__(512) BlocksWeighKernel(BlocksArgs a, uint32_t 
 // ---- host -----------------------------------------------------------------------------------------------------------------------------------
 static size_t WeighSpace(const BlocksArgs& a) { return a.Tq <= 1 ? 0 : BlocksAlign((size_t)a.B * a.Hkv * a.nblk * ((a.Tq + 31) / 32) * 4); }
 
-template <bool BF16, int DC, int CT>
+template <bool BF16, int DC, int CT, int NT>
 static gpann_status AttendWalk(const BlocksArgs& a, uint16_t* out, float* lse, hipStream_t st) {
     const uint32_t cols = 16 * CT, mtiles = (a.G + cols - 1) / cols, tpw = std::max(1u, cols / a.G);
     const uint64_t waves = mtiles > 1 ? (uint64_t)a.Tq * mtiles : (a.Tq + tpw - 1) / tpw, tiles = (waves + 7) / 8;
-    return BlocksLaunch(BlocksAttendWalkKernel<BF16, DC, CT>, BlocksPairGrid((uint64_t)a.B * a.Hkv, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, lse);
+    return BlocksLaunch(BlocksAttendWalkKernel<BF16, DC, CT, NT>, BlocksPairGrid((uint64_t)a.B * a.Hkv, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, lse);
 }
 
 template <bool BF16, int DC>
@@ -668,8 +673,11 @@ static gpann_status Attend(const BlocksArgs& a, uint16_t* out, float* lse, hipSt
         // 32 columns a wavefront read LDS half as often for each, but make half the workgroups (one per CU at a time) of a larger union: 8192 rows x 32 heads,
         // 1024 workgroups of 32 columns, 536 us against 588; 777 rows x 12 heads, 120 workgroups, 152 us against 103.  (Wide heads have no registers for it.)
         if constexpr (DC <= 8)
-            if (pairs * (((uint64_t)a.Tq * a.G + 255) / 256) >= 512) return AttendWalk<BF16, DC, 2>(a, out, lse, st);
-        return AttendWalk<BF16, DC, 1>(a, out, lse, st);
+            if (pairs * (((uint64_t)a.Tq * a.G + 255) / 256) >= 512)
+                return a.bs % 64 == 0 ? AttendWalk<BF16, DC, 2, 4>(a, out, lse, st) : AttendWalk<BF16, DC, 2, 2>(a, out, lse, st);
+        if constexpr (DC <= 8)
+            if (a.bs % 64 == 0) return AttendWalk<BF16, DC, 1, 4>(a, out, lse, st);
+        return AttendWalk<BF16, DC, 1, 2>(a, out, lse, st);
     }
     // few query rows: their keys are divided over wavefronts until the chip's 2048 have something to do
     uint32_t waves = 1;

@@ -103,28 +103,24 @@ __device__ __forceinline__ void BlocksQueryGradRow(const BlocksArgs& a, uint32_t
     }
 }
 
-// NT tiles of 16 keys of the stage at LDS byte `at` against a wavefront's 16 columns
-template <bool BF16, int DC, int NT>
-__device__ __forceinline__ void BlocksWalkQueryGrad(float scale2, uint32_t tile0, const BlocksWalkAddresses<DC>& ad, uint32_t at, const int (&start)[4],
-                                                    const uint32_t (&mask)[4], const BlocksWalkColumns<1>& col, uint32_t g4, const u32x4_t (&q)[DC / 2],
-                                                    const u32x4_t (&go)[DC / 2], float lse2, float delta, f32x4_t (&acc)[DC], f32x4_t (&wk)[DC], float& off) {
+// two tiles of 16 keys, the first at LDS byte `at`, against a wavefront's 16 columns
+template <bool BF16, int DC, typename F>
+__device__ __forceinline__ void BlocksWalkQueryGrad(float scale2, const BlocksWalkAddresses<DC>& ad, uint32_t at, const int (&start)[2], const uint32_t (&mask)[2],
+                                                    const BlocksWalkColumns<1>& col, uint32_t g4, const u32x4_t (&q)[DC / 2], const u32x4_t (&go)[DC / 2], float lse2,
+                                                    float delta, f32x4_t (&acc)[DC], f32x4_t (&wk)[DC], float& off, F&& meanwhile) {
     using S = BlocksWalkShape<DC>;
     constexpr uint32_t TILE = S::D * 32;
     constexpr int KS = DC / 2;
-#pragma unroll
-    for (int z = 0; z < NT / 2; ++z) {
-        const uint32_t t0 = tile0 + 2 * z;
+    {
         f32x4_t x[2], y[2];
         {
             u32x4_t k[2][KS], v[2][KS];
+            ad.EachRowStep(at, [&](int s, uint32_t byte) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) k[i][s] = BlocksReadRow(at + ad.rows[s] + (t0 + i) * TILE);
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) v[i][s] = BlocksReadRow(at + ad.rows[s] + S::TENSOR + (t0 + i) * TILE);
+                for (int i = 0; i < 2; ++i) k[i][s] = BlocksReadRow(byte + i * TILE);
+            });
+            __builtin_amdgcn_sched_barrier(0);
+            ad.EachRowStep(at, [&](int s, uint32_t byte) { v[0][s] = BlocksReadRow(byte + S::TENSOR); });
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 2; ++i) x[i] = y[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -132,23 +128,28 @@ __device__ __forceinline__ void BlocksWalkQueryGrad(float scale2, uint32_t tile0
             for (int s = 0; s < KS; ++s)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) x[i] = BlocksMfma<BF16>(k[i][s], q[s], x[i]);
+            __builtin_amdgcn_sched_barrier(0);
+            ad.EachRowStep(at, [&](int s, uint32_t byte) { v[1][s] = BlocksReadRow(byte + S::TENSOR + TILE); });
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) y[i] = BlocksMfma<BF16>(v[i][s], go[s], y[i]);
+                for (int s = 0; s < KS; ++s) y[i] = BlocksMfma<BF16>(v[i][s], go[s], y[i]);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        meanwhile();   // the next stage is asked for under the products' cover
         u32x2_t kt[DC][2];
+        ad.template EachDimension<DC>(at, [&](int d, uint32_t byte) {
 #pragma unroll
-        for (int d = 0; d < DC; ++d)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) kt[d][i] = BlocksReadTransposed(at + ad.turned[d] + (t0 + i) * TILE);
+            for (int i = 0; i < 2; ++i) kt[d][i] = BlocksReadTransposed(byte + i * TILE);
+        });
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const bool member = (mask[t0 + i] >> col.in[0]) & 1;
+            const bool member = (mask[i] >> col.in[0]) & 1;
             const float less = member ? -lse2 : -__builtin_inff();
-            if (start[t0 + i] + 16 > col.seen_by_all) {
-                const int limit = col.visible[0] - start[t0 + i];
+            if (start[i] + 16 > col.seen_by_all) {
+                const int limit = col.visible[0] - start[i];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[i][j] = (int)g4 + j < limit ? x[i][j] : -__builtin_inff();
             }
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
     TakeWholeRegisterFile();
     using S = BlocksWalkShape<DC>;
     constexpr int KS = DC / 2;
-    extern __shared__ __attribute__((aligned(16))) char s_walk[];
+    extern __shared__ __attribute__((aligned(1024))) char s_walk[];
     __shared__ uint32_t s_count, s_scratch[8][64];
     const BlocksWalkTables<DC> tab(s_walk);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -232,29 +233,36 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
 #pragma unroll
         for (uint32_t s = 0; s + 1 < S::BUFFERS; ++s)
             if (s < stages) {
-                d[s] = walk.Describe(a, w, tab, window, s, units, col.seen_by_any);
-                walk.Load(d[s], lds + s * S::STAGE);
+                const BlocksWalkSource from = walk.Describe(a, w, tab, window, s, units, col.seen_by_any, d[s]);
+                walk.Load(from, lds + s * S::STAGE);
             }
         uint32_t buf = 0;
         for (uint32_t s = 0; s < stages; ++s) {
             const bool more = s + S::BUFFERS - 1 < stages;
-            if (more) d[S::BUFFERS - 1] = walk.Describe(a, w, tab, window, s + S::BUFFERS - 1, units, col.seen_by_any);
+            const BlocksWalkSource from = walk.Describe(a, w, tab, window, s + S::BUFFERS - 1, units, col.seen_by_any, d[S::BUFFERS - 1]);
             if (S::BUFFERS > 2 && s + 1 < stages)
                 BlocksDmaWait<(S::BUFFERS - 2) * S::LOADS>();
             else
                 BlocksDmaWait<0>();
             BlocksStageBarrier();
-            if (more) walk.Load(d[S::BUFFERS - 1], lds + (buf == 0 ? S::BUFFERS - 1 : buf - 1) * S::STAGE);
-            int start[4];
-            uint32_t mask[4];
+            bool asked = false;
+            auto load = [&]() {
+                if (more && !asked) walk.Load(from, lds + (buf == 0 ? S::BUFFERS - 1 : buf - 1) * S::STAGE);
+                asked = true;
+            };
+#pragma unroll 1
+            for (uint32_t z = 0; z < 4; z += 2) {
+                int start[2];
+                uint32_t mask[2];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                start[y] = __builtin_amdgcn_readlane(d[0].start, y);
-                mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)d[0].mask, y);
+                for (uint32_t y = 0; y < 2; ++y) {
+                    start[y] = __builtin_amdgcn_readlane(d[0].start, (int)(z + y));
+                    mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)d[0].mask, (int)(z + y));
+                }
+                if (mask[0] | mask[1])
+                    BlocksWalkQueryGrad<BF16, DC>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, go, lse2, delta, acc, wk, off, load);
             }
-            const uint32_t at = lds + buf * S::STAGE;
-            if (mask[0] | mask[1]) BlocksWalkQueryGrad<BF16, DC, 2>(scale2, 0, ad, at, start, mask, col, g * 4, q, go, lse2, delta, acc, wk, off);
-            if (mask[2] | mask[3]) BlocksWalkQueryGrad<BF16, DC, 2>(scale2, 2, ad, at, start, mask, col, g * 4, q, go, lse2, delta, acc, wk, off);
+            load();
 #pragma unroll
             for (uint32_t y = 0; y + 1 < S::BUFFERS; ++y) d[y] = d[y + 1];
             buf = buf + 1 == S::BUFFERS ? 0 : buf + 1;
@@ -390,7 +398,7 @@ __global__ void __launch_bounds__(1024) BlocksPartsKernel(BlocksArgs a, uint32_t
 // Four stages: one being read transposed, the next by rows, one in flight, one being asked for.
 template <int DC, int RGS>
 struct BlocksKeyShape {
-    static constexpr uint32_t D = DC * 16, CPR = D / 8, ROWS = 32 * RGS, TENSOR = ROWS * D * 2, STAGE = 2 * TENSOR + 512, BUFFERS = 4;
+    static constexpr uint32_t D = DC * 16, CPR = D / 8, ROWS = 32 * RGS, TENSOR = ROWS * D * 2, STAGE = 2 * TENSOR + 1024, BUFFERS = 4;
 };
 
 template <bool BF16, int DC, int ND, int RGS>
@@ -402,7 +410,7 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
     using W = BlocksWalkShape<DC>;
     using S = BlocksKeyShape<DC, RGS>;
     constexpr int KS = DC / 2, D = DC * 16, OD = DC / ND;
-    extern __shared__ __attribute__((aligned(16))) char s_keys[];   // stages {Q rows, dO rows, lse2, delta}; afterwards the sums of the row groups; the row list behind
+    extern __shared__ __attribute__((aligned(1024))) char s_keys[];   // stages {Q rows, dO rows, lse2, delta}; afterwards the sums of the row groups; the row list behind
     uint32_t* s_list = reinterpret_cast<uint32_t*>(s_keys + S::BUFFERS * S::STAGE);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     uint32_t pair, x;
@@ -470,7 +478,7 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
             if (a.scale2 <= 0.f) kf[s] = a.scale2 == 0.f ? u32x4_t{0u, 0u, 0u, 0u} : kf[s] ^ 0x80008000u;   // the scale's sign, on the keys' side here
             asm volatile("" : "+v"(kf[s]), "+v"(vf[s]));
         }
-        const BlocksWalkAddresses<DC> ad(lane);
+        const BlocksWalkAddresses<DC> ad(lane, hd * OD);
         const uint32_t lds = BlocksLdsAddress(s_keys);
         // Row i of the part: query row list[i / G], head i % G of the group.  A wavefront asks for PER / 8 pieces of 64 / CPR rows of both tensors a stage,
         // the last one for the rows' numbers too; `place`: what a lane adds to a row's address.
@@ -520,29 +528,18 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
             BlocksDmaWaitFor(mine * min(behind, stages - 1 - min(s, stages - 1)));
             BlocksStageBarrier();
         };
-        // LDS addresses of this lane's operands: everything but the stage is a constant offset
-        uint32_t by_rows[KS], turned[OD], by_info = lds + 2 * S::TENSOR + (rg * 32 + g * 4) * 4;
-#pragma unroll
-        for (int j = 0; j < KS; ++j) by_rows[j] = lds + rg * 2 * D * 32 + ad.rows[j];
-#pragma unroll
-        for (int d = 0; d < OD; ++d) turned[d] = lds + rg * 2 * D * 32 + ad.turned[hd * OD + d];
+        const uint32_t by_info = lds + 2 * S::TENSOR + (rg * 32 + g * 4) * 4, by_row = lds + rg * 2 * D * 32;
         auto rows_of = [&](uint32_t stage, uint32_t tensor, u32x4_t(&f)[2][KS]) {
-#pragma unroll
-            for (int j = 0; j < KS; ++j) {
-                uint32_t at = by_rows[j] + stage;
-                asm volatile("" : "+v"(at));
+            ad.EachRowStep(by_row + stage, [&](int j, uint32_t at) {
 #pragma unroll
                 for (int y = 0; y < 2; ++y) f[y][j] = BlocksReadRow(at + tensor + y * D * 32);
-            }
+            });
         };
         auto turned_of = [&](uint32_t stage, uint32_t tensor, u32x2_t(&f)[OD][2]) {
-#pragma unroll
-            for (int d = 0; d < OD; ++d) {
-                uint32_t at = turned[d] + stage;
-                asm volatile("" : "+v"(at));
+            ad.template EachDimension<OD>(by_row + stage, [&](int d, uint32_t at) {
 #pragma unroll
                 for (int y = 0; y < 2; ++y) f[d][y] = BlocksReadTransposed(at + tensor + y * D * 32);
-            }
+            });
         };
         auto product = [&](const u32x4_t(&f)[2][KS], const u32x4_t(&keys)[KS], f32x4_t(&x)[2]) {
 #pragma unroll

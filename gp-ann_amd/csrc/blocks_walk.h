@@ -177,10 +177,13 @@ __device__ __forceinline__ uint32_t BlocksWalkList(const BlocksArgs& a, const Bl
     return *s_count;
 }
 
-// The four 16-row tiles of a stage, tile y in lane y
-struct BlocksWalkStage {
+// The four 16-row tiles of a stage, tile y in lane y: for the loads ...
+struct BlocksWalkSource {
     uint4 address;     // of its block
     int row, last;     // its first row in the block; the last row of the block that the sequence has
+};
+// ... and for the products
+struct BlocksWalkStage {
     int start;         // its position
     uint32_t mask;     // which query rows of this wavefront look at it
 };
@@ -189,34 +192,36 @@ struct BlocksWalkStage {
 template <int DC>
 struct BlocksWalker {
     using S = BlocksWalkShape<DC>;
-    uint32_t row[S::LOADS], chunk[S::LOADS];   // row in its tile, byte offset of the chunk in the row
+    // row in its tile and byte offset of the chunk in the row: all of a wavefront's instructions of a stage have the same where a row is a power of two
+    static constexpr uint32_t PLACES = (S::CPR & (S::CPR - 1)) == 0 ? 1 : S::LOADS;
+    uint32_t row[PLACES], chunk[PLACES];
     uint32_t wave, lane, tpb, inverse, krow, vrow;
     __device__ __forceinline__ BlocksWalker(const BlocksArgs& a, uint32_t wave_, uint32_t lane_) : wave(wave_), lane(lane_), tpb(a.bs / 16) {
         inverse = tpb > 1 ? 0xFFFFFFFFu / tpb + 1 : 0;
         krow = (uint32_t)a.ks[1] * 2;
         vrow = (uint32_t)a.vs[1] * 2;
 #pragma unroll
-        for (uint32_t x = 0; x < S::LOADS; ++x) {
+        for (uint32_t x = 0; x < PLACES; ++x) {
             const uint32_t at = (wave + 8 * x) % S::CPR * 64 + lane, r = at / S::CPR;
             row[x] = r % 16;
             chunk[x] = S::Chunk(at % S::CPR, r) * 16;
         }
     }
     // `seen`: rows that the last query row of this wavefront sees (a prefix)
-    __device__ __forceinline__ BlocksWalkStage Describe(const BlocksArgs& a, const BlocksWalkRows& w, const BlocksWalkTables<DC>& tab, uint32_t window, uint32_t s,
-                                                        uint32_t units, int seen) const {
-        BlocksWalkStage d;
+    __device__ __forceinline__ BlocksWalkSource Describe(const BlocksArgs& a, const BlocksWalkRows& w, const BlocksWalkTables<DC>& tab, uint32_t window, uint32_t s,
+                                                         uint32_t units, int seen, BlocksWalkStage& st) const {
+        BlocksWalkSource d;
         const uint32_t unit = 4 * s + (lane & 3), in = min(unit, units - 1), e = inverse ? __umulhi(in, inverse) : in;   // in / tpb, exact below 2^16
         const int block = tab.list[e];
         d.address = tab.address[e];
         d.row = (int)(in - e * tpb) * 16;
         d.last = w.n - 1 - block * (int)a.bs;
-        d.start = block * (int)a.bs + d.row;
-        d.mask = tab.masks[(block - (int)window) * 8 + (int)wave];
-        if (unit >= units || d.start >= seen) d.mask = 0;
+        st.start = block * (int)a.bs + d.row;
+        st.mask = tab.masks[(block - (int)window) * 8 + (int)wave];
+        if (unit >= units || st.start >= seen) st.mask = 0;
         return d;
     }
-    __device__ __forceinline__ void Load(const BlocksWalkStage& d, uint32_t to) const {
+    __device__ __forceinline__ void Load(const BlocksWalkSource& d, uint32_t to) const {
 #pragma unroll
         for (uint32_t x = 0; x < S::LOADS; ++x) {
             const uint32_t j = wave + 8 * x;
@@ -225,23 +230,48 @@ struct BlocksWalker {
             const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(value ? d.address.z : d.address.x), tile);
             const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(value ? d.address.w : d.address.y), tile);
             const int first = __builtin_amdgcn_readlane(d.row, tile), last = __builtin_amdgcn_readlane(d.last, tile);
-            const uint32_t r = (uint32_t)min(first + (int)row[x], last);   // rows past the sequence's end are not read
-            BlocksDma(((uint64_t)hi << 32) | lo, r * (value ? vrow : krow) + chunk[x], to + (value ? S::TENSOR : 0) + j % S::CPR * 1024);
+            const uint32_t place = PLACES == 1 ? 0 : x, r = (uint32_t)min(first + (int)row[place], last);   // rows past the sequence's end are not read
+            BlocksDma(((uint64_t)hi << 32) | lo, r * (value ? vrow : krow) + chunk[place], to + (value ? S::TENSOR : 0) + j % S::CPR * 1024);
         }
     }
 };
 
-// LDS addresses of a lane's part of a stage's operands, relative to the stage
+// LDS addresses of a lane's part of a stage's operands.  Where a row is a power of two of chunks, a permuted chunk is an exclusive or, so step s and dimension
+// tile d are one exclusive or away from a base (stages begin at multiples of 1024 bytes): two registers instead of one for every step and tile.
 template <int DC>
 struct BlocksWalkAddresses {
-    uint32_t rows[DC / 2], turned[DC];   // by rows: step s of row lane % 16; transposed: 16 dimensions d of rows 4 g ..
-    __device__ __forceinline__ explicit BlocksWalkAddresses(uint32_t lane) {
-        using S = BlocksWalkShape<DC>;
+    using S = BlocksWalkShape<DC>;
+    static constexpr bool POWER = (S::CPR & (S::CPR - 1)) == 0;
+    uint32_t rows[POWER ? 1 : DC / 2], turned[POWER ? 1 : DC];
+    // `first`: the first of the dimension tiles that this lane's wavefront reads transposed
+    __device__ __forceinline__ explicit BlocksWalkAddresses(uint32_t lane, uint32_t first = 0) {
         const uint32_t r = lane & 15, g = lane >> 4, row = g * 4 + r / 4;
 #pragma unroll
-        for (uint32_t s = 0; s < DC / 2; ++s) rows[s] = (r * S::CPR + S::Slot(s * 4 + g, r)) * 16;
+        for (uint32_t s = 0; s < (POWER ? 1 : DC / 2); ++s) rows[s] = (r * S::CPR + S::Slot(s * 4 + g, r)) * 16;
 #pragma unroll
-        for (uint32_t d = 0; d < DC; ++d) turned[d] = (row * S::CPR + S::Slot(d * 2 + (r & 3) / 2, row)) * 16 + (r & 1) * 8;
+        for (uint32_t d = 0; d < (POWER ? 1 : DC); ++d) turned[d] = (row * S::CPR + S::Slot((first + d) * 2 + (r & 3) / 2, row)) * 16 + (r & 1) * 8;
+    }
+    // by rows: step s of row lane % 16 of the tile at LDS byte `at`; f(address of step s)
+    template <typename F>
+    __device__ __forceinline__ void EachRowStep(uint32_t at, F&& f) const {
+        const uint32_t base = at + rows[0];
+#pragma unroll
+        for (int s = 0; s < DC / 2; ++s) {
+            uint32_t x = POWER ? base ^ (64 * s) : at + rows[POWER ? 0 : s];
+            asm volatile("" : "+v"(x));   // (else the constant offsets that follow would be added on the vector unit, one by one)
+            f(s, x);
+        }
+    }
+    // transposed: 16 dimensions of rows 4 g .. of the tile at LDS byte `at`; a power of two of dimension tiles, or all that are left
+    template <int COUNT, typename F>
+    __device__ __forceinline__ void EachDimension(uint32_t at, F&& f) const {
+        const uint32_t base = at + turned[0];
+#pragma unroll
+        for (int d = 0; d < COUNT; ++d) {
+            uint32_t x = POWER ? base ^ (32 * d) : at + turned[POWER ? 0 : d];
+            asm volatile("" : "+v"(x));
+            f(d, x);
+        }
     }
 };
 
