@@ -214,77 +214,80 @@ __global__ void __launch_bounds__(512) BlocksAttendKernel(BlocksArgs a, uint32_t
 }
 
 // ---- forward, neighbouring query rows together ----------------------------------------------------------------------------------------------------
-// NT tiles of 16 keys, the first at LDS byte `at`, against a wavefront's CT x 16 columns; `mask`: which of its query rows look at them.  Operands are read in
-// batches ahead of the products that need them (the scheduling barriers keep the compiler from pairing every read with its use, a full LDS latency each).
-// scale2 >= 0 (the sign is the queries').
-template <bool BF16, int DC, int CT, int NT, typename F>
-__device__ __forceinline__ void BlocksWalkAttend(float scale2, const BlocksWalkAddresses<DC>& ad, uint32_t at, const int (&start)[NT],
-                                                 const uint32_t (&mask)[NT], const BlocksWalkColumns<CT>& col, uint32_t g4, const u32x4_t (&q)[CT][DC / 2],
+// NT tiles of 16 keys, the first at LDS byte `at`, against a wavefront's CT x 16 columns.  `mask`: which of its query rows look at them, of every tile or once
+// for all, which are of one block then; `start`: their positions, or the first one's.  Operands are read in batches ahead of the products that need them (the
+// scheduling barriers keep the compiler from pairing every read with its use, a full LDS latency each).  scale2 >= 0 (the sign is the queries').
+template <bool BF16, int DC, int CT, int NT, int NM, typename F>
+__device__ __forceinline__ void BlocksWalkAttend(float scale2, const BlocksWalkAddresses<DC>& ad, uint32_t at, const int (&start)[NM],
+                                                 const uint32_t (&mask)[NM], const BlocksWalkColumns<CT>& col, uint32_t g4, const u32x4_t (&q)[CT][DC / 2],
                                                  f32x4_t (&o)[CT][DC], float (&top)[CT], float (&sum)[CT], F&& meanwhile) {
     using S = BlocksWalkShape<DC>;
     constexpr uint32_t TILE = S::D * 32;   // bytes of 16 rows
-    constexpr int KS = DC / 2, BATCH = DC * CT > 8 ? 2 : NT;
+    constexpr int KS = DC / 2, BATCH = DC * CT > 8 ? 2 : NT, PER = NT / NM;
     const float inf = __builtin_inff();
     f32x4_t x[CT][NT];
+    {
+        uint32_t step[KS];
+        ad.RowSteps(at, step);
 #pragma unroll
-    for (int y0 = 0; y0 < NT; y0 += BATCH) {
-        u32x4_t k[BATCH][KS];
-        ad.EachRowStep(at, [&](int s, uint32_t x) {
+        for (int y0 = 0; y0 < NT; y0 += BATCH) {
+            u32x4_t k[BATCH][KS];
 #pragma unroll
-            for (int y = 0; y < BATCH; ++y) k[y][s] = BlocksReadRow(x + (y0 + y) * TILE);
-        });
-        __builtin_amdgcn_sched_barrier(0);
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-            for (int y = 0; y < BATCH; ++y) x[c][y0 + y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
+                for (int y = 0; y < BATCH; ++y) k[y][s] = BlocksReadRow(step[s] + (y0 + y) * TILE);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int y = 0; y < BATCH; ++y) x[c][y0 + y] = BlocksMfma<BF16>(k[y][s], q[c][s], x[c][y0 + y]);
+                for (int y = 0; y < BATCH; ++y) x[c][y0 + y] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int y = 0; y < BATCH; ++y) x[c][y0 + y] = BlocksMfma<BF16>(k[y][s], q[c][s], x[c][y0 + y]);
+        }
     }
     __builtin_amdgcn_sched_barrier(0);
     meanwhile();   // the next stage is asked for under the products' cover: asked for by all wavefronts right behind a barrier, it would hold them all up
+    uint32_t turned[DC];
     u32x2_t v[DC][2];
-    ad.template EachDimension<DC>(at, [&](int d, uint32_t x) {
+    ad.template Dimensions<DC>(at, turned);
 #pragma unroll
-        for (int y = 0; y < 2; ++y) v[d][y] = BlocksReadTransposed(x + S::TENSOR + y * TILE);
-    });
+    for (int d = 0; d < DC; ++d)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) v[d][y] = BlocksReadTransposed(turned[d] + S::TENSOR + y * TILE);
     __builtin_amdgcn_sched_barrier(0);
-    bool plain = true;   // every column looks at every key
 #pragma unroll
-    for (int y = 0; y < NT; ++y) plain = plain && mask[y] == col.full && start[y] + 16 <= col.seen_by_all;
-    float from[CT][NT], best[CT];
+    for (int e = 0; e < NM; ++e)
+        if (start[e] + 16 * PER > col.seen_by_all) {   // not every column sees every key
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                const int limit = col.visible[c] - start[e] - (int)g4;
+#pragma unroll
+                for (int y = 0; y < PER; ++y)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[c][e * PER + y][i] = y * 16 + i < limit ? x[c][e * PER + y][i] : -inf;
+            }
+        }
+    bool member[CT][NM];
+    float best[CT];
+    bool raise = false;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         best[c] = -inf;
-        if (plain) {
 #pragma unroll
-            for (int y = 0; y < NT; ++y) {
-                from[c][y] = 0.f;
-                best[c] = fmaxf(best[c], fmaxf(fmaxf(x[c][y][0], x[c][y][1]), fmaxf(x[c][y][2], x[c][y][3])));
-            }
-        } else {
+        for (int e = 0; e < NM; ++e) {
+            member[c][e] = (mask[e] >> col.in[c]) & 1;
+            float most = BlocksMaxOf4(x[c][e * PER]);
 #pragma unroll
-            for (int y = 0; y < NT; ++y) {
-                const bool member = (mask[y] >> col.in[c]) & 1;
-                if (start[y] + 16 > col.seen_by_all) {
-                    const int limit = col.visible[c] - start[y];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[c][y][i] = (int)g4 + i < limit ? x[c][y][i] : -inf;
-                }
-                from[c][y] = member ? 0.f : inf;
-                const float most = fmaxf(fmaxf(x[c][y][0], x[c][y][1]), fmaxf(x[c][y][2], x[c][y][3]));
-                best[c] = fmaxf(best[c], member ? most : -inf);
-            }
+            for (int y = 1; y < PER; ++y) most = BlocksMaxOf4(x[c][e * PER + y], most);
+            best[c] = fmaxf(best[c], member[c][e] ? most : -inf);
         }
         best[c] = BlocksMaxOver4(best[c]) * scale2;
+        raise = raise || best[c] > top[c] + kBlocksSlack;
     }
-    bool raise = false;
-#pragma unroll
-    for (int c = 0; c < CT; ++c) raise = raise || best[c] > top[c] + kBlocksSlack;
     if (__ballot(raise)) {
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
@@ -300,25 +303,23 @@ __device__ __forceinline__ void BlocksWalkAttend(float scale2, const BlocksWalkA
     }
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-        const float base = top[c] == -inf ? 0.f : top[c];
+        const float base = top[c] == -inf ? 0.f : -top[c];
 #pragma unroll
         for (int y = 0; y < NT; ++y) {
-            const float less = -(from[c][y] + base);   // -inf: a tile that the column does not look at
+            const float less = member[c][y / PER] ? base : -inf;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[c][y][i] = BlocksExp2(__builtin_fmaf(x[c][y][i], scale2, less));
-                sum[c] += x[c][y][i];
-            }
+            for (int i = 0; i < 4; ++i) x[c][y][i] = BlocksExp2(__builtin_fmaf(x[c][y][i], scale2, less));
+            sum[c] += (x[c][y][0] + x[c][y][1]) + (x[c][y][2] + x[c][y][3]);
         }
     }
 #pragma unroll
     for (int z = 0; z < NT / 2; ++z) {
         u32x2_t next[DC][2];
         if (z + 1 < NT / 2) {
-            ad.template EachDimension<DC>(at, [&](int d, uint32_t x) {
 #pragma unroll
-                for (int y = 0; y < 2; ++y) next[d][y] = BlocksReadTransposed(x + S::TENSOR + (2 * z + 2 + y) * TILE);
-            });
+            for (int d = 0; d < DC; ++d)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) next[d][y] = BlocksReadTransposed(turned[d] + S::TENSOR + (2 * z + 2 + y) * TILE);
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -342,6 +343,7 @@ __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint
     TakeWholeRegisterFile();
     using S = BlocksWalkShape<DC>;
     constexpr int KS = DC / 2;
+    constexpr bool ONE = NT == 4;
     extern __shared__ __attribute__((aligned(1024))) char s_walk[];   // stages, tables
     __shared__ uint32_t s_count, s_scratch[8][64];
     const BlocksWalkTables<DC> tab(s_walk);
@@ -388,17 +390,15 @@ __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint
     for (uint32_t window = 0; window < blocks; window += S::WINDOW) {
         const uint32_t in_window = min(S::WINDOW, blocks - window);
         const uint32_t units = BlocksWalkList<DC>(a, w, window, in_window, tab, &s_count) * tpb, stages = (units + 3) / 4;
-        BlocksWalkStage d[S::BUFFERS];   // of stages s, s + 1, ...
-#pragma unroll
-        for (uint32_t s = 0; s + 1 < S::BUFFERS; ++s)
-            if (s < stages) {
-                const BlocksWalkSource from = walk.Describe(a, w, tab, window, s, units, col.seen_by_any, d[s]);
-                walk.Load(from, lds + s * S::STAGE);
-            }
+        BlocksWalkStage now = {}, next = {};   // of the stages that are multiplied and loaded now
+        BlocksWalkSource from = {};
+        if (stages) from = walk.Describe(a, w, tab, window, 0, units, col.seen_by_any, next);
+        for (uint32_t s = 0; s + 1 < S::BUFFERS && s < stages; ++s) walk.Load(from, s, lds + s * S::STAGE);
         uint32_t buf = 0;
         for (uint32_t s = 0; s < stages; ++s) {
-            const bool more = s + S::BUFFERS - 1 < stages;
-            const BlocksWalkSource from = walk.Describe(a, w, tab, window, s + S::BUFFERS - 1, units, col.seen_by_any, d[S::BUFFERS - 1]);
+            const uint32_t ahead = s + S::BUFFERS - 1;
+            if (s % kDescribed == 0) now = next;
+            if (ahead % kDescribed == 0 && ahead < stages) from = walk.Describe(a, w, tab, window, ahead, units, col.seen_by_any, next);
             if (S::BUFFERS > 2 && s + 1 < stages)
                 BlocksDmaWait<(S::BUFFERS - 2) * S::LOADS>();
             else
@@ -406,24 +406,24 @@ __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint
             BlocksStageBarrier();   // stage s has landed, and nobody reads stage s - 1 any more
             bool asked = false;
             auto load = [&]() {
-                if (more && !asked) walk.Load(from, lds + (buf == 0 ? S::BUFFERS - 1 : buf - 1) * S::STAGE);
+                if (ahead < stages && !asked) walk.Load(from, ahead, lds + (buf == 0 ? S::BUFFERS - 1 : buf - 1) * S::STAGE);
                 asked = true;
             };
 #pragma unroll 1
             for (uint32_t z = 0; z < 4; z += NT) {
-                int start[NT];
-                uint32_t mask[NT], any = 0;
+                const uint32_t first = s % kDescribed * 4 + z;
+                int start[ONE ? 1 : NT];
+                uint32_t mask[ONE ? 1 : NT], any = 0;
 #pragma unroll
-                for (uint32_t y = 0; y < NT; ++y) {
-                    start[y] = __builtin_amdgcn_readlane(d[0].start, (int)(z + y));
-                    mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)d[0].mask, (int)(z + y));
+                for (uint32_t y = 0; y < (ONE ? 1 : NT); ++y) {
+                    start[y] = __builtin_amdgcn_readlane(now.start, (int)(first + y));
+                    mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)now.mask, (int)(first + y));
                     any |= mask[y];
                 }
-                if (any) BlocksWalkAttend<BF16, DC, CT, NT>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, o, top, sum, load);
+                if (any)
+                    BlocksWalkAttend<BF16, DC, CT, NT>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, o, top, sum, load);
             }
             load();
-#pragma unroll
-            for (uint32_t y = 0; y + 1 < S::BUFFERS; ++y) d[y] = d[y + 1];
             buf = buf + 1 == S::BUFFERS ? 0 : buf + 1;
         }
         __syncthreads();

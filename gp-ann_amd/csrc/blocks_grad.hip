@@ -103,81 +103,95 @@ __device__ __forceinline__ void BlocksQueryGradRow(const BlocksArgs& a, uint32_t
     }
 }
 
-// two tiles of 16 keys, the first at LDS byte `at`, against a wavefront's 16 columns
-template <bool BF16, int DC, typename F>
-__device__ __forceinline__ void BlocksWalkQueryGrad(float scale2, const BlocksWalkAddresses<DC>& ad, uint32_t at, const int (&start)[2], const uint32_t (&mask)[2],
+// two tiles of 16 keys, the first at LDS byte `at`, against a wavefront's 16 columns; `less_delta`: minus the column's delta, four times over
+template <bool BF16, int DC, int NM, typename F>
+__device__ __forceinline__ void BlocksWalkQueryGrad(float scale2, const BlocksWalkAddresses<DC>& ad, uint32_t at, const int (&start)[NM], const uint32_t (&mask)[NM],
                                                     const BlocksWalkColumns<1>& col, uint32_t g4, const u32x4_t (&q)[DC / 2], const u32x4_t (&go)[DC / 2], float lse2,
-                                                    float delta, f32x4_t (&acc)[DC], f32x4_t (&wk)[DC], float& off, F&& meanwhile) {
+                                                    const f32x4_t& less_delta, f32x4_t (&acc)[DC], f32x4_t (&wk)[DC], float& off, F&& meanwhile) {
     using S = BlocksWalkShape<DC>;
     constexpr uint32_t TILE = S::D * 32;
-    constexpr int KS = DC / 2;
+    constexpr int KS = DC / 2, PER = 2 / NM;
+    f32x4_t x[2], y[2];
     {
-        f32x4_t x[2], y[2];
-        {
-            u32x4_t k[2][KS], v[2][KS];
-            ad.EachRowStep(at, [&](int s, uint32_t byte) {
+        uint32_t step[KS];
+        u32x4_t k[2][KS], v[2][KS];
+        ad.RowSteps(at, step);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) k[i][s] = BlocksReadRow(byte + i * TILE);
-            });
-            __builtin_amdgcn_sched_barrier(0);
-            ad.EachRowStep(at, [&](int s, uint32_t byte) { v[0][s] = BlocksReadRow(byte + S::TENSOR); });
-            __builtin_amdgcn_sched_barrier(0);
+        for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) x[i] = y[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) x[i] = BlocksMfma<BF16>(k[i][s], q[s], x[i]);
-            __builtin_amdgcn_sched_barrier(0);
-            ad.EachRowStep(at, [&](int s, uint32_t byte) { v[1][s] = BlocksReadRow(byte + S::TENSOR + TILE); });
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int s = 0; s < KS; ++s) y[i] = BlocksMfma<BF16>(v[i][s], go[s], y[i]);
-        }
+            for (int i = 0; i < 2; ++i) k[i][s] = BlocksReadRow(step[s] + i * TILE);
         __builtin_amdgcn_sched_barrier(0);
-        meanwhile();   // the next stage is asked for under the products' cover
-        u32x2_t kt[DC][2];
-        ad.template EachDimension<DC>(at, [&](int d, uint32_t byte) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) kt[d][i] = BlocksReadTransposed(byte + i * TILE);
-        });
+        for (int s = 0; s < KS; ++s) v[0][s] = BlocksReadRow(step[s] + S::TENSOR);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const bool member = (mask[i] >> col.in[0]) & 1;
-            const float less = member ? -lse2 : -__builtin_inff();
-            if (start[i] + 16 > col.seen_by_all) {
-                const int limit = col.visible[0] - start[i];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[i][j] = (int)g4 + j < limit ? x[i][j] : -__builtin_inff();
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[i][j] = BlocksExp2(__builtin_fmaf(x[i][j], scale2, less));
-                y[i][j] = x[i][j] * (y[i][j] - delta);
-                off += y[i][j];
-            }
+            x[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            y[i] = less_delta;
         }
-        // one rounding of p and ds to the tensors' type, as of p in the forward
-        const u32x4_t p = BlocksPackOperand<BF16>(x[0], x[1]), ds = BlocksPackOperand<BF16>(y[0], y[1]);
 #pragma unroll
-        for (int d = 0; d < DC; ++d) {
-            const u32x4_t kk = {kt[d][0][0], kt[d][0][1], kt[d][1][0], kt[d][1][1]};
-            acc[d] = BlocksMfma<BF16>(kk, ds, acc[d]);
-            wk[d] = BlocksMfma<BF16>(kk, p, wk[d]);
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[i] = BlocksMfma<BF16>(k[i][s], q[s], x[i]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) v[1][s] = BlocksReadRow(step[s] + S::TENSOR + TILE);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) y[i] = BlocksMfma<BF16>(v[i][s], go[s], y[i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    meanwhile();   // the next stage is asked for under the products' cover
+    u32x2_t kt[DC][2];
+    {
+        uint32_t turned[DC];
+        ad.template Dimensions<DC>(at, turned);
+#pragma unroll
+        for (int d = 0; d < DC; ++d)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) kt[d][i] = BlocksReadTransposed(turned[d] + i * TILE);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int e = 0; e < NM; ++e)
+        if (start[e] + 16 * PER > col.seen_by_all) {
+            const int limit = col.visible[0] - start[e] - (int)g4;
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[e * PER + i][j] = i * 16 + j < limit ? x[e * PER + i][j] : -__builtin_inff();
         }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float less = ((mask[i / PER] >> col.in[0]) & 1) ? -lse2 : -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[i][j] = BlocksExp2(__builtin_fmaf(x[i][j], scale2, less));
+            y[i][j] *= x[i][j];
+        }
+        off += (y[i][0] + y[i][1]) + (y[i][2] + y[i][3]);
+    }
+    // one rounding of p and ds to the tensors' type, as of p in the forward
+    const u32x4_t p = BlocksPackOperand<BF16>(x[0], x[1]), ds = BlocksPackOperand<BF16>(y[0], y[1]);
+#pragma unroll
+    for (int d = 0; d < DC; ++d) {
+        const u32x4_t kk = {kt[d][0][0], kt[d][0][1], kt[d][1][0], kt[d][1][1]};
+        acc[d] = BlocksMfma<BF16>(kk, ds, acc[d]);
+        wk[d] = BlocksMfma<BF16>(kk, p, wk[d]);
     }
 }
 
-template <bool BF16, int DC>
+// ONE: a pair of tiles is of one block (blocks of a multiple of 32 rows)
+template <bool BF16, int DC, bool ONE>
 __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint32_t tpw, uint32_t mtiles, uint32_t tiles, const uint16_t* __restrict__ out,
                                                              const uint16_t* __restrict__ dout, const float* __restrict__ lse, uint16_t* __restrict__ dq,
                                                              BlocksRowInfo info) {
     TakeWholeRegisterFile();
     using S = BlocksWalkShape<DC>;
     constexpr int KS = DC / 2;
+    constexpr uint32_t NT = 2;
     extern __shared__ __attribute__((aligned(1024))) char s_walk[];
     __shared__ uint32_t s_count, s_scratch[8][64];
     const BlocksWalkTables<DC> tab(s_walk);
@@ -221,25 +235,25 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
 #pragma unroll
     for (int d = 0; d < DC; ++d) acc[d] = wk[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float off = 0.f;
+    f32x4_t less_delta = {-delta, -delta, -delta, -delta};
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[s]), "+v"(go[s]));
+    asm volatile("" : "+v"(less_delta));
     const BlocksWalker<DC> walk(a, wave, lane);
     const uint32_t lds = BlocksLdsAddress(s_walk);
 
     for (uint32_t window = 0; window < blocks; window += S::WINDOW) {
         const uint32_t in_window = min(S::WINDOW, blocks - window);
         const uint32_t units = BlocksWalkList<DC>(a, w, window, in_window, tab, &s_count) * tpb, stages = (units + 3) / 4;
-        BlocksWalkStage d[S::BUFFERS];
-#pragma unroll
-        for (uint32_t s = 0; s + 1 < S::BUFFERS; ++s)
-            if (s < stages) {
-                const BlocksWalkSource from = walk.Describe(a, w, tab, window, s, units, col.seen_by_any, d[s]);
-                walk.Load(from, lds + s * S::STAGE);
-            }
+        BlocksWalkStage now = {}, next = {};   // of the stages that are multiplied and loaded now
+        BlocksWalkSource from = {};
+        if (stages) from = walk.Describe(a, w, tab, window, 0, units, col.seen_by_any, next);
+        for (uint32_t s = 0; s + 1 < S::BUFFERS && s < stages; ++s) walk.Load(from, s, lds + s * S::STAGE);
         uint32_t buf = 0;
         for (uint32_t s = 0; s < stages; ++s) {
-            const bool more = s + S::BUFFERS - 1 < stages;
-            const BlocksWalkSource from = walk.Describe(a, w, tab, window, s + S::BUFFERS - 1, units, col.seen_by_any, d[S::BUFFERS - 1]);
+            const uint32_t ahead = s + S::BUFFERS - 1;
+            if (s % kDescribed == 0) now = next;
+            if (ahead % kDescribed == 0 && ahead < stages) from = walk.Describe(a, w, tab, window, ahead, units, col.seen_by_any, next);
             if (S::BUFFERS > 2 && s + 1 < stages)
                 BlocksDmaWait<(S::BUFFERS - 2) * S::LOADS>();
             else
@@ -247,24 +261,24 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
             BlocksStageBarrier();
             bool asked = false;
             auto load = [&]() {
-                if (more && !asked) walk.Load(from, lds + (buf == 0 ? S::BUFFERS - 1 : buf - 1) * S::STAGE);
+                if (ahead < stages && !asked) walk.Load(from, ahead, lds + (buf == 0 ? S::BUFFERS - 1 : buf - 1) * S::STAGE);
                 asked = true;
             };
 #pragma unroll 1
-            for (uint32_t z = 0; z < 4; z += 2) {
-                int start[2];
-                uint32_t mask[2];
+            for (uint32_t z = 0; z < 4; z += NT) {
+                const uint32_t first = s % kDescribed * 4 + z;
+                int start[ONE ? 1 : NT];
+                uint32_t mask[ONE ? 1 : NT], any = 0;
 #pragma unroll
-                for (uint32_t y = 0; y < 2; ++y) {
-                    start[y] = __builtin_amdgcn_readlane(d[0].start, (int)(z + y));
-                    mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)d[0].mask, (int)(z + y));
+                for (uint32_t y = 0; y < (ONE ? 1 : NT); ++y) {
+                    start[y] = __builtin_amdgcn_readlane(now.start, (int)(first + y));
+                    mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)now.mask, (int)(first + y));
+                    any |= mask[y];
                 }
-                if (mask[0] | mask[1])
-                    BlocksWalkQueryGrad<BF16, DC>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, go, lse2, delta, acc, wk, off, load);
+                if (any)
+                    BlocksWalkQueryGrad<BF16, DC>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, go, lse2, less_delta, acc, wk, off, load);
             }
             load();
-#pragma unroll
-            for (uint32_t y = 0; y + 1 < S::BUFFERS; ++y) d[y] = d[y + 1];
             buf = buf + 1 == S::BUFFERS ? 0 : buf + 1;
         }
         __syncthreads();
@@ -530,16 +544,20 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
         };
         const uint32_t by_info = lds + 2 * S::TENSOR + (rg * 32 + g * 4) * 4, by_row = lds + rg * 2 * D * 32;
         auto rows_of = [&](uint32_t stage, uint32_t tensor, u32x4_t(&f)[2][KS]) {
-            ad.EachRowStep(by_row + stage, [&](int j, uint32_t at) {
+            uint32_t step[KS];
+            ad.RowSteps(by_row + stage, step);
 #pragma unroll
-                for (int y = 0; y < 2; ++y) f[y][j] = BlocksReadRow(at + tensor + y * D * 32);
-            });
+            for (int j = 0; j < KS; ++j)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) f[y][j] = BlocksReadRow(step[j] + tensor + y * D * 32);
         };
         auto turned_of = [&](uint32_t stage, uint32_t tensor, u32x2_t(&f)[OD][2]) {
-            ad.template EachDimension<OD>(by_row + stage, [&](int d, uint32_t at) {
+            uint32_t turned[OD];
+            ad.template Dimensions<OD>(by_row + stage, turned);
 #pragma unroll
-                for (int y = 0; y < 2; ++y) f[d][y] = BlocksReadTransposed(at + tensor + y * D * 32);
-            });
+            for (int d = 0; d < OD; ++d)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) f[d][y] = BlocksReadTransposed(turned[d] + tensor + y * D * 32);
         };
         auto product = [&](const u32x4_t(&f)[2][KS], const u32x4_t(&keys)[KS], f32x4_t(&x)[2]) {
 #pragma unroll
@@ -766,7 +784,8 @@ gpann_status Backward(const BlocksArgs& a, const uint16_t* out, const float* lse
     if (a.Tq > 0) {
         const uint32_t mtiles = (a.G + 15) / 16, tpw = std::max(1u, 16 / a.G);
         const uint64_t waves = mtiles > 1 ? (uint64_t)a.Tq * mtiles : (a.Tq + tpw - 1) / tpw, tiles = (waves + 7) / 8;
-        GPANN_TRY(BlocksLaunch(BlocksQueryGradKernel<BF16, DC>, BlocksPairGrid(pairs, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, dout, lse,
+        auto kernel = a.bs % 32 == 0 ? BlocksQueryGradKernel<BF16, DC, true> : BlocksQueryGradKernel<BF16, DC, false>;
+        GPANN_TRY(BlocksLaunch(kernel, BlocksPairGrid(pairs, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, dout, lse,
                                dq, info));
     }
     if (a.Tk == 0) return GPANN_OK;

@@ -82,6 +82,8 @@ __device__ __forceinline__ u32x4_t BlocksColumn(const uint32_t (&w)[8][N], int d
 }
 
 __device__ __forceinline__ float BlocksExp2(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32: 1 ulp, -inf -> 0
+__device__ __forceinline__ float BlocksMaxOf4(const f32x4_t& x) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); }
+__device__ __forceinline__ float BlocksMaxOf4(const f32x4_t& x, float y) { return fmaxf(fmaxf(fmaxf(fmaxf(y, x[0]), x[1]), x[2]), x[3]); }
 // over the four lanes that hold a C column: v_permlane32_swap / v_permlane16_swap of a register with itself put a lane's value and that of lane ^ 32 (^ 16)
 // side by side, without the trip through LDS of a shuffle
 __device__ __forceinline__ float BlocksMaxOver4(float x) {

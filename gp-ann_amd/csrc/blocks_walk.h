@@ -177,12 +177,12 @@ __device__ __forceinline__ uint32_t BlocksWalkList(const BlocksArgs& a, const Bl
     return *s_count;
 }
 
-// The four 16-row tiles of a stage, tile y in lane y: for the loads ...
+// What a stage's loads and products have to know of its four 16-row tiles, for sixteen stages at a time: tile y of stage s in lane 4 (s % 16) + y
+constexpr uint32_t kDescribed = 16;
 struct BlocksWalkSource {
-    uint4 address;     // of its block
-    int row, last;     // its first row in the block; the last row of the block that the sequence has
+    uint2 k, v;        // addresses of its first row
+    int last;          // its last row that the sequence has, in the tile
 };
-// ... and for the products
 struct BlocksWalkStage {
     int start;         // its position
     uint32_t mask;     // which query rows of this wavefront look at it
@@ -192,46 +192,51 @@ struct BlocksWalkStage {
 template <int DC>
 struct BlocksWalker {
     using S = BlocksWalkShape<DC>;
-    // row in its tile and byte offset of the chunk in the row: all of a wavefront's instructions of a stage have the same where a row is a power of two
-    static constexpr uint32_t PLACES = (S::CPR & (S::CPR - 1)) == 0 ? 1 : S::LOADS;
-    uint32_t row[PLACES], chunk[PLACES];
+    // byte offsets in a tile: all of a wavefront's instructions of a stage have the same two where a row is a power of two of chunks, of keys and of values
+    static constexpr bool POWER = (S::CPR & (S::CPR - 1)) == 0;
+    static constexpr uint32_t PLACES = POWER ? 2 : S::LOADS;
+    uint32_t place[PLACES];
     uint32_t wave, lane, tpb, inverse, krow, vrow;
     __device__ __forceinline__ BlocksWalker(const BlocksArgs& a, uint32_t wave_, uint32_t lane_) : wave(wave_), lane(lane_), tpb(a.bs / 16) {
         inverse = tpb > 1 ? 0xFFFFFFFFu / tpb + 1 : 0;
         krow = (uint32_t)a.ks[1] * 2;
         vrow = (uint32_t)a.vs[1] * 2;
 #pragma unroll
-        for (uint32_t x = 0; x < PLACES; ++x) {
-            const uint32_t at = (wave + 8 * x) % S::CPR * 64 + lane, r = at / S::CPR;
-            row[x] = r % 16;
-            chunk[x] = S::Chunk(at % S::CPR, r) * 16;
-        }
+        for (uint32_t x = 0; x < PLACES; ++x) place[x] = Place(POWER ? 0 : x, POWER ? x == 1 : wave + 8 * x >= S::CPR, 15);
     }
-    // `seen`: rows that the last query row of this wavefront sees (a prefix)
+    __device__ __forceinline__ uint32_t Place(uint32_t x, bool value, int last) const {
+        const uint32_t at = (wave + 8 * x) % S::CPR * 64 + lane, r = at / S::CPR % 16;
+        return (uint32_t)min((int)r, last) * (value ? vrow : krow) + S::Chunk(at % S::CPR, r) * 16;
+    }
+    // of the stages from s on; `seen`: rows that the last query row of this wavefront sees (a prefix)
     __device__ __forceinline__ BlocksWalkSource Describe(const BlocksArgs& a, const BlocksWalkRows& w, const BlocksWalkTables<DC>& tab, uint32_t window, uint32_t s,
                                                          uint32_t units, int seen, BlocksWalkStage& st) const {
         BlocksWalkSource d;
-        const uint32_t unit = 4 * s + (lane & 3), in = min(unit, units - 1), e = inverse ? __umulhi(in, inverse) : in;   // in / tpb, exact below 2^16
-        const int block = tab.list[e];
-        d.address = tab.address[e];
-        d.row = (int)(in - e * tpb) * 16;
-        d.last = w.n - 1 - block * (int)a.bs;
-        st.start = block * (int)a.bs + d.row;
+        const uint32_t unit = 4 * s + lane, in = min(unit, units - 1), e = inverse ? __umulhi(in, inverse) : in;   // in / tpb, exact below 2^16
+        const int block = tab.list[e], row = (int)(in - e * tpb) * 16, last = w.n - 1 - block * (int)a.bs;
+        const uint32_t first = (uint32_t)min(row, last & ~15);   // a tile behind the sequence's end: its last one's rows (nobody looks at them)
+        const uint4 base = tab.address[e];
+        const uint64_t k = (((uint64_t)base.y << 32) | base.x) + (uint64_t)first * krow, v = (((uint64_t)base.w << 32) | base.z) + (uint64_t)first * vrow;
+        d.k = uint2{(uint32_t)k, (uint32_t)(k >> 32)};
+        d.v = uint2{(uint32_t)v, (uint32_t)(v >> 32)};
+        d.last = min(15, last - (int)first);
+        st.start = block * (int)a.bs + row;
         st.mask = tab.masks[(block - (int)window) * 8 + (int)wave];
         if (unit >= units || st.start >= seen) st.mask = 0;
         return d;
     }
-    __device__ __forceinline__ void Load(const BlocksWalkSource& d, uint32_t to) const {
+    __device__ __forceinline__ void Load(const BlocksWalkSource& d, uint32_t s, uint32_t to) const {
 #pragma unroll
         for (uint32_t x = 0; x < S::LOADS; ++x) {
             const uint32_t j = wave + 8 * x;
-            const bool value = j >= S::CPR;
-            const int tile = (int)(j % S::CPR / (S::CPR / 4));   // 16 rows are CPR / 4 instructions
-            const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(value ? d.address.z : d.address.x), tile);
-            const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(value ? d.address.w : d.address.y), tile);
-            const int first = __builtin_amdgcn_readlane(d.row, tile), last = __builtin_amdgcn_readlane(d.last, tile);
-            const uint32_t place = PLACES == 1 ? 0 : x, r = (uint32_t)min(first + (int)row[place], last);   // rows past the sequence's end are not read
-            BlocksDma(((uint64_t)hi << 32) | lo, r * (value ? vrow : krow) + chunk[place], to + (value ? S::TENSOR : 0) + j % S::CPR * 1024);
+            const bool value = POWER ? x >= S::CPR / 8 : j >= S::CPR;
+            const int tile = (int)(s % kDescribed * 4 + j % S::CPR / (S::CPR / 4));   // 16 rows are CPR / 4 instructions
+            const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(value ? d.v.x : d.k.x), tile);
+            const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(value ? d.v.y : d.k.y), tile);
+            const int last = __builtin_amdgcn_readlane(d.last, tile);
+            uint32_t offset = place[POWER ? (value ? 1 : 0) : x];
+            if (last < 15) offset = Place(x, value, last);   // rows past the sequence's end are not read
+            BlocksDma(((uint64_t)hi << 32) | lo, offset, to + (value ? S::TENSOR : 0) + j % S::CPR * 1024);
         }
     }
 };
@@ -251,26 +256,25 @@ struct BlocksWalkAddresses {
 #pragma unroll
         for (uint32_t d = 0; d < (POWER ? 1 : DC); ++d) turned[d] = (row * S::CPR + S::Slot((first + d) * 2 + (r & 3) / 2, row)) * 16 + (r & 1) * 8;
     }
-    // by rows: step s of row lane % 16 of the tile at LDS byte `at`; f(address of step s)
-    template <typename F>
-    __device__ __forceinline__ void EachRowStep(uint32_t at, F&& f) const {
-        const uint32_t base = at + rows[0];
+    // by rows: step s of row lane % 16 of the tile at LDS byte `at`
+    __device__ __forceinline__ void RowSteps(uint32_t at, uint32_t (&x)[DC / 2]) const {
+        uint32_t base = at + rows[0];
+        asm volatile("" : "+v"(base));   // (else the constant offsets that follow would be added on the vector unit, one by one)
 #pragma unroll
         for (int s = 0; s < DC / 2; ++s) {
-            uint32_t x = POWER ? base ^ (64 * s) : at + rows[POWER ? 0 : s];
-            asm volatile("" : "+v"(x));   // (else the constant offsets that follow would be added on the vector unit, one by one)
-            f(s, x);
+            x[s] = s == 0 ? base : POWER ? base ^ (64 * s) : at + rows[POWER ? 0 : s];
+            if (s > 0) asm volatile("" : "+v"(x[s]));
         }
     }
     // transposed: 16 dimensions of rows 4 g .. of the tile at LDS byte `at`; a power of two of dimension tiles, or all that are left
-    template <int COUNT, typename F>
-    __device__ __forceinline__ void EachDimension(uint32_t at, F&& f) const {
-        const uint32_t base = at + turned[0];
+    template <int COUNT>
+    __device__ __forceinline__ void Dimensions(uint32_t at, uint32_t (&x)[COUNT]) const {
+        uint32_t base = at + turned[0];
+        asm volatile("" : "+v"(base));
 #pragma unroll
         for (int d = 0; d < COUNT; ++d) {
-            uint32_t x = POWER ? base ^ (32 * d) : at + turned[POWER ? 0 : d];
-            asm volatile("" : "+v"(x));
-            f(d, x);
+            x[d] = d == 0 ? base : POWER ? base ^ (32 * d) : at + turned[POWER ? 0 : d];
+            if (d > 0) asm volatile("" : "+v"(x[d]));
         }
     }
 };

@@ -57,7 +57,7 @@ enum { /* calls a workspace is meant for (gpann_blocks_workspace_bytes) */
 
 /* The tensors of a call: q, out, dout, dq are [batch][q_rows][q_heads][head_dim]; k, v, dk, dv are [batch][kv_rows][kv_heads][head_dim] or, with a
  * page table, [n_pages][block_rows][kv_heads][head_dim] — a block is a page.  Strides are in elements, {batch or page, row, head}, the last dimension is
- * contiguous; a gradient has the strides of its tensor and dout those of out.  Strides have to be multiples of 8 (a row's at most 2^22) and tensors 16-byte aligned; a tensor
+ * contiguous; a gradient has the strides of its tensor and dout those of out.  Strides have to be multiples of 8 (at most 2^22 for a row, 2^31 for a head) and tensors 16-byte aligned; a tensor
  * that is written must not overlap itself. */
 typedef struct gpann_blocks_layout {
     uint32_t struct_bytes;        /* sizeof(gpann_blocks_layout) of the caller's header */
