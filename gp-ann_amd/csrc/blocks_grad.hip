@@ -103,95 +103,118 @@ __device__ __forceinline__ void BlocksQueryGradRow(const BlocksArgs& a, uint32_t
     }
 }
 
-// two tiles of 16 keys, the first at LDS byte `at`, against a wavefront's 16 columns; `less_delta`: minus the column's delta, four times over
-template <bool BF16, int DC, int NM, typename F>
+// NT tiles of 16 keys, the first at LDS byte `at`, against a wavefront's 16 columns, in pairs: a pair's logits are on the matrix cores while the weights of the one
+// before are computed, and its part of the sums while those of the one behind are.  `less_delta`: minus the column's delta, four times over.
+template <bool BF16, int DC, int NT, int NM, typename F>
 __device__ __forceinline__ void BlocksWalkQueryGrad(float scale2, const BlocksWalkAddresses<DC>& ad, uint32_t at, const int (&start)[NM], const uint32_t (&mask)[NM],
                                                     const BlocksWalkColumns<1>& col, uint32_t g4, const u32x4_t (&q)[DC / 2], const u32x4_t (&go)[DC / 2], float lse2,
                                                     const f32x4_t& less_delta, f32x4_t (&acc)[DC], f32x4_t (&wk)[DC], float& off, F&& meanwhile) {
     using S = BlocksWalkShape<DC>;
     constexpr uint32_t TILE = S::D * 32;
-    constexpr int KS = DC / 2, PER = 2 / NM;
-    f32x4_t x[2], y[2];
-    {
-        uint32_t step[KS];
-        u32x4_t k[2][KS], v[2][KS];
-        ad.RowSteps(at, step);
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) k[i][s] = BlocksReadRow(step[s] + i * TILE);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) v[0][s] = BlocksReadRow(step[s] + S::TENSOR);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            x[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            y[i] = less_delta;
-        }
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) x[i] = BlocksMfma<BF16>(k[i][s], q[s], x[i]);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) v[1][s] = BlocksReadRow(step[s] + S::TENSOR + TILE);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int s = 0; s < KS; ++s) y[i] = BlocksMfma<BF16>(v[i][s], go[s], y[i]);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    meanwhile();   // the next stage is asked for under the products' cover
+    constexpr int KS = DC / 2, NP = NT / 2, PER = NT / NM;
+    f32x4_t x[NT], y[NT];
+    u32x4_t k[2][KS], v[2][KS], p, ds;
     u32x2_t kt[DC][2];
-    {
-        uint32_t turned[DC];
-        ad.template Dimensions<DC>(at, turned);
+    uint32_t step[KS], turned[DC];
+    auto read_rows = [&](int z, u32x4_t(&f)[2][KS], uint32_t tensor) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) f[i][s] = BlocksReadRow(step[s] + tensor + (2 * z + i) * TILE);
+    };
+    auto read_turned = [&](int z) {
 #pragma unroll
         for (int d = 0; d < DC; ++d)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) kt[d][i] = BlocksReadTransposed(turned[d] + i * TILE);
-    }
+            for (int i = 0; i < 2; ++i) kt[d][i] = BlocksReadTransposed(turned[d] + (2 * z + i) * TILE);
+    };
+    auto logits = [&](int z) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[2 * z + i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            y[2 * z + i] = less_delta;
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[2 * z + i] = BlocksMfma<BF16>(k[i][s], q[s], x[2 * z + i]);
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) y[2 * z + i] = BlocksMfma<BF16>(v[i][s], go[s], y[2 * z + i]);
+    };
+    auto sums = [&]() {
+#pragma unroll
+        for (int d = 0; d < DC; ++d) {
+            const u32x4_t kk = {kt[d][0][0], kt[d][0][1], kt[d][1][0], kt[d][1][1]};
+            acc[d] = BlocksMfma<BF16>(kk, ds, acc[d]);
+            wk[d] = BlocksMfma<BF16>(kk, p, wk[d]);
+        }
+    };
+    ad.RowSteps(at, step);
+    read_rows(0, k, 0);
     __builtin_amdgcn_sched_barrier(0);
+    read_rows(0, v, S::TENSOR);
+    ad.template Dimensions<DC>(at, turned);
+    __builtin_amdgcn_sched_barrier(0);
+    logits(0);
+    __builtin_amdgcn_sched_barrier(0);
+    meanwhile();   // the next stage is asked for under the products' cover
+    if (NP == 1) read_turned(0);
 #pragma unroll
-    for (int e = 0; e < NM; ++e)
-        if (start[e] + 16 * PER > col.seen_by_all) {
-            const int limit = col.visible[0] - start[e] - (int)g4;
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[e * PER + i][j] = i * 16 + j < limit ? x[e * PER + i][j] : -__builtin_inff();
+    for (int z = 0; z < NP; ++z) {
+        if (z + 1 < NP) {
+            read_rows(z + 1, k, 0);
+            read_rows(z + 1, v, S::TENSOR);
         }
+        if (z > 0) read_turned(z - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        float less[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float less = ((mask[i / PER] >> col.in[0]) & 1) ? -lse2 : -__builtin_inff();
+        for (int i = 0; i < 2; ++i) {
+            const int e = (2 * z + i) / PER;
+            if (i == 0 || PER == 1) {
+                if (start[e] + (PER == 1 ? 16 : 32) + (PER == 4 ? 32 * z : 0) > col.seen_by_all) {
+                    const int limit = col.visible[0] - start[e] - (PER == 4 ? 32 * z : 0) - (int)g4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x[i][j] = BlocksExp2(__builtin_fmaf(x[i][j], scale2, less));
-            y[i][j] *= x[i][j];
+                    for (int j = 0; j < (PER == 1 ? 4 : 8); ++j)
+                        x[2 * z + i + j / 4][j % 4] = (j / 4) * 16 + j % 4 < limit ? x[2 * z + i + j / 4][j % 4] : -__builtin_inff();
+                }
+            }
+            less[i] = ((mask[e] >> col.in[0]) & 1) ? -lse2 : -__builtin_inff();
         }
-        off += (y[i][0] + y[i][1]) + (y[i][2] + y[i][3]);
-    }
-    // one rounding of p and ds to the tensors' type, as of p in the forward
-    const u32x4_t p = BlocksPackOperand<BF16>(x[0], x[1]), ds = BlocksPackOperand<BF16>(y[0], y[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (z > 0) sums();
+        if (z + 1 < NP) logits(z + 1);
 #pragma unroll
-    for (int d = 0; d < DC; ++d) {
-        const u32x4_t kk = {kt[d][0][0], kt[d][0][1], kt[d][1][0], kt[d][1][1]};
-        acc[d] = BlocksMfma<BF16>(kk, ds, acc[d]);
-        wk[d] = BlocksMfma<BF16>(kk, p, wk[d]);
+        for (int i = 2 * z; i < 2 * z + 2; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[i][j] = BlocksExp2(__builtin_fmaf(x[i][j], scale2, less[i - 2 * z]));
+                y[i][j] *= x[i][j];
+            }
+            off += (y[i][0] + y[i][1]) + (y[i][2] + y[i][3]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // one rounding of p and ds to the tensors' type, as of p in the forward
+        p = BlocksPackOperand<BF16>(x[2 * z], x[2 * z + 1]);
+        ds = BlocksPackOperand<BF16>(y[2 * z], y[2 * z + 1]);
     }
+    if (NP > 1) {
+        read_turned(NP - 1);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    sums();
 }
 
-// ONE: a pair of tiles is of one block (blocks of a multiple of 32 rows)
-template <bool BF16, int DC, bool ONE>
+// NT: tiles taken at a time, 4 where a block is a multiple of them; ONE: they are of one block
+template <bool BF16, int DC, uint32_t NT, bool ONE>
 __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint32_t tpw, uint32_t mtiles, uint32_t tiles, const uint16_t* __restrict__ out,
                                                              const uint16_t* __restrict__ dout, const float* __restrict__ lse, uint16_t* __restrict__ dq,
                                                              BlocksRowInfo info) {
     TakeWholeRegisterFile();
     using S = BlocksWalkShape<DC>;
     constexpr int KS = DC / 2;
-    constexpr uint32_t NT = 2;
     extern __shared__ __attribute__((aligned(1024))) char s_walk[];
     __shared__ uint32_t s_count, s_scratch[8][64];
     const BlocksWalkTables<DC> tab(s_walk);
@@ -276,7 +299,7 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
                     any |= mask[y];
                 }
                 if (any)
-                    BlocksWalkQueryGrad<BF16, DC>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, go, lse2, less_delta, acc, wk, off, load);
+                    BlocksWalkQueryGrad<BF16, DC, NT>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, go, lse2, less_delta, acc, wk, off, load);
             }
             load();
             buf = buf + 1 == S::BUFFERS ? 0 : buf + 1;
@@ -506,7 +529,7 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
         for (uint32_t y = 0; y < PIECES; ++y) {
             const uint32_t at = (wave + 8 * y) * 64 + lane;
             piece_row[y] = at / S::CPR;
-            place[y] = W::Chunk(at % S::CPR, piece_row[y] % 16) * 16;
+            place[y] = W::Slot(at % S::CPR, piece_row[y] % 16) * 16;
         }
         auto row_of = [&](uint32_t i, uint32_t& t, uint32_t& head) {
             const uint32_t in = inverse ? __umulhi(i, inverse) : i;   // i / G, exact below 2^16
@@ -784,7 +807,9 @@ gpann_status Backward(const BlocksArgs& a, const uint16_t* out, const float* lse
     if (a.Tq > 0) {
         const uint32_t mtiles = (a.G + 15) / 16, tpw = std::max(1u, 16 / a.G);
         const uint64_t waves = mtiles > 1 ? (uint64_t)a.Tq * mtiles : (a.Tq + tpw - 1) / tpw, tiles = (waves + 7) / 8;
-        auto kernel = a.bs % 32 == 0 ? BlocksQueryGradKernel<BF16, DC, true> : BlocksQueryGradKernel<BF16, DC, false>;
+        auto kernel = a.bs % 32 == 0 ? BlocksQueryGradKernel<BF16, DC, 2, true> : BlocksQueryGradKernel<BF16, DC, 2, false>;
+        if constexpr (DC <= 8)
+            if (a.bs % 64 == 0) kernel = BlocksQueryGradKernel<BF16, DC, 4, true>;
         GPANN_TRY(BlocksLaunch(kernel, BlocksPairGrid(pairs, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, dout, lse,
                                dq, info));
     }

@@ -6,8 +6,7 @@
 // so the union is far smaller than the sum; a 16-column tile costs the same whether one or all of its rows want the block.
 //
 // Rows go to LDS by DMA (no registers, issued stages ahead), 64 rows of K and of V a stage.  The 16-byte chunks of a row are permuted by a function of the
-// row such that both ways of reading are free of bank conflicts: by rows (ds_read_b128: eight rows, one chunk) and transposed (ds_read_b64_tr_b16: four
-// rows, two neighbouring chunks per 16 lanes).
+// row such that both ways of reading are free of bank conflicts: by rows (ds_read_b128) and transposed (ds_read_b64_tr_b16).
 #pragma once
 
 #include "blocks_tile.h"
@@ -21,23 +20,17 @@ struct BlocksWalkShape {
     static constexpr uint32_t WINDOW = D <= 128 ? 1024 : 512;   // blocks that LDS has room for at a time
     static constexpr size_t LDS = (size_t)BUFFERS * STAGE + WINDOW * (sizeof(uint4) + 32 + 4);
 
-    // Slot of a row's chunk.  LDS serves 256 bytes a cycle over 64 banks, so sixteen lanes' chunks (by rows: sixteen rows, one chunk) and thirty-two lanes'
-    // half chunks (transposed: eight rows, two neighbouring chunks) have to lie in sixteen different slots modulo 16; a row begins CPR slots after the one before.
+    // Slot of a row's chunk: an exclusive or with a function of the row.  LDS serves 256 bytes a cycle, so the lanes that it serves together have to lie in
+    // sixteen different slots modulo 16, and a row begins CPR slots after the one before.  Read by rows, lanes {0-3, 12-15, 20-27}, {4-11, 16-19, 28-31} and the
+    // same of the upper half go together: eight rows' chunk c and the eight others' chunk c + 1.  Transposed, half a wavefront goes together: eight rows'
+    // chunks c and c + 1.  So the rows of each eight get different pairs of slots, and two rows that share a pair are both of the eight rows of one kind, with
+    // different slots, or of different kinds, with the same one.
+    static constexpr uint32_t TURNS = CPR % 16 == 0 ? 16 : CPR % 8 == 0 ? 8 : 4;
     static __device__ __forceinline__ uint32_t Turn(uint32_t row) {
-        if (CPR == 12) return ((row >> 2) & 1) * 2 + ((row >> 3) & 1);
-        if (CPR % 16 == 8) return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
-        return ((row & 7) << 1) | ((row >> 3) & 1);
+        const uint32_t eighth = (row >> 3) & 1;
+        return (((row / (16 / TURNS)) & (TURNS / 2 - 1)) ^ (eighth * (TURNS / 4))) << 1 | eighth;
     }
-    static __device__ __forceinline__ uint32_t Slot(uint32_t chunk, uint32_t row) {
-        if ((CPR & (CPR - 1)) == 0) return chunk ^ Turn(row);
-        const uint32_t s = chunk + Turn(row);
-        return s >= CPR ? s - CPR : s;
-    }
-    static __device__ __forceinline__ uint32_t Chunk(uint32_t slot, uint32_t row) {
-        if ((CPR & (CPR - 1)) == 0) return slot ^ Turn(row);
-        const uint32_t t = Turn(row);
-        return slot >= t ? slot - t : slot + CPR - t;
-    }
+    static __device__ __forceinline__ uint32_t Slot(uint32_t chunk, uint32_t row) { return chunk ^ Turn(row); }   // and the chunk of a slot
 };
 
 // One LDS-DMA wave-instruction: 64 lanes x 16 bytes from base + offset to LDS bytes [lds, lds + 1024).  The compiler neither sees the bytes nor counts
@@ -206,7 +199,7 @@ struct BlocksWalker {
     }
     __device__ __forceinline__ uint32_t Place(uint32_t x, bool value, int last) const {
         const uint32_t at = (wave + 8 * x) % S::CPR * 64 + lane, r = at / S::CPR % 16;
-        return (uint32_t)min((int)r, last) * (value ? vrow : krow) + S::Chunk(at % S::CPR, r) * 16;
+        return (uint32_t)min((int)r, last) * (value ? vrow : krow) + S::Slot(at % S::CPR, r) * 16;
     }
     // of the stages from s on; `seen`: rows that the last query row of this wavefront sees (a prefix)
     __device__ __forceinline__ BlocksWalkSource Describe(const BlocksArgs& a, const BlocksWalkRows& w, const BlocksWalkTables<DC>& tab, uint32_t window, uint32_t s,
@@ -241,40 +234,49 @@ struct BlocksWalker {
     }
 };
 
-// LDS addresses of a lane's part of a stage's operands.  Where a row is a power of two of chunks, a permuted chunk is an exclusive or, so step s and dimension
-// tile d are one exclusive or away from a base (stages begin at multiples of 1024 bytes): two registers instead of one for every step and tile.
+// LDS addresses of a lane's part of a stage's operands.  A permuted chunk is an exclusive or in the low bits, so step s and dimension tile d are one exclusive
+// or and one constant away from a base (stages begin at multiples of 1024 bytes): two registers instead of one for every step and tile.
 template <int DC>
 struct BlocksWalkAddresses {
     using S = BlocksWalkShape<DC>;
-    static constexpr bool POWER = (S::CPR & (S::CPR - 1)) == 0;
-    uint32_t rows[POWER ? 1 : DC / 2], turned[POWER ? 1 : DC];
-    // `first`: the first of the dimension tiles that this lane's wavefront reads transposed
-    __device__ __forceinline__ explicit BlocksWalkAddresses(uint32_t lane, uint32_t first = 0) {
+    uint32_t rows, turned, first;
+    // `first_`: the first of the dimension tiles that this lane's wavefront reads transposed
+    __device__ __forceinline__ explicit BlocksWalkAddresses(uint32_t lane, uint32_t first_ = 0) : first(first_) {
         const uint32_t r = lane & 15, g = lane >> 4, row = g * 4 + r / 4;
-#pragma unroll
-        for (uint32_t s = 0; s < (POWER ? 1 : DC / 2); ++s) rows[s] = (r * S::CPR + S::Slot(s * 4 + g, r)) * 16;
-#pragma unroll
-        for (uint32_t d = 0; d < (POWER ? 1 : DC); ++d) turned[d] = (row * S::CPR + S::Slot((first + d) * 2 + (r & 3) / 2, row)) * 16 + (r & 1) * 8;
+        rows = (r * S::CPR + S::Slot(g, r)) * 16;
+        turned = (row * S::CPR + S::Slot((r & 3) / 2, row)) * 16 + (r & 1) * 8;
     }
     // by rows: step s of row lane % 16 of the tile at LDS byte `at`
     __device__ __forceinline__ void RowSteps(uint32_t at, uint32_t (&x)[DC / 2]) const {
-        uint32_t base = at + rows[0];
-        asm volatile("" : "+v"(base));   // (else the constant offsets that follow would be added on the vector unit, one by one)
+        constexpr int N = S::TURNS / 4;
+        uint32_t turn[N];
 #pragma unroll
-        for (int s = 0; s < DC / 2; ++s) {
-            x[s] = s == 0 ? base : POWER ? base ^ (64 * s) : at + rows[POWER ? 0 : s];
-            if (s > 0) asm volatile("" : "+v"(x[s]));
+        for (int s = 0; s < N; ++s) {
+            turn[s] = s == 0 ? at + rows : turn[0] ^ (64 * s);
+            asm volatile("" : "+v"(turn[s]));   // (else the constant offsets that follow would be added on the vector unit, one by one)
         }
+#pragma unroll
+        for (int s = 0; s < DC / 2; ++s) x[s] = turn[s % N] + s / N * N * 64;
     }
-    // transposed: 16 dimensions of rows 4 g .. of the tile at LDS byte `at`; a power of two of dimension tiles, or all that are left
+    // transposed: 16 dimensions of rows 4 g .. of the tile at LDS byte `at`
     template <int COUNT>
     __device__ __forceinline__ void Dimensions(uint32_t at, uint32_t (&x)[COUNT]) const {
-        uint32_t base = at + turned[0];
-        asm volatile("" : "+v"(base));
+        constexpr int N = S::TURNS / 2;
+        if constexpr (COUNT == DC || COUNT % N == 0 || N % COUNT == 0) {   // `first` is a multiple of COUNT: its bits are not d's
+            uint32_t turn[COUNT < N ? COUNT : N];
 #pragma unroll
-        for (int d = 0; d < COUNT; ++d) {
-            x[d] = d == 0 ? base : POWER ? base ^ (32 * d) : at + turned[POWER ? 0 : d];
-            if (d > 0) asm volatile("" : "+v"(x[d]));
+            for (int d = 0; d < (COUNT < N ? COUNT : N); ++d) {
+                turn[d] = d == 0 ? (at + turned + first / N * N * 32) ^ (first % N * 32) : turn[0] ^ (32 * d);
+                asm volatile("" : "+v"(turn[d]));
+            }
+#pragma unroll
+            for (int d = 0; d < COUNT; ++d) x[d] = turn[d % N] + d / N * N * 32;
+        } else {
+#pragma unroll
+            for (int d = 0; d < COUNT; ++d) {
+                x[d] = ((at + turned) ^ ((first + d) % N * 32)) + (first + d) / N * N * 32;
+                asm volatile("" : "+v"(x[d]));
+            }
         }
     }
 };
