@@ -207,6 +207,75 @@ __device__ __forceinline__ void BlocksWalkQueryGrad(float scale2, const BlocksWa
     sums();
 }
 
+// ... where the sums and the operands of a row leave too few registers for that: one pair of tiles, operands in batches
+template <bool BF16, int DC, int NM, typename F>
+__device__ __forceinline__ void BlocksWalkQueryGradTight(float scale2, const BlocksWalkAddresses<DC>& ad, uint32_t at, const int (&start)[NM], const uint32_t (&mask)[NM],
+                                                         const BlocksWalkColumns<1>& col, uint32_t g4, const u32x4_t (&q)[DC / 2], const u32x4_t (&go)[DC / 2],
+                                                         float lse2, float delta, f32x4_t (&acc)[DC], f32x4_t (&wk)[DC], float& off, F&& meanwhile) {
+    using S = BlocksWalkShape<DC>;
+    constexpr uint32_t TILE = S::D * 32;
+    constexpr int KS = DC / 2, SOME = DC > 12 ? KS / 4 : KS / 2, TURNED = DC > 12 ? 2 : 4;
+    f32x4_t x[2], y[2];
+    meanwhile();
+    auto product = [&](uint32_t tensor, const u32x4_t(&with)[KS], f32x4_t(&to)[2]) {
+        uint32_t step[KS];
+        ad.RowSteps(at, step);
+#pragma unroll
+        for (int s0 = 0; s0 < KS; s0 += SOME) {
+            u32x4_t f[2][SOME];
+#pragma unroll
+            for (int s = 0; s < SOME; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) f[i][s] = BlocksReadRow(step[s0 + s] + tensor + i * TILE);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int s = 0; s < SOME; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) to[i] = BlocksMfma<BF16>(f[i][s], with[s0 + s], to[i]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = y[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    product(0, q, x);
+    product(S::TENSOR, go, y);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int first = start[i * NM / 2] + (NM == 1 ? i * 16 : 0);
+        if (first + 16 > col.seen_by_all) {
+            const int limit = col.visible[0] - first - (int)g4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i][j] = j < limit ? x[i][j] : -__builtin_inff();
+        }
+        const float less = ((mask[i * NM / 2] >> col.in[0]) & 1) ? -lse2 : -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[i][j] = BlocksExp2(__builtin_fmaf(x[i][j], scale2, less));
+            y[i][j] = x[i][j] * (y[i][j] - delta);
+        }
+        off += (y[i][0] + y[i][1]) + (y[i][2] + y[i][3]);
+    }
+    const u32x4_t p = BlocksPackOperand<BF16>(x[0], x[1]), ds = BlocksPackOperand<BF16>(y[0], y[1]);   // rounded as above
+    uint32_t turned[DC];
+    ad.template Dimensions<DC>(at, turned);
+#pragma unroll
+    for (int d0 = 0; d0 < DC; d0 += TURNED) {
+        u32x2_t kt[TURNED][2];
+#pragma unroll
+        for (int d = 0; d < TURNED; ++d)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) kt[d][i] = BlocksReadTransposed(turned[d0 + d] + i * TILE);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < TURNED; ++d) {
+            const u32x4_t kk = {kt[d][0][0], kt[d][0][1], kt[d][1][0], kt[d][1][1]};
+            acc[d0 + d] = BlocksMfma<BF16>(kk, ds, acc[d0 + d]);
+            wk[d0 + d] = BlocksMfma<BF16>(kk, p, wk[d0 + d]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 // NT: tiles taken at a time, 4 where a block is a multiple of them; ONE: they are of one block
 template <bool BF16, int DC, uint32_t NT, bool ONE>
 __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint32_t tpw, uint32_t mtiles, uint32_t tiles, const uint16_t* __restrict__ out,
@@ -258,10 +327,10 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
 #pragma unroll
     for (int d = 0; d < DC; ++d) acc[d] = wk[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float off = 0.f;
-    f32x4_t less_delta = {-delta, -delta, -delta, -delta};
+    f32x4_t less_delta = {-delta, -delta, -delta, -delta};   // (where the products start from it)
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[s]), "+v"(go[s]));
-    asm volatile("" : "+v"(less_delta));
+    if (DC <= 8) asm volatile("" : "+v"(less_delta));
     const BlocksWalker<DC> walk(a, wave, lane);
     const uint32_t lds = BlocksLdsAddress(s_walk);
 
@@ -298,8 +367,12 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
                     mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)now.mask, (int)(first + y));
                     any |= mask[y];
                 }
-                if (any)
-                    BlocksWalkQueryGrad<BF16, DC, NT>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, go, lse2, less_delta, acc, wk, off, load);
+                if (any) {
+                    if constexpr (DC > 8)
+                        BlocksWalkQueryGradTight<BF16, DC>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, go, lse2, delta, acc, wk, off, load);
+                    else
+                        BlocksWalkQueryGrad<BF16, DC, NT>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, go, lse2, less_delta, acc, wk, off, load);
+                }
             }
             load();
             buf = buf + 1 == S::BUFFERS ? 0 : buf + 1;
@@ -447,6 +520,7 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
     using W = BlocksWalkShape<DC>;
     using S = BlocksKeyShape<DC, RGS>;
     constexpr int KS = DC / 2, D = DC * 16, OD = DC / ND;
+    constexpr bool TIGHT = DC > 8;   // too few registers for operands of two products at a time: every one is read right before its use
     extern __shared__ __attribute__((aligned(1024))) char s_keys[];   // stages {Q rows, dO rows, lse2, delta}; afterwards the sums of the row groups; the row list behind
     uint32_t* s_list = reinterpret_cast<uint32_t*>(s_keys + S::BUFFERS * S::STAGE);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -629,9 +703,9 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
                 for (int i = 0; i < 4; ++i) about[i >> 1][i & 1] = BlocksReadRow(at + (i >> 1) * 256 + (i & 1) * 64);
             }
             __builtin_amdgcn_sched_barrier(0);
-            add_keys();
+            if constexpr (!TIGHT) add_keys();
             __builtin_amdgcn_sched_barrier(0);
-            rows_of(next, S::TENSOR, f1);
+            if constexpr (!TIGHT) rows_of(next, S::TENSOR, f1);
             __builtin_amdgcn_sched_barrier(0);
             if (more) load_rows(s + 3, 0, to);
             __builtin_amdgcn_sched_barrier(0);
@@ -656,29 +730,39 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
                     }
             }
             __builtin_amdgcn_sched_barrier(0);
-            turned_of(stage, S::TENSOR, ot);
+            if constexpr (TIGHT)
+                rows_of(next, S::TENSOR, f1);
+            else
+                turned_of(stage, S::TENSOR, ot);
             __builtin_amdgcn_sched_barrier(0);
             const u32x4_t po = BlocksPackOperand<BF16>(p[0], p[1]);
             dso = BlocksPackOperand<BF16>(ds[0], ds[1]);
             product(f1, vf, ds1);
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (TIGHT) turned_of(stage, S::TENSOR, ot);
             if (more) {
 #pragma unroll
                 for (uint32_t y = 1; y < (PER + 7) / 8; ++y) load_rows(s + 3, y, to);
                 load_info(s + 3, to);
             }
             __builtin_amdgcn_sched_barrier(0);
-            turned_of(stage, 0, qt);
+            if constexpr (!TIGHT) turned_of(stage, 0, qt);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int d = 0; d < OD; ++d) av[d] = BlocksMfma<BF16>(po, u32x4_t{ot[d][0][0], ot[d][0][1], ot[d][1][0], ot[d][1][1]}, av[d]);
+            if constexpr (TIGHT) {
+                __builtin_amdgcn_sched_barrier(0);
+                turned_of(stage, 0, qt);
+                __builtin_amdgcn_sched_barrier(0);
+                add_keys();
+            }
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
                 p[y] = p1[y];
                 ds[y] = ds1[y];
             }
         }
-        add_keys();
+        if constexpr (!TIGHT) add_keys();
     }
     // the second row group's sums are added to the first's
     if (RGS > 1) {
