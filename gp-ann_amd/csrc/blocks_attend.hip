@@ -336,14 +336,13 @@ __device__ __forceinline__ void BlocksWalkAttend(float scale2, const BlocksWalkA
     }
 }
 
-// NT: tiles taken at a time, 4 where a block is a multiple of them
-template <bool BF16, int DC, int CT, int NT>
+// NT: tiles taken at a time; NM: of how many blocks they may be
+template <bool BF16, int DC, int CT, int NT, int NM>
 __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint32_t tpw, uint32_t mtiles, uint32_t tiles, uint16_t* __restrict__ out,
                                                               float* __restrict__ lse) {
     TakeWholeRegisterFile();
     using S = BlocksWalkShape<DC>;
     constexpr int KS = DC / 2;
-    constexpr bool ONE = NT == 4;
     extern __shared__ __attribute__((aligned(1024))) char s_walk[];   // stages, tables
     __shared__ uint32_t s_count, s_scratch[8][64];
     const BlocksWalkTables<DC> tab(s_walk);
@@ -412,12 +411,12 @@ __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint
 #pragma unroll 1
             for (uint32_t z = 0; z < 4; z += NT) {
                 const uint32_t first = s % kDescribed * 4 + z;
-                int start[ONE ? 1 : NT];
-                uint32_t mask[ONE ? 1 : NT], any = 0;
+                int start[NM];
+                uint32_t mask[NM], any = 0;
 #pragma unroll
-                for (uint32_t y = 0; y < (ONE ? 1 : NT); ++y) {
-                    start[y] = __builtin_amdgcn_readlane(now.start, (int)(first + y));
-                    mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)now.mask, (int)(first + y));
+                for (uint32_t y = 0; y < NM; ++y) {
+                    start[y] = __builtin_amdgcn_readlane(now.start, (int)(first + y * (NT / NM)));
+                    mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)now.mask, (int)(first + y * (NT / NM)));
                     any |= mask[y];
                 }
                 if (any)
@@ -658,11 +657,11 @@ __global__ void __launch_bounds__(512) BlocksWeighKernel(BlocksArgs a, uint32_t 
 // ---- host -----------------------------------------------------------------------------------------------------------------------------------
 static size_t WeighSpace(const BlocksArgs& a) { return a.Tq <= 1 ? 0 : BlocksAlign((size_t)a.B * a.Hkv * a.nblk * ((a.Tq + 31) / 32) * 4); }
 
-template <bool BF16, int DC, int CT, int NT>
+template <bool BF16, int DC, int CT, int NT, int NM>
 static gpann_status AttendWalk(const BlocksArgs& a, uint16_t* out, float* lse, hipStream_t st) {
     const uint32_t cols = 16 * CT, mtiles = (a.G + cols - 1) / cols, tpw = std::max(1u, cols / a.G);
     const uint64_t waves = mtiles > 1 ? (uint64_t)a.Tq * mtiles : (a.Tq + tpw - 1) / tpw, tiles = (waves + 7) / 8;
-    return BlocksLaunch(BlocksAttendWalkKernel<BF16, DC, CT, NT>, BlocksPairGrid((uint64_t)a.B * a.Hkv, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, lse);
+    return BlocksLaunch(BlocksAttendWalkKernel<BF16, DC, CT, NT, NM>, BlocksPairGrid((uint64_t)a.B * a.Hkv, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, lse);
 }
 
 template <bool BF16, int DC>
@@ -674,10 +673,12 @@ static gpann_status Attend(const BlocksArgs& a, uint16_t* out, float* lse, hipSt
         // 1024 workgroups of 32 columns, 536 us against 588; 777 rows x 12 heads, 120 workgroups, 152 us against 103.  (Wide heads have no registers for it.)
         if constexpr (DC <= 8)
             if (pairs * (((uint64_t)a.Tq * a.G + 255) / 256) >= 512)
-                return a.bs % 64 == 0 ? AttendWalk<BF16, DC, 2, 4>(a, out, lse, st) : AttendWalk<BF16, DC, 2, 2>(a, out, lse, st);
+                return a.bs % 64 == 0   ? AttendWalk<BF16, DC, 2, 4, 1>(a, out, lse, st)
+                       : a.bs % 32 == 0 ? AttendWalk<BF16, DC, 2, 2, 1>(a, out, lse, st)
+                                        : AttendWalk<BF16, DC, 2, 2, 2>(a, out, lse, st);
         if constexpr (DC <= 8)
-            if (a.bs % 64 == 0) return AttendWalk<BF16, DC, 1, 4>(a, out, lse, st);
-        return AttendWalk<BF16, DC, 1, 2>(a, out, lse, st);
+            if (a.bs % 32 == 0) return a.bs % 64 == 0 ? AttendWalk<BF16, DC, 1, 4, 1>(a, out, lse, st) : AttendWalk<BF16, DC, 1, 4, 2>(a, out, lse, st);
+        return a.bs % 32 == 0 ? AttendWalk<BF16, DC, 1, 2, 1>(a, out, lse, st) : AttendWalk<BF16, DC, 1, 2, 2>(a, out, lse, st);
     }
     // few query rows: their keys are divided over wavefronts until the chip's 2048 have something to do
     uint32_t waves = 1;

@@ -276,8 +276,8 @@ __device__ __forceinline__ void BlocksWalkQueryGradTight(float scale2, const Blo
     }
 }
 
-// NT: tiles taken at a time, 4 where a block is a multiple of them; ONE: they are of one block
-template <bool BF16, int DC, uint32_t NT, bool ONE>
+// NT: tiles taken at a time; NM: of how many blocks they may be
+template <bool BF16, int DC, int NT, int NM>
 __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint32_t tpw, uint32_t mtiles, uint32_t tiles, const uint16_t* __restrict__ out,
                                                              const uint16_t* __restrict__ dout, const float* __restrict__ lse, uint16_t* __restrict__ dq,
                                                              BlocksRowInfo info) {
@@ -359,12 +359,12 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
 #pragma unroll 1
             for (uint32_t z = 0; z < 4; z += NT) {
                 const uint32_t first = s % kDescribed * 4 + z;
-                int start[ONE ? 1 : NT];
-                uint32_t mask[ONE ? 1 : NT], any = 0;
+                int start[NM];
+                uint32_t mask[NM], any = 0;
 #pragma unroll
-                for (uint32_t y = 0; y < (ONE ? 1 : NT); ++y) {
-                    start[y] = __builtin_amdgcn_readlane(now.start, (int)(first + y));
-                    mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)now.mask, (int)(first + y));
+                for (uint32_t y = 0; y < NM; ++y) {
+                    start[y] = __builtin_amdgcn_readlane(now.start, (int)(first + y * (NT / NM)));
+                    mask[y] = (uint32_t)__builtin_amdgcn_readlane((int)now.mask, (int)(first + y * (NT / NM)));
                     any |= mask[y];
                 }
                 if (any) {
@@ -891,9 +891,9 @@ gpann_status Backward(const BlocksArgs& a, const uint16_t* out, const float* lse
     if (a.Tq > 0) {
         const uint32_t mtiles = (a.G + 15) / 16, tpw = std::max(1u, 16 / a.G);
         const uint64_t waves = mtiles > 1 ? (uint64_t)a.Tq * mtiles : (a.Tq + tpw - 1) / tpw, tiles = (waves + 7) / 8;
-        auto kernel = a.bs % 32 == 0 ? BlocksQueryGradKernel<BF16, DC, 2, true> : BlocksQueryGradKernel<BF16, DC, 2, false>;
+        auto kernel = a.bs % 32 == 0 ? BlocksQueryGradKernel<BF16, DC, 2, 1> : BlocksQueryGradKernel<BF16, DC, 2, 2>;
         if constexpr (DC <= 8)
-            if (a.bs % 64 == 0) kernel = BlocksQueryGradKernel<BF16, DC, 4, true>;
+            if (a.bs % 32 == 0) kernel = a.bs % 64 == 0 ? BlocksQueryGradKernel<BF16, DC, 4, 1> : BlocksQueryGradKernel<BF16, DC, 4, 2>;
         GPANN_TRY(BlocksLaunch(kernel, BlocksPairGrid(pairs, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, dout, lse,
                                dq, info));
     }
