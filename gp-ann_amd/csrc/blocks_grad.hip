@@ -458,12 +458,22 @@ __global__ void __launch_bounds__(1024) BlocksPartsKernel(BlocksArgs a, uint32_t
     uint32_t base = 0, slots = 0;
     for (uint32_t j0 = 0; j0 < a.nblk; j0 += 1024) {
         const uint32_t in = min(1024u, a.nblk - j0);
-        for (uint32_t j = wave; j < in; j += 16) {
-            const uint32_t* row = bits + ((uint64_t)pair * a.nblk + j0 + j) * words;
-            uint32_t c = 0;
-            for (uint32_t w = lane; w < words; w += 64) c += (uint32_t)__popc(row[w]);
-            for (int s = 32; s > 0; s >>= 1) c += __shfl_xor(c, s);
-            if (lane == 0) s_n[j] = c;
+        for (uint32_t j = wave; j < in; j += 16 * 8) {   // eight blocks' words on their way at a time
+            const uint32_t* row[8];
+            uint32_t c[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                row[i] = bits + ((uint64_t)pair * a.nblk + j0 + min(j + 16 * i, in - 1)) * words;
+                c[i] = 0;
+            }
+            for (uint32_t w = lane; w < words; w += 64)
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) c[i] += (uint32_t)__popc(row[i][w]);
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                for (int s = 32; s > 0; s >>= 1) c[i] += __shfl_xor(c[i], s);
+                if (lane == 0 && j + 16 * i < in) s_n[j + 16 * i] = c[i];
+            }
         }
         __syncthreads();
         const uint32_t j = j0 + tid, rows = tid < in ? s_n[tid] : 0, n = tid < in ? max(1u, (rows + part - 1) / part) : 0, m = n > 1 ? n : 0;
@@ -806,7 +816,7 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
     }
 }
 
-// adds the parts of a block; four dimensions a thread
+// adds the parts of a block, in order; four dimensions a thread
 template <bool BF16>
 __global__ void __launch_bounds__(256) BlocksKeyGradJoinKernel(BlocksArgs a, uint32_t d, uint32_t part_rows, uint32_t slots, const uint32_t* __restrict__ counts,
                                                                const int* __restrict__ first_slot, const float* __restrict__ partial, uint16_t* __restrict__ dk,
@@ -816,22 +826,21 @@ __global__ void __launch_bounds__(256) BlocksKeyGradJoinKernel(BlocksArgs a, uin
     if (slot < 0) return;
     const uint32_t n = (counts[(uint64_t)pair * a.nblk + block] + part_rows - 1) / part_rows;
     const uint64_t step = (uint64_t)a.bs * 2 * d;
-    const float* from = partial + ((uint64_t)pair * slots + slot) * step;
-    for (uint32_t i = threadIdx.x * 4; i < a.bs * 2 * d; i += 1024) {
-        const uint32_t row = block * a.bs + i / (2 * d), value = i / d % 2, c = i % d;
-        if (row >= a.Tk) break;
-        float4 x = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t p = 0; p < n; ++p) {
-            const float4 y = *reinterpret_cast<const float4*>(from + p * step + i);
-            x.x += y.x;
-            x.y += y.y;
-            x.z += y.z;
-            x.w += y.w;
-        }
-        const float f = value ? 1.f : a.scale;
-        uint16_t* to = value ? dv + b * a.vs[0] + row * a.vs[1] + h * a.vs[2] + c : dk + b * a.ks[0] + row * a.ks[1] + h * a.ks[2] + c;
-        *reinterpret_cast<u32x2_t*>(to) = u32x2_t{BlocksPack<BF16>(x.x * f, x.y * f), BlocksPack<BF16>(x.z * f, x.w * f)};
+    const uint32_t i = (blockIdx.z * 256 + threadIdx.x) * 4, row = block * a.bs + i / (2 * d), value = i / d % 2, c = i % d;
+    if (i >= a.bs * 2 * d || row >= a.Tk) return;
+    const float* from = partial + ((uint64_t)pair * slots + slot) * step + i;
+    float4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (uint32_t p = 0; p < n; ++p) {
+        const float4 y = *reinterpret_cast<const float4*>(from + p * step);
+        x.x += y.x;
+        x.y += y.y;
+        x.z += y.z;
+        x.w += y.w;
     }
+    const float f = value ? 1.f : a.scale;
+    uint16_t* to = value ? dv + b * a.vs[0] + row * a.vs[1] + h * a.vs[2] + c : dk + b * a.ks[0] + row * a.ks[1] + h * a.ks[2] + c;
+    *reinterpret_cast<u32x2_t*>(to) = u32x2_t{BlocksPack<BF16>(x.x * f, x.y * f), BlocksPack<BF16>(x.z * f, x.w * f)};
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------------------
@@ -910,8 +919,8 @@ gpann_status Backward(const BlocksArgs& a, const uint16_t* out, const float* lse
     else
         GPANN_TRY((KeyGrad<BF16, DC, 1, 2>(a, s, dout, info, dk, dv, ws, st)));
     if (s.slots > 0) {
-        hipLaunchKernelGGL(BlocksKeyGradJoinKernel<BF16>, dim3(a.nblk, (uint32_t)pairs), dim3(256), 0, st, a, DC * 16, s.part_rows, s.slots, counts, first_slot,
-                           reinterpret_cast<const float*>(ws + s.partial), dk, dv);
+        hipLaunchKernelGGL(BlocksKeyGradJoinKernel<BF16>, dim3(a.nblk, (uint32_t)pairs, (a.bs * 2 * DC * 16 + 1023) / 1024), dim3(256), 0, st, a, DC * 16, s.part_rows,
+                           s.slots, counts, first_slot, reinterpret_cast<const float*>(ws + s.partial), dk, dv);
         GPANN_HIP_TRY(hipGetLastError());
     }
     return GPANN_OK;
