@@ -99,7 +99,9 @@ __device__ __forceinline__ bool BlocksPairOf(uint32_t id, uint32_t pairs, uint32
     tile = rest % tiles;
     return pair < pairs;
 }
-// bits[sequence, head][block][query row / 32] of the rows that probe a block; every word is written
+// bits[sequence, head][block][query row / 32] of the rows that probe a block; every word is written.  A workgroup has kMarkRows query rows and kMarkBlocks blocks
+constexpr uint32_t kMarkRows = 128, kMarkBlocks = 512;
+gpann_status BlocksCheckMarks(const gpann_blocks_layout* L);   // what its grid, and the others of (sequence, head) pairs, have room for
 gpann_status BlocksMarkProbes(const BlocksArgs& a, uint32_t words, uint32_t* bits, hipStream_t st);
 size_t BlocksBackwardSpace(const BlocksArgs& a, uint32_t d);
 

@@ -40,10 +40,17 @@ gpann_status BlocksCheckLayout(const gpann_blocks_layout* L) {
             GPANN_REQUIRE(s[i] <= (i == 0 ? (int64_t)1 << 40 : i == 1 ? (int64_t)1 << 22 : (int64_t)1 << 31),
                           "a stride above 2^40 (batch or page), 2^22 (row) or 2^31 (head) elements");
         }
+    GPANN_REQUIRE(BlocksAligned(4, L->q_len) && BlocksAligned(4, L->kv_len) && BlocksAligned(4, L->page_table), "lengths and page table must be 4-byte aligned");
     if (L->page_table) {
         GPANN_REQUIRE(L->page_stride >= BlocksPerSequence(L), "layout.page_stride is smaller than a sequence's blocks");
         GPANN_REQUIRE(L->n_pages <= 0x7fffffffu, "more than 2^31 - 1 pages");
     }
+    return GPANN_OK;
+}
+
+gpann_status BlocksCheckMarks(const gpann_blocks_layout* L) {
+    GPANN_REQUIRE((uint64_t)L->batch * L->kv_heads <= 65535, "more than 65535 (sequence, head) pairs");
+    GPANN_REQUIRE(L->q_rows <= 65535 * kMarkRows, "more than 65535 * 128 query rows");
     return GPANN_OK;
 }
 
@@ -375,14 +382,15 @@ __global__ void __launch_bounds__(1024) BlocksRouteRowKernel(BlocksArgs a, const
         BlocksSelect<0>(s_key, nb, a.P, first, last, threadIdx.x, out);
 }
 
+// A workgroup per query row and head, or matrix tiles: those hold a workgroup's keys in 128 KB, so with more blocks they would have fewer than four query rows
+static bool BlocksRouteByRow(uint32_t rows, uint32_t blocks) { return rows < 16 || blocks > 128 * 1024 / 8 / 4; }
 template <bool BF16, int DC>
 static gpann_status Route(const BlocksArgs& a, const float* summary, uint32_t first, uint32_t last, int32_t* probes, hipStream_t st) {
     // keys of a workgroup's query rows in 128 KB; groups are given up while there are not two workgroups per CU
     const uint64_t pairs = (uint64_t)a.B * a.Hkv, room = 128 * 1024 / 8;
-    if (a.Tq < 16 || a.nblk > room / 4) {   // the matrix tiles would hold fewer than four query rows
+    if (BlocksRouteByRow(a.Tq, a.nblk)) {
         const size_t lds = (size_t)a.nblk * 8;
         auto kernel = BlocksRouteRowKernel<BF16, DC>;
-        GPANN_REQUIRE(pairs <= 65535, "more than 65535 (sequence, head) pairs");
         if (lds > 32 * 1024) GPANN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         hipLaunchKernelGGL(kernel, dim3(a.Tq, (uint32_t)pairs), dim3(1024), lds, st, a, summary, first, last, probes);
         GPANN_HIP_TRY(hipGetLastError());
@@ -570,6 +578,10 @@ gpann_status gpann_blocks_route(const gpann_blocks_layout* L, const void* q, con
     GPANN_REQUIRE(nprobe >= 1 && nprobe <= GPANN_BLOCKS_MAX_PROBE, "nprobe must be 1 .. GPANN_BLOCKS_MAX_PROBE");
     GPANN_REQUIRE(first <= nprobe && last <= nprobe - first, "first + last must not exceed nprobe");
     GPANN_REQUIRE(last >= 1 || !(L->flags & GPANN_BLOCKS_CAUSAL), "a causal route needs last >= 1");
+    if (BlocksRouteByRow(L->q_rows, BlocksPerSequence(L))) {
+        GPANN_REQUIRE((uint64_t)L->batch * L->kv_heads <= 65535, "more than 65535 (sequence, head) pairs");
+        GPANN_REQUIRE(L->q_rows < 1u << 22, "2^22 query rows or more over more than 4096 blocks");
+    }
     GPANN_BLOCKS_ENTER(L, stream);
     const BlocksArgs a = BlocksMakeArgs(L, q, nullptr, nullptr, nullptr, nprobe);
     if (a.B == 0 || a.Tq == 0) return GPANN_OK;

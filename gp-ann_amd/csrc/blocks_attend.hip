@@ -745,6 +745,7 @@ gpann_status gpann_blocks_weigh(const gpann_blocks_layout* L, const void* q, con
     GPANN_REQUIRE(BlocksAligned(16, q) && BlocksAligned(16, k), "q and k must be 16-byte aligned");
     GPANN_REQUIRE(BlocksAligned(4, probes) && BlocksAligned(4, lse) && BlocksAligned(4, mass_in) && BlocksAligned(4, mass_out), "probes, lse and mass must be 4-byte aligned");
     GPANN_REQUIRE(nprobe >= 1 && nprobe <= GPANN_BLOCKS_MAX_PROBE, "nprobe must be 1 .. GPANN_BLOCKS_MAX_PROBE");
+    if (L->q_rows > 1) GPANN_TRY(BlocksCheckMarks(L));
     const BlocksArgs a = BlocksMakeArgs(L, q, k, nullptr, probes, nprobe);
     GPANN_TRY(BlocksCheckWorkspace(workspace, workspace_bytes, WeighSpace(a)));
     GPANN_BLOCKS_ENTER(L, stream);

@@ -408,7 +408,6 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
 }
 
 // ---- which query rows probe a block -------------------------------------------------------------------------------------------------------------
-constexpr uint32_t kMarkRows = 128, kMarkBlocks = 512;   // query rows and blocks of a workgroup
 // One workgroup per pair, kMarkRows query rows and kMarkBlocks blocks: bits are set in LDS and every word is written, so nothing has to be cleared
 __global__ void __launch_bounds__(256) BlocksBitsKernel(BlocksArgs a, uint32_t words, uint32_t* __restrict__ bits) {
     __shared__ uint32_t s_bits[kMarkBlocks * (kMarkRows / 32)];
@@ -950,7 +949,7 @@ extern "C" gpann_status gpann_blocks_attend_backward(const gpann_blocks_layout* 
     GPANN_REQUIRE(BlocksDisjoint(L->q_stride, L->batch, L->q_rows, L->q_heads, L->head_dim), "dq overlaps itself");
     GPANN_REQUIRE(BlocksDisjoint(L->k_stride, L->batch, L->kv_rows, L->kv_heads, L->head_dim), "dk overlaps itself");
     GPANN_REQUIRE(BlocksDisjoint(L->v_stride, L->batch, L->kv_rows, L->kv_heads, L->head_dim), "dv overlaps itself");
-    GPANN_REQUIRE((uint64_t)L->batch * L->kv_heads <= 65535, "more than 65535 (sequence, head) pairs");
+    GPANN_TRY(BlocksCheckMarks(L));
     GPANN_REQUIRE((uint64_t)L->batch * L->q_rows * L->q_heads < 0xFFFFFFFFull, "2^32 - 1 (query row, head) rows or more");
     const BlocksArgs a = BlocksMakeArgs(L, q, k, v, probes, nprobe);
     GPANN_TRY(BlocksCheckWorkspace(workspace, workspace_bytes, BackwardLayout(a, L->head_dim).total));

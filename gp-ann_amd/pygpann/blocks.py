@@ -72,6 +72,8 @@ class Layout:
         c.q_len, c.kv_len, c.page_table = q_len or None, kv_len or None, page_table or None
         q_stride = tuple(q_stride or q)
         for name, s in (("q_stride", q_stride), ("k_stride", k_stride or kv), ("v_stride", v_stride or kv), ("out_stride", out_stride or q)):
+            if not all(-1 << 63 <= operator.index(x) < 1 << 63 for x in s):
+                raise GpannError(1, f"invalid argument: {name} = {tuple(s)} is not three signed 64-bit numbers")
             setattr(c, name, (C.c_int64 * 3)(*s))
         self.blocks = blocks
 

@@ -25,7 +25,15 @@
  *
  * Rows of a batch beyond q_len[b] are neither read nor written by route and attend (their probes, out and lse stay as they were); gradients are written
  * over the whole tensors, zero where no query reaches.  Cache rows beyond kv_len[b] are never read.  A probe outside the sequence's blocks (negative, too
- * large, not visible) and a page outside [0, n_pages) are skipped; a block probed twice by one row counts once. */
+ * large, not visible) and a page outside [0, n_pages) are skipped; a block probed twice by one row counts once.  What a call writes must not overlap what it
+ * reads, but for gpann_blocks_weigh in place.
+ *
+ * Rounding: logits, sums, softmax statistics and masses are binary32, centroids and scores as above; weights and ds are rounded once to the tensors' type
+ * where they enter a matrix product, so in GPANN_BLOCKS_FP16 those below 2^-25 count as 0 (scale a loss whose gradients are that small).
+ *
+ * Refused, besides what the arguments' comments say: backward and weigh (of more than one query row) of more than 65535 (sequence, key/value head) pairs or
+ * 65535 * 128 query rows; backward of 2^32 - 1 (query row, head) rows; route of fewer than 16 query rows or more than 4096 blocks of more than 65535 pairs
+ * or 2^22 query rows; any call of more than 2^23 workgroups (GPANN_ERR_UNSUPPORTED). */
 #ifndef GPANN_BLOCKS_H
 #define GPANN_BLOCKS_H
 
@@ -57,8 +65,8 @@ enum { /* calls a workspace is meant for (gpann_blocks_workspace_bytes) */
 
 /* The tensors of a call: q, out, dout, dq are [batch][q_rows][q_heads][head_dim]; k, v, dk, dv are [batch][kv_rows][kv_heads][head_dim] or, with a
  * page table, [n_pages][block_rows][kv_heads][head_dim] — a block is a page.  Strides are in elements, {batch or page, row, head}, the last dimension is
- * contiguous; a gradient has the strides of its tensor and dout those of out.  Strides have to be multiples of 8 (at most 2^22 for a row, 2^31 for a head) and tensors 16-byte aligned; a tensor
- * that is written must not overlap itself. */
+ * contiguous; a gradient has the strides of its tensor and dout those of out.  Strides have to be multiples of 8, at most 2^22 of a row, 2^31 of a head
+ * and 2^40 of a batch or page, tensors 16-byte aligned, and a tensor that is written must not overlap itself. */
 typedef struct gpann_blocks_layout {
     uint32_t struct_bytes;        /* sizeof(gpann_blocks_layout) of the caller's header */
     int32_t device;

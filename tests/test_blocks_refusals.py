@@ -164,3 +164,29 @@ def test_reference_gradients_against_differences():
             down = loss()
             x[i] = keep
             assert abs((up - down) / (2 * h) - grad[i]) < 1e-8      # h^2 times third derivatives of order 1, and 1e-16 / h of rounding
+
+
+@pytest.mark.parametrize("field", ["q_len", "kv_len", "page_table"])
+def test_lengths_and_page_tables_have_to_be_aligned(blocks, field):
+    L = _layout(blocks, **{field: 18}, n_pages=8)
+    for name, call in _calls(blocks, L).items():
+        _refused(blocks, call, match="4-byte aligned")
+
+
+def test_strides_that_would_wrap_are_refused(blocks):
+    for bad in (1 << 64, (1 << 63), -(1 << 64)):
+        with pytest.raises(blocks.GpannError):
+            _layout(blocks, k_stride=(bad, 128, 64))
+
+
+def test_more_pairs_or_query_rows_than_a_grid_has_room_for_are_refused(blocks):
+    many = dict(batch=60000, q_rows=2, kv_rows=16, q_heads=2, kv_heads=2, block_rows=16)
+    calls = _calls(blocks, _layout(blocks, **many), workspace_bytes=1 << 40)
+    for name in ("backward", "weigh", "route"):
+        _refused(blocks, calls[name], match="65535")
+    long = dict(batch=1, q_rows=65535 * 128 + 1, kv_rows=16, q_heads=1, kv_heads=1, block_rows=16)
+    calls = _calls(blocks, _layout(blocks, **long), workspace_bytes=1 << 40)
+    for name in ("backward", "weigh"):
+        _refused(blocks, calls[name], match="query rows")
+    long = dict(batch=1, q_rows=1 << 22, kv_rows=16 * 4097, q_heads=1, kv_heads=1, block_rows=16)
+    _refused(blocks, _calls(blocks, _layout(blocks, **long))["route"], match="query rows")

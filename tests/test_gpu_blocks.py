@@ -229,6 +229,26 @@ def test_values_that_are_not_numbers_reach_only_the_rows_that_see_them(blocks):
             assert (np.abs(out[b, t, heads] - want) <= tol).all()
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(dim=128, bs=64, kv_rows=400), dict(dim=192, dtype="fp16"), dict(dim=256, bs=16, kv_rows=100)], ids=str)
+def test_gradients_of_rows_that_do_not_see_what_is_not_a_number(blocks, kw):
+    """odd query rows look at blocks 0 and 4, even ones at blocks 1 and 2, which hold a NaN and infinities"""
+    probes = np.full((1, 40, 2, 3), -1, np.int32)
+    probes[0, 1::2, :, :2], probes[0, ::2, :, :2] = (0, 4), (1, 2)
+    p = Problem(blocks, **{**dict(seed=18, batch=1, q_rows=40, kv_rows=200, probes=probes, nprobe=3), **kw})
+    bs = p.bs
+    p.v[0, bs + 1], p.v[0, bs + 2], p.k[0, 2 * bs + 3] = float("inf"), float("nan"), float("nan")
+    p.attend()
+    p.backward()
+    torch.cuda.synchronize()
+    assert torch.isnan(p.dq[0, ::2]).all()
+    p.dq[0, ::2] = 0
+    for x in (p.dk, p.dv):
+        x[0, bs:3 * bs] = 0
+    every = p.rows
+    p.rows = lambda: (row for row in every() if row[1] % 2)
+    p.check_backward()
+
+
 def test_blocks_that_lie_beyond_32_bits(blocks):
     """pages 2^31 elements apart"""
     p = Problem(blocks, seed=17, batch=1, kv_rows=96, paged=True, nprobe=3)
