@@ -45,6 +45,12 @@ template <bool BF16>
 __device__ __forceinline__ u32x4_t BlocksPackOperand(const f32x4_t& a, const f32x4_t& b) {
     return u32x4_t{BlocksPack<BF16>(a[0], a[1]), BlocksPack<BF16>(a[2], a[3]), BlocksPack<BF16>(b[0], b[1]), BlocksPack<BF16>(b[2], b[3])};
 }
+// eight ones: the other operand's sum over its 32 rows, in every row of C
+template <bool BF16>
+__device__ __forceinline__ u32x4_t BlocksOnes() {
+    constexpr uint32_t two = BF16 ? 0x3F803F80u : 0x3C003C00u;
+    return u32x4_t{two, two, two, two};
+}
 
 // by rows: `p` = the lane's row + 8 * (lane / 16)
 template <int KS>
