@@ -7,8 +7,9 @@ namespace gpann {
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------------------
 // One pass over the probed rows with a running maximum and sum per query row, in powers of two (softmax(x) = 2^(x log2 e - max) / sum).  A wavefront works
-// on one query row's heads of a group (at most 16: the columns of the matrix tiles) and takes 32 keys a step: X^T = K Q^T, then O^T += V^T P^T, both
-// operands straight from memory (blocks_tile.h).  `waves` wavefronts share a query row's keys and join through LDS.
+// on one query row's heads of a group (at most 16: the columns of the matrix tiles): X^T = K Q^T, then O^T += V^T P^T.
+//
+// First the form that reads both operands straight from memory, 32 keys a step (blocks_tile.h): for rows that are done again by themselves.
 template <bool BF16, int DC>
 struct BlocksStep {
     static constexpr int KS = DC / 2, N = DC / 2;
@@ -94,31 +95,14 @@ __device__ __forceinline__ void BlocksAttendStep(const BlocksArgs& a, int visibl
 }
 
 // All of a query row's probed rows from tile `u` to `end`, 32 a step
-template <bool BF16, int DC, bool AHEAD>
+template <bool BF16, int DC>
 __device__ __forceinline__ void BlocksAttendRange(const BlocksArgs& a, uint32_t h, int visible, int block, int64_t ko, int64_t vo, uint32_t u, uint32_t end,
                                                   uint32_t lane, const u32x4_t (&q)[DC / 2], f32x4_t (&o)[DC], float& top, float& sum) {
     BlocksCursor c(u, a.bs / 16);
-    if constexpr (AHEAD && DC <= 8) {   // the next step's rows are on their way while this one is multiplied
-        BlocksStep<BF16, DC> s0, s1;
-        BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u, lane, s0);
-        for (;;) {
-            const bool more = u + 2 < end;
-            if (more) BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u - 2, lane, s1);
-            BlocksAttendStep(a, visible, lane, s0, q, o, top, sum);
-            if (!more) break;
-            u += 2;
-            const bool again = u + 2 < end;
-            if (again) BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u - 2, lane, s0);
-            BlocksAttendStep(a, visible, lane, s1, q, o, top, sum);
-            if (!again) break;
-            u += 2;
-        }
-    } else {
-        for (; u < end; u += 2) {
-            BlocksStep<BF16, DC> s;
-            BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u, lane, s);
-            BlocksAttendStep(a, visible, lane, s, q, o, top, sum);
-        }
+    for (; u < end; u += 2) {
+        BlocksStep<BF16, DC> s;
+        BlocksLoadStep(a, h, visible, block, ko, vo, c, end - u, lane, s);
+        BlocksAttendStep(a, visible, lane, s, q, o, top, sum);
     }
 }
 
@@ -137,19 +121,175 @@ __device__ __forceinline__ void BlocksAttendStore(const BlocksArgs& a, uint32_t 
     if (lse && g == 0) lse[((int64_t)b * a.Tq + t) * a.Hq + head] = sum == 0.f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
 }
 
+// The form for one query row a sequence: `waves` wavefronts of `splits` workgroups share a query row's keys and join through LDS (and memory).  Rows come to
+// LDS by DMA, whole rows an instruction, into a place of the wavefront's own; from there a step's K, then its V, go to registers, and the next step's follow at
+// once.  (Read from memory as the matrix instruction wants them, 16 bytes of 16 rows side by side, K costs the address unit 64 cycles an instruction instead
+// of 16: 16 x 64 rows for each of 8 heads, 11.0 us that way.)
+template <int DC>
+struct BlocksTokenShape {
+    using W = BlocksWalkShape<DC>;
+    static constexpr uint32_t D = DC * 16, TILES = D <= 128 ? 2 : 1, TILE = D * 32, TENSOR = TILES * TILE, PER = W::CPR / 4, LOADS = TILES * PER, RING = 8 * 2 * TENSOR;
+};
+struct BlocksTokenStep {   // 16-row tiles of a step
+    uint64_t k[2], v[2];   // addresses of their first rows
+    int start[2], last[2]; // positions of those; the last row that may be read, in the tile
+    uint64_t second;       // the second tile is a tile of the range (64 bits: padding behind it would be copied through memory)
+};
+template <int DC>
+struct BlocksTokenLoader {
+    using S = BlocksTokenShape<DC>;
+    uint32_t kplace[S::PER], vplace[S::PER], lane, krow, vrow;
+    __device__ __forceinline__ BlocksTokenLoader(const BlocksArgs& a, uint32_t lane_) : lane(lane_), krow((uint32_t)a.ks[1] * 2), vrow((uint32_t)a.vs[1] * 2) {
+#pragma unroll
+        for (uint32_t j = 0; j < S::PER; ++j) {
+            kplace[j] = Place(j, krow, 15);
+            vplace[j] = Place(j, vrow, 15);
+        }
+    }
+    __device__ __forceinline__ uint32_t Place(uint32_t j, uint32_t stride, int last) const {
+        const uint32_t at = j * 64 + lane, row = at / S::W::CPR;
+        return (uint32_t)min((int)row, last) * stride + S::W::Slot(at % S::W::CPR, row) * 16;
+    }
+    __device__ __forceinline__ void Load(const BlocksTokenStep& st, bool value, uint32_t to) const {
+#pragma unroll
+        for (uint32_t x = 0; x < S::TILES; ++x)
+#pragma unroll
+            for (uint32_t j = 0; j < S::PER; ++j) {
+                uint32_t offset = value ? vplace[j] : kplace[j];
+                if (st.last[x] < 15) offset = Place(j, value ? vrow : krow, st.last[x]);   // rows past the last visible one are not read
+                BlocksDma(value ? st.v[x] : st.k[x], offset, to + (x * S::PER + j) * 1024);
+            }
+    }
+};
+
 template <bool BF16, int DC>
-__global__ void __launch_bounds__(512) BlocksAttendKernel(BlocksArgs a, uint32_t waves, uint32_t mtiles, uint32_t tiles, uint16_t* __restrict__ out,
-                                                          float* __restrict__ lse) {
+__device__ __forceinline__ void BlocksAttendTokens(const BlocksArgs& a, uint32_t h, int visible, int block, int64_t ko, int64_t vo, uint32_t u, uint32_t end,
+                                                   uint32_t lane, uint32_t ring, u32x4_t (&q)[DC / 2], f32x4_t (&o)[DC], float& top, float& sum) {
+    using S = BlocksTokenShape<DC>;
+    constexpr int KS = DC / 2, T = S::TILES;
+    const float inf = __builtin_inff();
+    const int g4 = (int)(lane >> 4) * 4;
+    BlocksCursor c(u, a.bs / 16);
+    const BlocksTokenLoader<DC> loader(a, lane);
+    const BlocksWalkAddresses<DC> ad(lane);
+    auto describe = [&](uint32_t left) {
+        BlocksTokenStep st{};
+        st.second = T == 2 && left > 1;
+#pragma unroll
+        for (int x = 0; x < T; ++x) {
+            const int blk = __builtin_amdgcn_readlane(block, (int)c.slot), base = (int)c.sub * 16, most = visible - 1 - blk * (int)a.bs;
+            const int first = min(base, most & ~15);   // a tile without visible rows: the rows of the last one with any
+            st.start[x] = blk * (int)a.bs + base;
+            st.last[x] = min(15, most - first);
+            st.k[x] = (uint64_t)(a.k + BlocksReadLane64(ko, c.slot) + h * a.ks[2] + first * a.ks[1]);
+            st.v[x] = (uint64_t)(a.v + BlocksReadLane64(vo, c.slot) + h * a.vs[2] + first * a.vs[1]);
+            if (x == 0 && st.second) c.Next();
+        }
+        c.Next();
+        return st;
+    };
+    BlocksTokenStep st = describe(end - u);
+    loader.Load(st, false, ring);
+    loader.Load(st, true, ring + S::TENSOR);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[s]));   // here, not in the loop, is where these loads are waited for
+    for (; u < end; u += T) {
+        const bool more = u + T < end;
+        const BlocksTokenStep next = more ? describe(end - u - T) : st;
+        BlocksDmaWait<S::LOADS>();   // K has landed; V is on its way
+        f32x4_t x[2];
+        {
+            uint32_t step[KS];
+            u32x4_t k[T][KS];
+            ad.RowSteps(ring, step);
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int y = 0; y < T; ++y) k[y][s] = BlocksReadRow(step[s] + y * S::TILE);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // its place is free again
+            if (more) loader.Load(next, false, ring);
+            x[0] = x[1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int y = 0; y < T; ++y) x[y] = BlocksMfma<BF16>(k[y][s], q[s], x[y]);
+        }
+        const bool edge = (T == 2 && !st.second) || st.start[0] + 16 > visible || (T == 2 && st.start[1] + 16 > visible);
+        float best = -inf;
+#pragma unroll
+        for (int y = 0; y < T; ++y) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[y][i] *= a.scale2;
+            if (edge)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[y][i] = (y == 0 || st.second) && st.start[y] + g4 + i < visible ? x[y][i] : -inf;
+            best = BlocksMaxOf4(x[y], best);
+        }
+        best = BlocksMaxOver4(best);
+        if (__ballot(best > top + kBlocksSlack)) {
+            best = fmaxf(top, best);
+            const float shrink = top == best ? 1.f : BlocksExp2(top - best);   // (top = best = -inf: nothing seen yet)
+            top = best;
+            sum *= shrink;
+#pragma unroll
+            for (int d = 0; d < DC; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][i] *= shrink;
+        }
+        const float from = top == -inf ? 0.f : top;   // 2^(-inf - 0) = 0
+#pragma unroll
+        for (int y = 0; y < T; ++y) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[y][i] = BlocksExp2(x[y][i] - from);
+            sum += (x[y][0] + x[y][1]) + (x[y][2] + x[y][3]);
+        }
+        // the weights enter the second product in the type of the values: 2^-9 (bf16) or 2^-12 (fp16) of each at most, as the values themselves
+        const u32x4_t p = BlocksPackOperand<BF16>(x[0], x[1]);
+        if (more)
+            BlocksDmaWait<S::LOADS>();   // V has landed; the next K is on its way
+        else
+            BlocksDmaWait<0>();
+        u32x2_t v[DC][2];
+        uint32_t turned[DC];
+        ad.template Dimensions<DC>(ring + S::TENSOR, turned);
+#pragma unroll
+        for (int d = 0; d < DC; ++d)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) v[d][y] = y < T ? BlocksReadTransposed(turned[d] + y * S::TILE) : u32x2_t{0u, 0u};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (more) loader.Load(next, true, ring + S::TENSOR);
+        if (edge)   // 0 * value, whatever stands in for a row outside
+#pragma unroll
+            for (int y = 0; y < T; ++y)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const int at = st.start[y] + g4 + 2 * w;
+                    const bool there = y == 0 || st.second;
+                    const uint32_t keep = (there && at < visible ? 0xFFFFu : 0u) | (there && at + 1 < visible ? 0xFFFF0000u : 0u);
+#pragma unroll
+                    for (int d = 0; d < DC; ++d) v[d][y][w] &= keep;
+                }
+#pragma unroll
+        for (int d = 0; d < DC; ++d) o[d] = BlocksMfma<BF16>(u32x4_t{v[d][0][0], v[d][0][1], v[d][1][0], v[d][1][1]}, p, o[d]);
+        st = next;
+    }
+}
+
+template <bool BF16, int DC>
+__global__ void __launch_bounds__(512) BlocksAttendKernel(BlocksArgs a, uint32_t waves, uint32_t splits, uint32_t mtiles, uint32_t tiles, uint16_t* __restrict__ out,
+                                                          float* __restrict__ lse, float* __restrict__ sums) {
     TakeWholeRegisterFile();
     constexpr int D = DC * 16;
-    extern __shared__ float s_join[];   // waves > 1: [wavefront][16 rows][D], then [wavefront][16][2]
+    extern __shared__ __attribute__((aligned(1024))) float s_join[];   // the wavefronts' places; behind them, waves > 1: [wavefront][16 rows][D + 2]
     __shared__ uint32_t s_scratch[8][64];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     uint32_t pair, tile;
-    if (!BlocksPairOf(blockIdx.x, a.B * a.Hkv, tiles, pair, tile)) return;
+    if (!BlocksPairOf(blockIdx.x, a.B * a.Hkv, tiles * splits, pair, tile)) return;
+    const uint32_t split = tile % splits;
+    tile /= splits;
     const uint32_t b = pair / a.Hkv, h = pair % a.Hkv, per = 8 / waves;
     const int n = BlocksKvLen(a, b), m = BlocksQLen(a, b);
-    const uint32_t task = tile * per + wave / waves, part = wave % waves, t = task / mtiles, mt = task % mtiles;
+    const uint32_t task = tile * per + wave / waves, part = split * waves + wave % waves, parts = splits * waves, t = task / mtiles, mt = task % mtiles;
     const uint32_t heads = min(16u, a.G - mt * 16), head = h * a.G + mt * 16 + min(r, heads - 1);
     const bool live = (int)t < m;
     const int visible = live ? BlocksVisible(a, n, m, (int)t) : 0;
@@ -162,20 +302,26 @@ __global__ void __launch_bounds__(512) BlocksAttendKernel(BlocksArgs a, uint32_t
         int block;
         int64_t ko, vo;
         const uint32_t count = BlocksGatherProbes(a, a.probes + (((int64_t)b * a.Tq + t) * a.Hkv + h) * a.P, b, visible, s_scratch[wave], lane, block, ko, vo);
-        const uint32_t tpb = a.bs / 16, units = count * tpb, chunk = ((units + waves - 1) / waves + 1) & ~1u;
+        const uint32_t tpb = a.bs / 16, units = count * tpb, chunk = ((units + parts - 1) / parts + 1) & ~1u;
         uint32_t u = part * chunk;
         const uint32_t end = min(units, u + chunk);
         if (u < end) {
             u32x4_t q[DC / 2];
             BlocksLoadRows<DC / 2>(a.q + b * a.qs[0] + t * a.qs[1] + head * a.qs[2] + g * 8, q);
-            BlocksAttendRange<BF16, DC, true>(a, h, visible, block, ko, vo, u, end, lane, q, o, top, sum);
+            BlocksAttendTokens<BF16, DC>(a, h, visible, block, ko, vo, u, end, lane, BlocksLdsAddress(s_join) + wave * 2 * BlocksTokenShape<DC>::TENSOR, q, o, top, sum);
         }
     }
     sum = BlocksSumOver4(sum);
     if (waves == 1) {
-        if (live && r < heads) BlocksAttendStore<BF16, DC>(a, b, t, head, g, o, top, sum, out, lse);
+        if (!live || r >= heads) return;
+        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);   // (a NaN sum stays one)
+        uint16_t* dst = out + b * a.os[0] + (int64_t)t * a.os[1] + head * a.os[2] + g * 4;
+#pragma unroll
+        for (int d = 0; d < DC; ++d) *reinterpret_cast<u32x2_t*>(dst + d * 16) = u32x2_t{BlocksPack<BF16>(o[d][0] * inv, o[d][1] * inv), BlocksPack<BF16>(o[d][2] * inv, o[d][3] * inv)};
+        if (lse && g == 0) lse[((int64_t)b * a.Tq + t) * a.Hq + head] = sum == 0.f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
         return;
     }
+    __syncthreads();   // (the sums take the place of the rows)
     float* s_ml = s_join + 8 * 16 * D;
     if (g == 0) {
         s_ml[(wave * 16 + r) * 2] = top;
@@ -183,9 +329,7 @@ __global__ void __launch_bounds__(512) BlocksAttendKernel(BlocksArgs a, uint32_t
     }
     if (r < heads && sum != 0.f) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int d = 0; d < DC; ++d) s_join[(wave * 16 + r) * D + (g * 4 + i) * DC + d] = o[d][i];
+        for (int d = 0; d < DC; ++d) *reinterpret_cast<f32x4_t*>(s_join + (wave * 16 + r) * D + d * 16 + g * 4) = o[d];
     }
     __syncthreads();
     // two neighbouring dimensions of one row a thread
@@ -206,11 +350,44 @@ __global__ void __launch_bounds__(512) BlocksAttendKernel(BlocksArgs a, uint32_t
             x += f * s_join[at * D + c];
             y += f * s_join[at * D + c + 1];
         }
+        if (splits > 1) {
+            float* to = sums + ((uint64_t)(pair * tiles + tile) * splits + split) * 16 * (D + 2) + row * (D + 2);
+            *reinterpret_cast<float2*>(to + c) = float2{x, y};
+            if (c == 0) *reinterpret_cast<float2*>(to + D) = float2{best, total};
+            continue;
+        }
         const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
         const uint32_t head2 = h * a.G + mt2 * 16 + row;
         *reinterpret_cast<uint32_t*>(out + b * a.os[0] + (int64_t)t2 * a.os[1] + head2 * a.os[2] + c) = BlocksPack<BF16>(x * inv, y * inv);
         if (lse && c == 0) lse[((int64_t)b * a.Tq + t2) * a.Hq + head2] = total == 0.f ? -__builtin_inff() : (best + __log2f(total)) * kLn2;
     }
+}
+
+// joins the parts of a query row's keys that workgroups had; two neighbouring dimensions of one head a thread
+template <bool BF16>
+__global__ void __launch_bounds__(256) BlocksAttendJoinKernel(BlocksArgs a, uint32_t d, uint32_t splits, uint32_t mtiles, uint32_t tiles, const float* __restrict__ sums,
+                                                              uint16_t* __restrict__ out, float* __restrict__ lse) {
+    const uint32_t task = blockIdx.y, pair = task / tiles, tile = task % tiles, b = pair / a.Hkv, h = pair % a.Hkv, t = tile / mtiles, mt = tile % mtiles;
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x, c = i % (d / 2) * 2, row = i / (d / 2);
+    if (row >= min(16u, a.G - mt * 16) || (int)t >= BlocksQLen(a, b)) return;
+    const float* from = sums + ((uint64_t)task * splits * 16 + row) * (d + 2);
+    const uint64_t step = (uint64_t)16 * (d + 2);
+    float best = -__builtin_inff();
+    for (uint32_t s = 0; s < splits; ++s) best = fmaxf(best, from[s * step + d]);
+    const float base = best == -__builtin_inff() ? 0.f : best;
+    float total = 0.f, x = 0.f, y = 0.f;
+#pragma unroll 4
+    for (uint32_t s = 0; s < splits; ++s) {
+        const float2 part = *reinterpret_cast<const float2*>(from + s * step + d), v = *reinterpret_cast<const float2*>(from + s * step + c);
+        const float f = part.y == 0.f ? 0.f : BlocksExp2(part.x - base);   // (a part without rows holds zeros)
+        total += f * part.y;
+        x += f * v.x;
+        y += f * v.y;
+    }
+    const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
+    const uint32_t head = h * a.G + mt * 16 + row;
+    *reinterpret_cast<uint32_t*>(out + b * a.os[0] + (int64_t)t * a.os[1] + head * a.os[2] + c) = BlocksPack<BF16>(x * inv, y * inv);
+    if (lse && c == 0) lse[((int64_t)b * a.Tq + t) * a.Hq + head] = total == 0.f ? -__builtin_inff() : (best + __log2f(total)) * kLn2;
 }
 
 // ---- forward, neighbouring query rows together ----------------------------------------------------------------------------------------------------
@@ -453,7 +630,7 @@ __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint
             const uint32_t count = vis > 0 ? BlocksGatherProbes(a, a.probes + (((int64_t)w.b * a.Tq + t) * a.Hkv + w.h) * a.P, w.b, vis, s_scratch[wave], lane, block, ko, vo) : 0;
             if (count) {
                 BlocksLoadRows<KS>(a.q + w.b * a.qs[0] + (int64_t)t * a.qs[1] + head * a.qs[2] + g * 8, q[0]);
-                BlocksAttendRange<BF16, DC, false>(a, w.h, vis, block, ko, vo, 0, count * tpb, lane, q[0], o[0], top[0], sum[0]);
+                BlocksAttendRange<BF16, DC>(a, w.h, vis, block, ko, vo, 0, count * tpb, lane, q[0], o[0], top[0], sum[0]);
             }
             sum[0] = BlocksSumOver4(sum[0]);
             if (r < some) BlocksAttendStore<BF16, DC>(a, w.b, t, head, g, o[0], top[0], sum[0], out, lse);
@@ -655,6 +832,7 @@ __global__ void __launch_bounds__(512) BlocksWeighKernel(BlocksArgs a, uint32_t 
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------------------
+constexpr uint32_t kSplitSteps = 2;
 static size_t WeighSpace(const BlocksArgs& a) { return a.Tq <= 1 ? 0 : BlocksAlign((size_t)a.B * a.Hkv * a.nblk * ((a.Tq + 31) / 32) * 4); }
 
 template <bool BF16, int DC, int CT, int NT, int NM>
@@ -664,10 +842,25 @@ static gpann_status AttendWalk(const BlocksArgs& a, uint16_t* out, float* lse, h
     return BlocksLaunch(BlocksAttendWalkKernel<BF16, DC, CT, NT, NM>, BlocksPairGrid((uint64_t)a.B * a.Hkv, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, lse);
 }
 
+// How a query row's keys are divided where there are few of them: over the wavefronts of a workgroup until the chip's 2048 have something to do, then over
+// workgroups until there is one per CU
+struct BlocksDivision {
+    uint32_t waves = 1, splits = 1, mtiles;
+    uint64_t pairs, tiles;
+    explicit BlocksDivision(const BlocksArgs& a) : mtiles((a.G + 15) / 16), pairs((uint64_t)a.B * a.Hkv) {
+        const uint64_t tasks = (uint64_t)a.Tq * mtiles, units = (uint64_t)std::min(a.P, a.nblk) * (a.bs / 16);
+        while (waves < 8 && pairs * tasks * waves < 2048) waves *= 2;
+        if (waves == 8 && units > 16 * kSplitSteps && pairs * tasks <= 64)
+            while (pairs * tasks * splits * 2 <= 256 && splits * 16 < units) splits *= 2;
+        tiles = (tasks * waves + 7) / 8;
+    }
+    size_t Space(uint32_t d) const { return splits > 1 ? BlocksAlign(pairs * tiles * splits * 16 * (d + 2) * 4) : 0; }
+};
+static size_t AttendSpace(const BlocksArgs& a, uint32_t d) { return a.Tq == 1 ? BlocksDivision(a).Space(d) : 0; }
+
 template <bool BF16, int DC>
-static gpann_status Attend(const BlocksArgs& a, uint16_t* out, float* lse, hipStream_t st) {
-    const uint32_t mtiles = (a.G + 15) / 16;
-    const uint64_t tasks = (uint64_t)a.Tq * mtiles, pairs = (uint64_t)a.B * a.Hkv;
+static gpann_status Attend(const BlocksArgs& a, uint16_t* out, float* lse, float* ws, hipStream_t st) {
+    const uint64_t pairs = (uint64_t)a.B * a.Hkv;
     if (a.Tq > 1) {
         // 32 columns a wavefront read LDS half as often for each, but make half the workgroups (one per CU at a time) of a larger union: 8192 rows x 32 heads,
         // 1024 workgroups of 32 columns, 536 us against 588; 777 rows x 12 heads, 120 workgroups, 152 us against 103.  (Wide heads have no registers for it.)
@@ -680,12 +873,14 @@ static gpann_status Attend(const BlocksArgs& a, uint16_t* out, float* lse, hipSt
             if (a.bs % 32 == 0) return a.bs % 64 == 0 ? AttendWalk<BF16, DC, 1, 4, 1>(a, out, lse, st) : AttendWalk<BF16, DC, 1, 4, 2>(a, out, lse, st);
         return a.bs % 32 == 0 ? AttendWalk<BF16, DC, 1, 2, 1>(a, out, lse, st) : AttendWalk<BF16, DC, 1, 2, 2>(a, out, lse, st);
     }
-    // few query rows: their keys are divided over wavefronts until the chip's 2048 have something to do
-    uint32_t waves = 1;
-    while (waves < 8 && pairs * tasks * waves < 2048) waves *= 2;
-    const uint64_t tiles = (tasks * waves + 7) / 8;
-    const size_t lds = waves > 1 ? (size_t)8 * 16 * (DC * 16 + 2) * 4 : 0;
-    return BlocksLaunch(BlocksAttendKernel<BF16, DC>, BlocksPairGrid(pairs, tiles), lds, st, a, waves, mtiles, (uint32_t)tiles, out, lse);
+    const BlocksDivision v(a);
+    const size_t lds = std::max<size_t>(BlocksTokenShape<DC>::RING, v.waves > 1 ? (size_t)8 * 16 * (DC * 16 + 2) * 4 : 0);
+    GPANN_TRY(BlocksLaunch(BlocksAttendKernel<BF16, DC>, BlocksPairGrid(pairs, v.tiles * v.splits), lds, st, a, v.waves, v.splits, v.mtiles, (uint32_t)v.tiles, out, lse, ws));
+    if (v.splits == 1) return GPANN_OK;
+    hipLaunchKernelGGL(BlocksAttendJoinKernel<BF16>, dim3((std::min(16u, a.G) * DC * 8 + 255) / 256, (uint32_t)(pairs * v.tiles)), dim3(256), 0, st, a, DC * 16, v.splits,
+                       v.mtiles, (uint32_t)v.tiles, ws, out, lse);
+    GPANN_HIP_TRY(hipGetLastError());
+    return GPANN_OK;
 }
 
 template <bool BF16, int DC>
@@ -716,6 +911,7 @@ gpann_status gpann_blocks_workspace_bytes(const gpann_blocks_layout* L, uint32_t
     GPANN_REQUIRE((calls & ~31u) == 0, "unknown bits in calls");
     const BlocksArgs a = BlocksMakeArgs(L, nullptr, nullptr, nullptr, nullptr, nprobe);
     size_t need = 0;
+    if (calls & GPANN_BLOCKS_ATTEND) need = std::max(need, AttendSpace(a, L->head_dim));
     if (calls & GPANN_BLOCKS_BACKWARD) need = std::max(need, BlocksBackwardSpace(a, L->head_dim));
     if (calls & GPANN_BLOCKS_WEIGH) need = std::max(need, WeighSpace(a));
     *out_bytes = need;
@@ -724,18 +920,17 @@ gpann_status gpann_blocks_workspace_bytes(const gpann_blocks_layout* L, uint32_t
 
 gpann_status gpann_blocks_attend(const gpann_blocks_layout* L, const void* q, const void* k, const void* v, const int32_t* probes, uint32_t nprobe, void* out,
                                  float* lse, void* workspace, size_t workspace_bytes, void* stream) {
-    (void)workspace;
-    (void)workspace_bytes;
     GPANN_TRY(BlocksCheckLayout(L));
     GPANN_REQUIRE(q && k && v && probes && out, "a tensor is null");
     GPANN_REQUIRE(BlocksAligned(16, q) && BlocksAligned(16, k) && BlocksAligned(16, v) && BlocksAligned(16, out), "q, k, v and out must be 16-byte aligned");
     GPANN_REQUIRE(BlocksAligned(4, probes) && BlocksAligned(4, lse), "probes and lse must be 4-byte aligned");
     GPANN_REQUIRE(nprobe >= 1 && nprobe <= GPANN_BLOCKS_MAX_PROBE, "nprobe must be 1 .. GPANN_BLOCKS_MAX_PROBE");
     GPANN_REQUIRE(BlocksDisjoint(L->out_stride, L->batch, L->q_rows, L->q_heads, L->head_dim), "out overlaps itself");
-    GPANN_BLOCKS_ENTER(L, stream);
     const BlocksArgs a = BlocksMakeArgs(L, q, k, v, probes, nprobe);
+    GPANN_TRY(BlocksCheckWorkspace(workspace, workspace_bytes, AttendSpace(a, L->head_dim)));
+    GPANN_BLOCKS_ENTER(L, stream);
     if (a.B == 0 || a.Tq == 0) return GPANN_OK;
-    GPANN_BLOCKS_DISPATCH(L, Attend, a, static_cast<uint16_t*>(out), lse, static_cast<hipStream_t>(stream));
+    GPANN_BLOCKS_DISPATCH(L, Attend, a, static_cast<uint16_t*>(out), lse, static_cast<float*>(workspace), static_cast<hipStream_t>(stream));
 }
 
 gpann_status gpann_blocks_weigh(const gpann_blocks_layout* L, const void* q, const void* k, const int32_t* probes, uint32_t nprobe, const float* lse,

@@ -87,7 +87,7 @@ typedef struct gpann_blocks_layout {
     int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
 } gpann_blocks_layout;
 
-/* Bytes of workspace that any of `calls` (GPANN_BLOCKS_ROUTE | ...) needs for this layout; may be 0. */
+/* Bytes of workspace that any of `calls` (GPANN_BLOCKS_ROUTE | ...) needs for this layout; 0 where a call needs none (`workspace` may be NULL then). */
 gpann_status gpann_blocks_workspace_bytes(const gpann_blocks_layout* layout, uint32_t nprobe, uint32_t calls, size_t* out_bytes);
 
 /* Centroids of the blocks that hold one of the last `new_rows` rows of each sequence (0: of all its blocks).  Others stay as they were.

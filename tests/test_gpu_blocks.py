@@ -187,6 +187,26 @@ def test_attend_paged(blocks, kw):
     p.check_attend()
 
 
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("kw", [dict(bs=16, q_heads=6), dict(bs=48, q_heads=2, dtype="fp16"), dict(bs=64, q_heads=80, paged=True), dict(bs=256, q_heads=34, dtype="fp16", causal=False)], ids=str)
+def test_single_tokens_at_every_length(blocks, dim, kw):
+    """one query row a sequence: lengths around the tiles, keys divided over workgroups, pages that end inside a tile, an infinity in the last row"""
+    lens = [0, 1, 15, 16, 17, 47, 49, 700]
+    probes = np.random.default_rng(3).permuted(np.tile(np.arange(44), (8, 1, 2, 1)), axis=-1)[..., :40]
+    probes[..., 0] = 0
+    p = Problem(blocks, seed=19, batch=8, q_rows=1, kv_rows=700, kv_heads=2, dim=dim, kv_len=lens, nprobe=40, probes=probes, **kw)
+    p.attend()
+    torch.cuda.synchronize()
+    p.check_attend()
+    if not p.paged:
+        p.v[1, 0, :, 3], p.v[6, 48, :, 5] = float("inf"), float("inf")      # seen by one sequence's token: its weight is not 0
+        p.attend()
+        torch.cuda.synchronize()
+        assert (p.out[1, 0, :, 3] == float("inf")).all() and torch.isfinite(p.out[1, 0, :, 4:]).all()
+        seen = torch.from_numpy((p.probes_np[6, 0] == 48 // p.bs).any(-1)).repeat_interleave(p.G).cuda()
+        assert torch.equal(p.out[6, 0, :, 5] == float("inf"), seen) and torch.isfinite(p.out[6, 0, :, 6:]).all()
+
+
 def test_pages_that_do_not_exist_are_skipped(blocks):
     p = Problem(blocks, seed=14, paged=True)
     p.table_np[0, 1], p.table_np[1, 2], p.table_np[0, 3] = -1, p.n_pages, -2 ** 31
