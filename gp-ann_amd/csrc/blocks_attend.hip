@@ -652,50 +652,76 @@ __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint
 }
 
 // ---- attention weights of the cache rows ------------------------------------------------------------------------------------------------------
-// One query row per sequence: a cache row gets the weights of one group's heads, from one wavefront of the workgroup that copies the pair's masses.
+// One query row per sequence: a cache row gets the weights of one group's heads, from one wavefront.  `shares` workgroups divide a pair: its probed tiles, whose
+// masses are written with their weights, and the copying of all other rows' masses.
 template <bool BF16, int DC>
-__global__ void __launch_bounds__(512) BlocksWeighTokenKernel(BlocksArgs a, uint32_t mtiles, uint32_t vector, const float* __restrict__ lse, const float* mass_in,
-                                                              float* mass_out) {
+__global__ void __launch_bounds__(512) BlocksWeighTokenKernel(BlocksArgs a, uint32_t mtiles, uint32_t vector, uint32_t shares, const float* __restrict__ lse,
+                                                              const float* mass_in, float* mass_out) {
     TakeWholeRegisterFile();
     constexpr int KS = DC / 2;
-    __shared__ uint32_t s_scratch[8][64];
+    __shared__ uint32_t s_scratch[8][64], s_probed[GPANN_BLOCKS_MAX_BLOCKS / 32];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const uint32_t pair = blockIdx.x, b = pair / a.Hkv, h = pair % a.Hkv;
+    const uint32_t pair = blockIdx.x / shares, share = blockIdx.x % shares, b = pair / a.Hkv, h = pair % a.Hkv;
     const int n = BlocksKvLen(a, b), visible = a.Tq ? BlocksVisible(a, n, BlocksQLen(a, b), 0) : 0;
     const float* from = mass_in + (uint64_t)pair * a.Tk;
     float* to = mass_out + (uint64_t)pair * a.Tk;
-    if (mass_in != mass_out) {
-        if (vector)
-            for (uint32_t i = threadIdx.x * 4; i < a.Tk; i += 2048) *reinterpret_cast<float4*>(to + i) = *reinterpret_cast<const float4*>(from + i);
-        else
-            for (uint32_t i = threadIdx.x; i < a.Tk; i += 512) to[i] = from[i];
+    const bool copies = mass_in != mass_out;
+    if (copies) {
+        s_probed[threadIdx.x] = 0;
         __syncthreads();
     }
-    if (visible == 0) return;
     int block;
     int64_t ko, vo;
-    const uint32_t count = BlocksGatherProbes(a, a.probes + (int64_t)pair * a.P, b, visible, s_scratch[wave], lane, block, ko, vo);
+    const uint32_t count = visible > 0 ? BlocksGatherProbes(a, a.probes + (int64_t)pair * a.P, b, visible, s_scratch[wave], lane, block, ko, vo) : 0;
     const uint32_t tpb = a.bs / 16, units = count * tpb;
     auto load = [&](uint32_t u, u32x4_t(&rows)[KS], int& start, float& before) {   // (clamped behind the last unit: of no use there)
         const uint32_t unit = min(u, units - 1), slot = unit / tpb, base = unit % tpb * 16;
         const int blk = __builtin_amdgcn_readlane(block, (int)slot), last = visible - 1 - blk * (int)a.bs;
         start = blk * (int)a.bs + (int)base;
         BlocksLoadRows<KS>(a.k + BlocksReadLane64(ko, slot) + h * a.ks[2] + min((int)(base + r), last) * a.ks[1] + g * 8, rows);
-        before = from[min(start + (int)(g * 4 + (r & 3)), visible - 1)];
+        before = from[min(start + (int)(g * 4 + (r & 3)), (int)a.Tk - 1)];
     };
-    if (units == 0) return;
     u32x4_t kr[KS], q[KS];
-    int start;
-    float before;
-    load(wave, kr, start, before);
+    int start = 0;
+    float before = 0.f, l0 = 0.f;
     const uint32_t heads0 = min(16u, a.G);
-    BlocksLoadRows<KS>(a.q + b * a.qs[0] + (h * a.G + min(r, heads0 - 1)) * a.qs[2] + g * 8, q);
-    const float l0 = lse[(int64_t)b * a.Hq + h * a.G + min(r, heads0 - 1)];
-    for (uint32_t u = wave; u < units; u += 8) {
+    const uint32_t u0 = share * 8 + wave;
+    if (u0 < units) {
+        load(u0, kr, start, before);
+        BlocksLoadRows<KS>(a.q + b * a.qs[0] + (h * a.G + min(r, heads0 - 1)) * a.qs[2] + g * 8, q);
+        l0 = lse[(int64_t)b * a.Hq + h * a.G + min(r, heads0 - 1)];
+    }
+    if (copies) {
+        if (wave == 0 && lane < count) atomicOr(s_probed + block / 32, 1u << (block & 31));
+        __syncthreads();
+        auto probed = [&](uint32_t row) { return (s_probed[row / a.bs / 32] >> (row / a.bs & 31)) & 1; };
+        // a batch of loads, then their stores (which the compiler has to take for writes to what is loaded next)
+        const uint32_t part = ((a.Tk + shares - 1) / shares + 3) & ~3u, row0 = share * part, rows = min(a.Tk, row0 + part);
+        constexpr uint32_t SOME = 8;
+        if (vector)
+            for (uint32_t i0 = row0 + threadIdx.x * 4; i0 < rows; i0 += 2048 * SOME) {
+                f32x4_t x[SOME];
+#pragma unroll
+                for (uint32_t y = 0; y < SOME; ++y) x[y] = *reinterpret_cast<const f32x4_t*>(from + min(i0 + y * 2048, rows - 4));
+#pragma unroll
+                for (uint32_t y = 0; y < SOME; ++y)
+                    if (i0 + y * 2048 < rows && !probed(i0 + y * 2048)) *reinterpret_cast<f32x4_t*>(to + i0 + y * 2048) = x[y];
+            }
+        else
+            for (uint32_t i0 = row0 + threadIdx.x; i0 < rows; i0 += 512 * SOME) {
+                float x[SOME];
+#pragma unroll
+                for (uint32_t y = 0; y < SOME; ++y) x[y] = from[min(i0 + y * 512, rows - 1)];
+#pragma unroll
+                for (uint32_t y = 0; y < SOME; ++y)
+                    if (i0 + y * 512 < rows && !probed(i0 + y * 512)) to[i0 + y * 512] = x[y];
+            }
+    }
+    for (uint32_t u = u0; u < units; u += 8 * shares) {
         u32x4_t next[KS];
         int next_start;
         float next_before;
-        load(u + 8, next, next_start, next_before);
+        load(u + 8 * shares, next, next_start, next_before);
         f32x4_t w = {0.f, 0.f, 0.f, 0.f};
         for (uint32_t mt = 0; mt < mtiles; ++mt) {
             const uint32_t heads = min(16u, a.G - mt * 16), head = h * a.G + mt * 16 + min(r, heads - 1);
@@ -711,7 +737,7 @@ __global__ void __launch_bounds__(512) BlocksWeighTokenKernel(BlocksArgs a, uint
         for (int i = 0; i < 4; ++i) {
             w[i] = BlocksSumRow16(w[i]);
             const int key = start + (int)g * 4 + i;
-            if ((int)r == i && key < visible) to[key] = before + w[i];
+            if ((int)r == i && key < (copies ? (int)a.Tk : visible)) to[key] = key < visible ? before + w[i] : before;
         }
         start = next_start;
         before = next_before;
@@ -888,7 +914,9 @@ static gpann_status Weigh(const BlocksArgs& a, const float* lse, const float* ma
     const uint64_t pairs = (uint64_t)a.B * a.Hkv;
     if (a.Tq <= 1) {
         const uint32_t vector = a.Tk % 4 == 0 && BlocksAligned(16, mass_in) && BlocksAligned(16, mass_out) ? 1 : 0;
-        return BlocksLaunch(BlocksWeighTokenKernel<BF16, DC>, pairs, 0, st, a, (a.G + 15) / 16, vector, lse, mass_in, mass_out);
+        uint32_t shares = 1;   // a pair is divided until there is a workgroup per CU, or a tile a wavefront
+        while (pairs * shares * 2 <= 256 && shares * 16 <= std::min(a.P, a.nblk) * (a.bs / 16)) shares *= 2;
+        return BlocksLaunch(BlocksWeighTokenKernel<BF16, DC>, pairs * shares, 0, st, a, (a.G + 15) / 16, vector, shares, lse, mass_in, mass_out);
     }
     const uint32_t words = (a.Tq + 31) / 32, pieces = (a.bs + 63) / 64;
     uint32_t* bits = reinterpret_cast<uint32_t*>(ws);

@@ -383,6 +383,13 @@ def test_weigh(blocks, kw, in_place):
     assert np.array_equal(got[~touched], before[~touched])
 
 
+@pytest.mark.parametrize("kw", [dict(kv_rows=1000, kv_len=[1000, 700]), dict(kv_rows=1001, kv_len=[999, 1001], nprobe=20, dtype="fp16", dim=96), dict(kv_rows=3000, bs=256, paged=True)],
+                         ids=str)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_weigh_a_token_divided_over_workgroups(blocks, kw, in_place):
+    test_weigh(blocks, {**dict(q_rows=1, bs=128, nprobe=7), **kw}, in_place)
+
+
 @pytest.mark.parametrize("kw", [dict(keep=50), dict(keep=50, first=4, last=10), dict(keep=1), dict(keep=150), dict(keep=400), dict(keep=149, last=1), dict(keep=7, first=3, last=4),
                                 dict(keep=60, kv_len=[0, 61]), dict(keep=33, paged=True, bs=16, first=1), dict(keep=40, ties=True), dict(keep=40, ties=True, kv_rows=3000, last=5),
                                 dict(keep=2000, kv_rows=5000, dim=256, dtype="fp16", kv_heads=1), dict(keep=900, kv_rows=1024, packed=True)], ids=str)
