@@ -92,13 +92,16 @@ __device__ __forceinline__ float BlocksToFloat(uint16_t x, bool bf16) {
 }
 
 // Workgroup id -> (pair, tile) such that the workgroups of one (sequence, key/value head) pair get ids that are equal modulo 8: workgroups are dealt to
-// the chip's eight dies round robin, so a pair's keys and values stay in one die's L2.  Grid: 8 * ceil(pairs / 8) * tiles; false: nothing to do.
+// the chip's eight dies round robin, so a pair's keys and values stay in one die's L2.  Pairs that are left over when every die has as many as the others go
+// over all dies (12 pairs of 20 tiles: 40 workgroups on four dies of 32 CUs and 20 on the others, or 30 on each).  false: nothing to do.
 __device__ __forceinline__ bool BlocksPairOf(uint32_t id, uint32_t pairs, uint32_t tiles, uint32_t& pair, uint32_t& tile) {
-    const uint32_t lane = id & 7, rest = id >> 3;
-    pair = (rest / tiles) * 8 + lane;
-    tile = rest % tiles;
+    const uint32_t lane = id & 7, rest = id >> 3, own = pairs / 8 * tiles;   // workgroups of pairs of its own that a die has
+    const uint32_t x = rest < own ? rest : (rest - own) * 8 + lane;
+    pair = rest < own ? x / tiles * 8 + lane : pairs / 8 * 8 + x / tiles;
+    tile = x % tiles;
     return pair < pairs;
 }
+inline uint64_t BlocksPairGrid(uint64_t pairs, uint64_t tiles) { return 8 * (pairs / 8 * tiles + (pairs % 8 * tiles + 7) / 8); }
 // bits[sequence, head][block][query row / 32] of the rows that probe a block; every word is written.  A workgroup has kMarkRows query rows and kMarkBlocks blocks
 constexpr uint32_t kMarkRows = 128, kMarkBlocks = 512;
 gpann_status BlocksCheckMarks(const gpann_blocks_layout* L);   // what its grid, and the others of (sequence, head) pairs, have room for
@@ -142,7 +145,5 @@ inline gpann_status BlocksLaunch(K kernel, uint64_t grid, size_t lds, hipStream_
             default: return bf16 ? fn<true, 16>(__VA_ARGS__) : fn<false, 16>(__VA_ARGS__);                                                  \
         }                                                                                                                                   \
     } while (0)
-
-inline uint64_t BlocksPairGrid(uint64_t pairs, uint64_t tiles) { return (pairs + 7) / 8 * 8 * tiles; }
 
 }  // namespace gpann

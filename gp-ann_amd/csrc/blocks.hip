@@ -382,13 +382,14 @@ __global__ void __launch_bounds__(1024) BlocksRouteRowKernel(BlocksArgs a, const
         BlocksSelect<0>(s_key, nb, a.P, first, last, threadIdx.x, out);
 }
 
-// A workgroup per query row and head, or matrix tiles: those hold a workgroup's keys in 128 KB, so with more blocks they would have fewer than four query rows
-static bool BlocksRouteByRow(uint32_t rows, uint32_t blocks) { return rows < 16 || blocks > 128 * 1024 / 8 / 4; }
+// A workgroup per query row and head, or matrix tiles of up to 16 query rows (512 blocks of 128 dimensions: 8 rows of 64 heads 32 us by row, 26 by tiles, 4 rows
+// 22 and 24; 2 rows of 512 heads 30 and 46, 4 rows 48 and 51).  Tiles hold a workgroup's keys in 128 KB: with more blocks they would have fewer than four rows.
+static bool BlocksRouteByRow(uint64_t pairs, uint32_t rows, uint32_t blocks) { return rows < 4 || pairs * rows <= 256 || blocks > 128 * 1024 / 8 / 4; }
 template <bool BF16, int DC>
 static gpann_status Route(const BlocksArgs& a, const float* summary, uint32_t first, uint32_t last, int32_t* probes, hipStream_t st) {
     // keys of a workgroup's query rows in 128 KB; groups are given up while there are not two workgroups per CU
     const uint64_t pairs = (uint64_t)a.B * a.Hkv, room = 128 * 1024 / 8;
-    if (BlocksRouteByRow(a.Tq, a.nblk)) {
+    if (BlocksRouteByRow(pairs, a.Tq, a.nblk)) {
         const size_t lds = (size_t)a.nblk * 8;
         auto kernel = BlocksRouteRowKernel<BF16, DC>;
         if (lds > 32 * 1024) GPANN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
@@ -578,7 +579,7 @@ gpann_status gpann_blocks_route(const gpann_blocks_layout* L, const void* q, con
     GPANN_REQUIRE(nprobe >= 1 && nprobe <= GPANN_BLOCKS_MAX_PROBE, "nprobe must be 1 .. GPANN_BLOCKS_MAX_PROBE");
     GPANN_REQUIRE(first <= nprobe && last <= nprobe - first, "first + last must not exceed nprobe");
     GPANN_REQUIRE(last >= 1 || !(L->flags & GPANN_BLOCKS_CAUSAL), "a causal route needs last >= 1");
-    if (BlocksRouteByRow(L->q_rows, BlocksPerSequence(L))) {
+    if (BlocksRouteByRow((uint64_t)L->batch * L->kv_heads, L->q_rows, BlocksPerSequence(L))) {
         GPANN_REQUIRE((uint64_t)L->batch * L->kv_heads <= 65535, "more than 65535 (sequence, head) pairs");
         GPANN_REQUIRE(L->q_rows < 1u << 22, "2^22 query rows or more over more than 4096 blocks");
     }

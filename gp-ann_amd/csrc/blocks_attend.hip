@@ -882,12 +882,15 @@ struct BlocksDivision {
     }
     size_t Space(uint32_t d) const { return splits > 1 ? BlocksAlign(pairs * tiles * splits * 16 * (d + 2) * 4) : 0; }
 };
-static size_t AttendSpace(const BlocksArgs& a, uint32_t d) { return a.Tq == 1 ? BlocksDivision(a).Space(d) : 0; }
+// ... where it has its wavefronts for itself: with more, neighbours share what they read (8 heads of 128 dimensions, 16 probes of 64 rows: 256 query rows 52 us
+// apart, 68 together, 512 rows 100 and 100; 64 heads: 32 rows 56 and 107, 64 rows 104 and 104, 128 rows 194 and 109)
+static bool BlocksApart(const BlocksArgs& a) { return a.Tq == 1 || (uint64_t)a.B * a.Hkv * a.Tq * ((a.G + 15) / 16) <= 2048; }
+static size_t AttendSpace(const BlocksArgs& a, uint32_t d) { return BlocksApart(a) ? BlocksDivision(a).Space(d) : 0; }
 
 template <bool BF16, int DC>
 static gpann_status Attend(const BlocksArgs& a, uint16_t* out, float* lse, float* ws, hipStream_t st) {
     const uint64_t pairs = (uint64_t)a.B * a.Hkv;
-    if (a.Tq > 1) {
+    if (!BlocksApart(a)) {
         // 32 columns a wavefront read LDS half as often for each, but make half the workgroups (one per CU at a time) of a larger union: 8192 rows x 32 heads,
         // 1024 workgroups of 32 columns, 536 us against 588; 777 rows x 12 heads, 120 workgroups, 152 us against 103.  (Wide heads have no registers for it.)
         if constexpr (DC <= 8)

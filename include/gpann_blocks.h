@@ -32,8 +32,8 @@
  * where they enter a matrix product, so in GPANN_BLOCKS_FP16 those below 2^-25 count as 0 (scale a loss whose gradients are that small).
  *
  * Refused, besides what the arguments' comments say: backward and weigh (of more than one query row) of more than 65535 (sequence, key/value head) pairs or
- * 65535 * 128 query rows; backward of 2^32 - 1 (query row, head) rows; route of fewer than 16 query rows or more than 4096 blocks of more than 65535 pairs
- * or 2^22 query rows; any call of more than 2^23 workgroups (GPANN_ERR_UNSUPPORTED). */
+ * 65535 * 128 query rows; backward of 2^32 - 1 (query row, head) rows; route of fewer than 4 query rows, or over more than 4096 blocks, of more than 65535
+ * pairs or 2^22 query rows; any call of more than 2^23 workgroups (GPANN_ERR_UNSUPPORTED). */
 #ifndef GPANN_BLOCKS_H
 #define GPANN_BLOCKS_H
 
