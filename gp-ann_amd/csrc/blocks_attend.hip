@@ -569,20 +569,18 @@ __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint
         BlocksWalkStage now = {}, next = {};   // of the stages that are multiplied and loaded now
         BlocksWalkSource from = {};
         if (stages) from = walk.Describe(a, w, tab, window, 0, units, col.seen_by_any, next);
-        for (uint32_t s = 0; s + 1 < S::BUFFERS && s < stages; ++s) walk.Load(from, s, lds + s * S::STAGE);
-        uint32_t buf = 0;
+        for (uint32_t s = 0; s < S::GROUP && s < stages; ++s) walk.Load(from, s, lds + s * S::STAGE);
         for (uint32_t s = 0; s < stages; ++s) {
-            const uint32_t ahead = s + S::BUFFERS - 1;
-            if (s % kDescribed == 0) now = next;
-            if (ahead % kDescribed == 0 && ahead < stages) from = walk.Describe(a, w, tab, window, ahead, units, col.seen_by_any, next);
-            if (S::BUFFERS > 2 && s + 1 < stages)
-                BlocksDmaWait<(S::BUFFERS - 2) * S::LOADS>();
-            else
+            const uint32_t ahead = s + S::GROUP, at = lds + s % S::BUFFERS * S::STAGE;
+            if (s % S::GROUP == 0) {
+                if (s % kDescribed == 0) now = next;
+                if (ahead % kDescribed == 0 && ahead < stages) from = walk.Describe(a, w, tab, window, ahead, units, col.seen_by_any, next);
                 BlocksDmaWait<0>();
-            BlocksStageBarrier();   // stage s has landed, and nobody reads stage s - 1 any more
+                BlocksStageBarrier();   // this group has landed, and nobody reads the one before any more
+            }
             bool asked = false;
             auto load = [&]() {
-                if (ahead < stages && !asked) walk.Load(from, ahead, lds + (buf == 0 ? S::BUFFERS - 1 : buf - 1) * S::STAGE);
+                if (ahead < stages && !asked) walk.Load(from, ahead, lds + ahead % S::BUFFERS * S::STAGE);
                 asked = true;
             };
 #pragma unroll 1
@@ -597,10 +595,9 @@ __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint
                     any |= mask[y];
                 }
                 if (any)
-                    BlocksWalkAttend<BF16, DC, CT, NT>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, o, top, sum, load);
+                    BlocksWalkAttend<BF16, DC, CT, NT>(scale2, ad, at + z * S::D * 32, start, mask, col, g * 4, q, o, top, sum, load);
             }
             load();
-            buf = buf + 1 == S::BUFFERS ? 0 : buf + 1;
         }
         __syncthreads();
     }

@@ -345,20 +345,18 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
         BlocksWalkStage now = {}, next = {};   // of the stages that are multiplied and loaded now
         BlocksWalkSource from = {};
         if (stages) from = walk.Describe(a, w, tab, window, 0, units, col.seen_by_any, next);
-        for (uint32_t s = 0; s + 1 < S::BUFFERS && s < stages; ++s) walk.Load(from, s, lds + s * S::STAGE);
-        uint32_t buf = 0;
+        for (uint32_t s = 0; s < S::GROUP && s < stages; ++s) walk.Load(from, s, lds + s * S::STAGE);
         for (uint32_t s = 0; s < stages; ++s) {
-            const uint32_t ahead = s + S::BUFFERS - 1;
-            if (s % kDescribed == 0) now = next;
-            if (ahead % kDescribed == 0 && ahead < stages) from = walk.Describe(a, w, tab, window, ahead, units, col.seen_by_any, next);
-            if (S::BUFFERS > 2 && s + 1 < stages)
-                BlocksDmaWait<(S::BUFFERS - 2) * S::LOADS>();
-            else
+            const uint32_t ahead = s + S::GROUP, at = lds + s % S::BUFFERS * S::STAGE;
+            if (s % S::GROUP == 0) {
+                if (s % kDescribed == 0) now = next;
+                if (ahead % kDescribed == 0 && ahead < stages) from = walk.Describe(a, w, tab, window, ahead, units, col.seen_by_any, next);
                 BlocksDmaWait<0>();
-            BlocksStageBarrier();
+                BlocksStageBarrier();   // this group has landed, and nobody reads the one before any more
+            }
             bool asked = false;
             auto load = [&]() {
-                if (ahead < stages && !asked) walk.Load(from, ahead, lds + (buf == 0 ? S::BUFFERS - 1 : buf - 1) * S::STAGE);
+                if (ahead < stages && !asked) walk.Load(from, ahead, lds + ahead % S::BUFFERS * S::STAGE);
                 asked = true;
             };
 #pragma unroll 1
@@ -374,13 +372,12 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
                 }
                 if (any) {
                     if constexpr (DC > 8)
-                        BlocksWalkQueryGradTight<BF16, DC>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, go, lse2, delta, acc, wk, sds, off, load);
+                        BlocksWalkQueryGradTight<BF16, DC>(scale2, ad, at + z * S::D * 32, start, mask, col, g * 4, q, go, lse2, delta, acc, wk, sds, off, load);
                     else
-                        BlocksWalkQueryGrad<BF16, DC, NT>(scale2, ad, lds + buf * S::STAGE + z * S::D * 32, start, mask, col, g * 4, q, go, lse2, less_delta, acc, wk, sds, off, load);
+                        BlocksWalkQueryGrad<BF16, DC, NT>(scale2, ad, at + z * S::D * 32, start, mask, col, g * 4, q, go, lse2, less_delta, acc, wk, sds, off, load);
                 }
             }
             load();
-            buf = buf + 1 == S::BUFFERS ? 0 : buf + 1;
         }
         __syncthreads();
     }

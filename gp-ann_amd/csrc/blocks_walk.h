@@ -16,8 +16,11 @@ namespace gpann {
 template <int DC>
 struct BlocksWalkShape {
     static constexpr uint32_t D = DC * 16, CPR = D / 8, ROWS = 64, TENSOR = ROWS * D * 2, STAGE = 2 * TENSOR;
-    static constexpr uint32_t BUFFERS = D <= 128 ? 3 : 2, LOADS = CPR / 4;   // LOADS: DMA instructions of a wavefront per stage
-    static constexpr uint32_t WINDOW = D <= 128 ? 1024 : 512;   // blocks that LDS has room for at a time
+    static constexpr uint32_t LOADS = CPR / 4;   // DMA instructions of a wavefront per stage
+    // Stages go in groups, one being multiplied and one on its way: a barrier a group.  (Two stages a group, because a wavefront multiplies few or many of a
+    // stage's tiles, and has to wait for the slowest one at every barrier.)
+    static constexpr uint32_t GROUP = D <= 128 ? 2 : 1, BUFFERS = 2 * GROUP;
+    static constexpr uint32_t WINDOW = D <= 96 ? 1024 : 512;   // blocks that LDS has room for at a time
     static constexpr size_t LDS = (size_t)BUFFERS * STAGE + WINDOW * (sizeof(uint4) + 32 + 4);
 
     // Slot of a row's chunk: an exclusive or with a function of the row.  LDS serves 256 bytes a cycle, so the lanes that it serves together have to lie in
