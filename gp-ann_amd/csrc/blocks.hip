@@ -97,7 +97,8 @@ BlocksArgs BlocksMakeArgs(const gpann_blocks_layout* L, const void* q, const voi
 
 // ---- centroids ------------------------------------------------------------------------------------------------------------------------------
 // One workgroup per (block, head, sequence).  A thread adds eight dimensions of every (256 * 8 / d)-th row in binary64 — sums of 16-bit floats, exact but
-// for exponents that lie more than 2^40 apart — and the row groups are added in LDS, always in the same order.
+// for exponents that lie more than 2^40 apart — and the row groups are added in LDS, always in the same order.  Bound by reading K once: 8192 rows x 8
+// heads of 128 dimensions (17 MB) 6.9 us; the last blocks of 64 sequences 5.6 us, a launch's time.
 template <bool BF16>
 __global__ void __launch_bounds__(256) BlocksSummarizeKernel(BlocksArgs a, uint32_t d, uint32_t new_rows, float* __restrict__ summary) {
     extern __shared__ double s_sum[];   // [row group][d]
@@ -212,7 +213,8 @@ __device__ __forceinline__ void BlocksSelect(const uint64_t* s_key, uint32_t nb,
 // products run on the binary64 matrix instruction (16 x 16 x 4, the vector unit's rate without its operand traffic; C: column l % 16, rows 4 i + l / 16): a
 // wavefront holds the sums of `tokens` <= 16 query rows (lane: row l % 16, every fourth four dimensions) and takes 16 blocks' centroids at a time straight from
 // memory; keys wait in LDS until the wavefronts turn to selecting, a query row each.  A workgroup has `groups` sets of query rows, whose blocks 8 / groups
-// wavefronts divide.
+// wavefronts divide.  8192 query rows x 8 heads of 128 dimensions over up to 128 blocks: 99 us, of which the selection is 49 (rounds of dependent comparisons and
+// scalar counts, two wavefronts a SIMD), the products 28, and reading query rows (67 MB) and centroids 18.
 template <bool BF16, int DC>
 __global__ void __launch_bounds__(512) BlocksRouteKernel(BlocksArgs a, uint32_t groups, uint32_t tokens, uint32_t tiles, const float* __restrict__ summary,
                                                          uint32_t first, uint32_t last, int32_t* __restrict__ probes) {
@@ -318,7 +320,7 @@ __device__ __forceinline__ double BlocksSumOver16(double x) {
 }
 
 // One query row per (sequence, head): a workgroup reads all its blocks' centroids once — bound by that read, so by what is in flight: 64 groups of 16 lanes,
-// four blocks each — and one wavefront selects.
+// four blocks each — and one wavefront selects.  64 sequences of up to 512 blocks, 8 heads of 128 dimensions (110 MB of centroids): 24.5 us, 4.5 TB/s.
 template <bool BF16, int DC>
 __global__ void __launch_bounds__(1024) BlocksRouteRowKernel(BlocksArgs a, const float* __restrict__ summary, uint32_t first, uint32_t last,
                                                              int32_t* __restrict__ probes) {
@@ -414,7 +416,8 @@ __device__ __forceinline__ uint32_t BlocksMassKey(float x) {
 
 constexpr uint32_t kEvictKeys = 32768;   // keys that fit LDS: sequences up to that length are read once
 // One workgroup per (head, sequence).  The smallest key that stays is found eleven, eleven and ten bits at a time: a histogram of the keys that agree with the
-// bits found so far, summed from its top.  Then one pass in row order: keys above it stay, and of those equal to it the lowest rows.
+// bits found so far, summed from its top.  Then one pass in row order: keys above it stay, and of those equal to it the lowest rows.  8 sequences x 8 heads x
+// 32768 rows: 57 us, bound by the six passes' instructions on the 64 CUs that have a head.  (Bins over the span of the keys, equal keys counted at once: 64 us.)
 template <bool HELD>
 __global__ void __launch_bounds__(1024) BlocksEvictSelectKernel(BlocksArgs a, const float* __restrict__ mass, uint32_t keep, uint32_t first, uint32_t last,
                                                                 int32_t* __restrict__ rows, int32_t* __restrict__ count) {
@@ -516,7 +519,7 @@ __global__ void __launch_bounds__(1024) BlocksEvictSelectKernel(BlocksArgs a, co
     });
 }
 
-// 16 bytes of a kept row per thread
+// 16 bytes of a kept row per thread: a copy, at a copy's rate (8 x 8192 rows x 8 heads of 128 dimensions, 537 MB moved: 93 us, 5.8 TB/s)
 __global__ void __launch_bounds__(256) BlocksEvictCopyKernel(BlocksArgs a, uint32_t chunks, uint32_t keep, const int32_t* __restrict__ rows,
                                                              const int32_t* __restrict__ count, const float* __restrict__ mass, uint16_t* __restrict__ k_out,
                                                              uint16_t* __restrict__ v_out, int64_t os0, int64_t os1, int64_t os2, float* __restrict__ mass_out) {

@@ -121,10 +121,11 @@ __device__ __forceinline__ void BlocksAttendStore(const BlocksArgs& a, uint32_t 
     if (lse && g == 0) lse[((int64_t)b * a.Tq + t) * a.Hq + head] = sum == 0.f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
 }
 
-// The form for one query row a sequence: `waves` wavefronts of `splits` workgroups share a query row's keys and join through LDS (and memory).  Rows come to
+// The form for few query rows, each apart: `waves` wavefronts of `splits` workgroups share a query row's keys and join through LDS (and memory).  Rows come to
 // LDS by DMA, whole rows an instruction, into a place of the wavefront's own; from there a step's K, then its V, go to registers, and the next step's follow at
 // once.  (Read from memory as the matrix instruction wants them, 16 bytes of 16 rows side by side, K costs the address unit 64 cycles an instruction instead
-// of 16: 16 x 64 rows for each of 8 heads, 11.0 us that way.)
+// of 16: 8 x 64 rows for each of 8 heads 8.3 us, 10.1 that way.)  Bound by memory in a batch (64 sequences, 32 x 64 rows for each of 8 heads of 128
+// dimensions, 538 MB: 100 us, 5.4 TB/s), by the trips one after the other alone (16 x 64 rows for each of 8 heads: 8.2 us and 3.8 for the join).
 template <int DC>
 struct BlocksTokenShape {
     using W = BlocksWalkShape<DC>;
@@ -363,7 +364,7 @@ __global__ void __launch_bounds__(512) BlocksAttendKernel(BlocksArgs a, uint32_t
     }
 }
 
-// joins the parts of a query row's keys that workgroups had; two neighbouring dimensions of one head a thread
+// joins the parts of a query row's keys that workgroups had; two neighbouring dimensions of one head a thread.  A launch's time, 3.8 us.
 template <bool BF16>
 __global__ void __launch_bounds__(256) BlocksAttendJoinKernel(BlocksArgs a, uint32_t d, uint32_t splits, uint32_t mtiles, uint32_t tiles, const float* __restrict__ sums,
                                                               uint16_t* __restrict__ out, float* __restrict__ lse) {
@@ -513,7 +514,12 @@ __device__ __forceinline__ void BlocksWalkAttend(float scale2, const BlocksWalkA
     }
 }
 
-// NT: tiles taken at a time; NM: of how many blocks they may be
+// The walk of blocks_walk.h with the running maximum and sum of a softmax.  NT: tiles taken at a time; NM: of how many blocks they may be.
+//
+// 8192 query rows of 32 heads, 8 key/value heads of 128 dimensions, 16 probes of 64 rows (125 GFLOP of probed products): 366 us, 342 TFLOP/s.  The matrix cores
+// are busy for 28 % of the cycles, the vector units for 40 %, LDS for 14 %: a wavefront goes through reads, products and weights of a stage one after the other,
+// a SIMD has only two of them (each takes half the register file), and a barrier waits for the one with most to do.  What made it faster was fewer vector
+// instructions (493 -> 383 us), not more overlap inside a wavefront (no difference) or wavefront priorities (none).
 template <bool BF16, int DC, int CT, int NT, int NM>
 __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint32_t tpw, uint32_t mtiles, uint32_t tiles, uint16_t* __restrict__ out,
                                                               float* __restrict__ lse) {
@@ -650,7 +656,8 @@ __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint
 
 // ---- attention weights of the cache rows ------------------------------------------------------------------------------------------------------
 // One query row per sequence: a cache row gets the weights of one group's heads, from one wavefront.  `shares` workgroups divide a pair: its probed tiles, whose
-// masses are written with their weights, and the copying of all other rows' masses.
+// masses are written with their weights, and the copying of all other rows' masses.  Bound by memory in a batch (64 sequences of up to 32768 rows, 32 x 64 of
+// them probed, 8 heads of 128 dimensions, 403 MB: 102 us, 3.9 TB/s); one sequence 7.3 us (28 by a workgroup for each head).
 template <bool BF16, int DC>
 __global__ void __launch_bounds__(512) BlocksWeighTokenKernel(BlocksArgs a, uint32_t mtiles, uint32_t vector, uint32_t shares, const float* __restrict__ lse,
                                                               const float* mass_in, float* mass_out) {
@@ -745,7 +752,8 @@ __global__ void __launch_bounds__(512) BlocksWeighTokenKernel(BlocksArgs a, uint
 
 // Many query rows: a wavefront takes a 64-key piece of a block, lists the query rows that probe it and lets their heads stream past the keys, 16 rows a
 // product with a key per lane column; what a key gets is added in one lane group's registers.  Wavefronts share nothing and go from piece to piece (those of a
-// pair on one die): a piece is two or three dependent trips to memory, so what counts is that eight are always under way on a CU.
+// pair on one die): a piece is two or three dependent trips to memory, so what counts is that eight are always under way on a CU.  8 sequences x 128 query rows,
+// 32 probes of 64 rows in 32768, 8 key/value heads of 128 dimensions: 118 us.
 template <bool BF16, int DC>
 __global__ void __launch_bounds__(512) BlocksWeighKernel(BlocksArgs a, uint32_t words, uint32_t pieces, const uint32_t* __restrict__ bits, const float* __restrict__ lse,
                                                          const float* mass_in, float* mass_out) {
@@ -855,7 +863,6 @@ __global__ void __launch_bounds__(512) BlocksWeighKernel(BlocksArgs a, uint32_t 
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------------------
-constexpr uint32_t kSplitSteps = 2;
 static size_t WeighSpace(const BlocksArgs& a) { return a.Tq <= 1 ? 0 : BlocksAlign((size_t)a.B * a.Hkv * a.nblk * ((a.Tq + 31) / 32) * 4); }
 
 template <bool BF16, int DC, int CT, int NT, int NM>
@@ -865,15 +872,16 @@ static gpann_status AttendWalk(const BlocksArgs& a, uint16_t* out, float* lse, h
     return BlocksLaunch(BlocksAttendWalkKernel<BF16, DC, CT, NT, NM>, BlocksPairGrid((uint64_t)a.B * a.Hkv, tiles), BlocksWalkShape<DC>::LDS, st, a, tpw, mtiles, (uint32_t)tiles, out, lse);
 }
 
-// How a query row's keys are divided where there are few of them: over the wavefronts of a workgroup until the chip's 2048 have something to do, then over
-// workgroups until there is one per CU
+// How a query row's keys are divided where there are few of them: over the wavefronts of a workgroup until the chip's 2048 have something to do, then, where
+// that leaves more than two steps each and there are few of them, over workgroups until there is one per CU (8 heads of 128 dimensions, undivided and divided:
+// 8 x 64 rows 10.0 and 10.1 us, 16 x 64 14.9 and 11.0, 32 x 64 24.1 and 12.8; 64 heads, 32 x 64: 27.3 and 21.8; 128 heads 28.8 and 29.6)
 struct BlocksDivision {
     uint32_t waves = 1, splits = 1, mtiles;
     uint64_t pairs, tiles;
     explicit BlocksDivision(const BlocksArgs& a) : mtiles((a.G + 15) / 16), pairs((uint64_t)a.B * a.Hkv) {
         const uint64_t tasks = (uint64_t)a.Tq * mtiles, units = (uint64_t)std::min(a.P, a.nblk) * (a.bs / 16);
         while (waves < 8 && pairs * tasks * waves < 2048) waves *= 2;
-        if (waves == 8 && units > 16 * kSplitSteps && pairs * tasks <= 64)
+        if (waves == 8 && units > 32 && pairs * tasks <= 64)
             while (pairs * tasks * splits * 2 <= 256 && splits * 16 < units) splits *= 2;
         tiles = (tasks * waves + 7) / 8;
     }
@@ -888,8 +896,9 @@ template <bool BF16, int DC>
 static gpann_status Attend(const BlocksArgs& a, uint16_t* out, float* lse, float* ws, hipStream_t st) {
     const uint64_t pairs = (uint64_t)a.B * a.Hkv;
     if (!BlocksApart(a)) {
-        // 32 columns a wavefront read LDS half as often for each, but make half the workgroups (one per CU at a time) of a larger union: 8192 rows x 32 heads,
-        // 1024 workgroups of 32 columns, 536 us against 588; 777 rows x 12 heads, 120 workgroups, 152 us against 103.  (Wide heads have no registers for it.)
+        // 32 columns a wavefront read LDS half as often for each, but make half the workgroups (one per CU at a time) of a larger union: 32 heads of 128
+        // dimensions, 8192 rows (1024 workgroups of 32 columns) 367 us against 419, 4096 rows (512) 273 and 278, 2048 rows (256) 170 and 162; 777 rows x 12 heads
+        // of 96 (120) 122 and 79.  (Wide heads have no registers for it.)  Pairs of blocks of 32 rows in one chain of products, 777 rows: 79 us against 89.
         if constexpr (DC <= 8)
             if (pairs * (((uint64_t)a.Tq * a.G + 255) / 256) >= 512)
                 return a.bs % 64 == 0   ? AttendWalk<BF16, DC, 2, 4, 1>(a, out, lse, st)
