@@ -187,6 +187,52 @@ def test_attend_paged(blocks, kw):
     p.check_attend()
 
 
+WALKS = [
+    dict(), dict(dim=96, bs=48, dtype="fp16"), dict(dim=128, bs=64), dict(dim=192, bs=16, dtype="fp16"), dict(dim=256, bs=128), dict(q_heads=8, bs=16, dim=128),
+    dict(q_heads=24, bs=64, dtype="fp16"), dict(q_heads=80, kv_heads=4, q_rows=70), dict(q_heads=128, bs=64), dict(causal=False, bs=256, kv_rows=600), dict(scale=-0.2), dict(scale=0.0),
+    dict(packed=True), dict(kv_len=[0, 1, 33, 150, 149, 64, 16, 97], q_len=[40, 40, 3, 40, 0, 17, 40, 33]), dict(paged=True, bs=16, nprobe=9), dict(paged=True, bs=64, dim=128, kv_rows=301),
+    dict(batch=1, kv_heads=1, q_heads=2, q_rows=2100, kv_rows=20000, bs=16, nprobe=5), dict(batch=1, kv_heads=1, q_heads=2, q_rows=2100, kv_rows=9000, bs=16, nprobe=5, dim=128),
+    dict(batch=3, kv_heads=4, q_heads=12, q_rows=300, kv_rows=700, dim=96, dtype="fp16", nprobe=12), dict(batch=16, q_heads=32, q_rows=129, dim=128, bs=64, kv_rows=256),
+    # enough of them for 32 columns a wavefront
+    *(dict(batch=16, kv_heads=16, q_heads=256, q_rows=20, **kw) for kw in (dict(bs=16), dict(dim=96, dtype="fp16"), dict(dim=128, bs=64), dict(dim=128, bs=48, dtype="fp16", causal=False))),
+    dict(batch=16, kv_heads=16, q_heads=640, q_rows=8, bs=64), dict(batch=16, kv_heads=16, q_heads=48, q_rows=90, bs=64, q_len=[90, 3] * 8, kv_len=[150, 149, 64, 65, 1, 0, 33, 96] * 2),
+]
+
+
+@pytest.mark.parametrize("kw", WALKS, ids=lambda x: "-".join(f"{k}{v}" for k, v in x.items()))
+def test_attend_many_rows_together(blocks, kw):
+    """more wavefronts of query rows than the chip has: neighbours walk the blocks that any of them probes"""
+    p = Problem(blocks, **{**dict(seed=71, batch=8, q_rows=40, q_heads=16, kv_heads=8), **kw})
+    p.attend()
+    torch.cuda.synchronize()
+    p.check_attend()
+
+
+@pytest.mark.parametrize("kw", [dict(batch=1, q_heads=128, kv_heads=64), dict(batch=8, q_heads=128, kv_heads=64), dict(batch=32, q_heads=640, kv_heads=16), dict(batch=16, dim=128)], ids=str)
+def test_many_rows_beside_values_that_are_not_numbers(blocks, kw):
+    """as above, with 16 and 32 columns a wavefront"""
+    kw = {**dict(batch=1, q_heads=512, kv_heads=32), **kw}
+    probes = np.full((kw["batch"], 40, kw["kv_heads"], 3), -1, np.int32)
+    probes[:, :, :, 0] = 0
+    probes[:, ::2, :, 1] = 1            # every second row looks at block 1, which holds the values that are none
+    probes[:, :, :, 2] = 4
+    p = Problem(blocks, seed=72, q_rows=40, kv_rows=150, probes=probes, nprobe=3, **kw)
+    p.v[:, 40], p.v[:, 41], p.k[:, 42], p.v[:, 140] = float("inf"), float("nan"), float("nan"), float("inf")   # row 140: seen by the rows from t = 30 on
+    p.attend()
+    torch.cuda.synchronize()
+    out = p.out.double().cpu().numpy()
+    for b, t, h, heads, vis in p.rows():
+        if b not in (0, p.batch - 1) or h % 5:
+            continue
+        want, _, tol, _ = ref.attend(p.q64[b, t, heads], p.k64[b, :, h], p.v64[b, :, h], probes[b, t, h], p.bs, p.nblk, vis, p.scale, p.dtype)
+        if t % 2 == 0:
+            assert np.isnan(out[b, t, heads]).all()
+        elif vis > 140:
+            assert (out[b, t, heads] == np.inf).all()
+        else:
+            assert (np.abs(out[b, t, heads] - want) <= tol).all()
+
+
 @pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
 @pytest.mark.parametrize("kw", [dict(bs=16, q_heads=6), dict(bs=48, q_heads=2, dtype="fp16"), dict(bs=64, q_heads=80, paged=True), dict(bs=256, q_heads=34, dtype="fp16", causal=False)], ids=str)
 def test_single_tokens_at_every_length(blocks, dim, kw):
@@ -335,6 +381,12 @@ def test_route(blocks, kw):
         assert np.array_equal(got[b, t, h], ref.route(p.q64[b, t, heads], cen[b, h], p.bs, vis, p.nprobe, first, last)), (b, t, h)
     for b in range(p.batch):
         assert (got[b, p.m[b]:] == 12345).all()
+
+
+@pytest.mark.parametrize("kw", [dict(dim=96, dtype="fp16"), dict(dim=192, q_heads=8), dict(dim=256, bs=16, q_heads=128), dict(dim=128, q_rows=23, kv_len=[150, 149, 1, 0], q_len=[23, 2, 23, 1]),
+                                dict(kv_rows=9000, bs=16, nprobe=30, q_rows=17), dict(kv_rows=5000, bs=16, nprobe=64, causal=False), dict(paged=True, dim=128, nprobe=5), dict(scale=-1.0)], ids=str)
+def test_route_by_tiles_of_query_rows(blocks, kw):
+    test_route(blocks, {**dict(batch=4, kv_heads=8, q_heads=16, q_rows=9, nprobe=3), **kw})
 
 
 def test_route_ties_and_values_that_are_not_numbers(blocks):
