@@ -16,8 +16,8 @@ namespace gpann {
 // (8192 rows of 128 dimensions in bf16, relative error of dq: 0.0017 is its own rounding, 0.0023 this, 0.0025 with the sum before the rounding, 0.0032
 // uncorrected.  The products for w cost 63 of 720 us.)
 //
-// 8192 query rows of 32 heads, 8 key/value heads of 128 dimensions, 16 probes of 64 rows: the query side takes 569 us (three products, 188 GFLOP: 330 TFLOP/s;
-// with the one for w the matrix cores are busy for 32 % of the cycles) and the key side 469 us (four products, 250 GFLOP: 530 TFLOP/s, 26 %); joining 18,
+// 8192 query rows of 32 heads, 8 key/value heads of 128 dimensions, 16 probes of 64 rows: the query side takes 549 us (three products, 188 GFLOP: 340 TFLOP/s;
+// with the one for w the matrix cores are busy for 33 % of the cycles) and the key side 470 us (four products, 250 GFLOP: 530 TFLOP/s, 26 %); joining 18,
 // counting and marking rows 8 each.  Both are bound as the forward is: two wavefronts a SIMD, whose reads, products and weights overlap little.
 
 // What the key side needs of a (query row, head) row: lse * log2 e (+inf: it weighs nothing) and delta.  Both arrays end with an entry of a row that weighs nothing.
