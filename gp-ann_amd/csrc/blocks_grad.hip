@@ -611,18 +611,19 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
         const BlocksWalkAddresses<DC> ad(lane, hd * OD);
         const uint32_t lds = BlocksLdsAddress(s_keys);
         // Row i of the part: query row list[i / G], head i % G of the group.  A wavefront asks for PER / 8 pieces of 64 / CPR rows of both tensors a stage,
-        // the last one for the rows' numbers too; `place`: what a lane adds to a row's address.
+        // the last one for the rows' numbers too; `place`: what a lane adds to a row's address.  Offsets are in units of 16 bytes: a head's stride, of up to 2^31
+        // elements, then fits 32 bits (in bytes it would not), and the shift is part of the addition to the base.
         constexpr uint32_t PER = S::ROWS * S::CPR / 64, PIECES = (PER + 7) / 8;
         const uint32_t inverse = a.G > 1 ? 0xFFFFFFFFu / a.G + 1 : 0;
         const char* q0 = reinterpret_cast<const char*>(a.q + b * a.qs[0] + (int64_t)h * a.G * a.qs[2]);
         const char* o0 = reinterpret_cast<const char*>(dout + b * a.os[0] + (int64_t)h * a.G * a.os[2]);
-        const uint32_t qrow = (uint32_t)a.qs[1] * 2, orow = (uint32_t)a.os[1] * 2, qhead = (uint32_t)a.qs[2] * 2, ohead = (uint32_t)a.os[2] * 2;
+        const uint32_t qrow = (uint32_t)(a.qs[1] / 8), orow = (uint32_t)(a.os[1] / 8), qhead = (uint32_t)(a.qs[2] / 8), ohead = (uint32_t)(a.os[2] / 8);
         uint32_t piece_row[PIECES], place[PIECES];
 #pragma unroll
         for (uint32_t y = 0; y < PIECES; ++y) {
             const uint32_t at = (wave + 8 * y) * 64 + lane;
             piece_row[y] = at / S::CPR;
-            place[y] = W::Slot(at % S::CPR, piece_row[y] % 16) * 16;
+            place[y] = W::Slot(at % S::CPR, piece_row[y] % 16);
         }
         auto row_of = [&](uint32_t i, uint32_t& t, uint32_t& head) {
             const uint32_t in = inverse ? __umulhi(i, inverse) : i;   // i / G, exact below 2^16
@@ -634,9 +635,9 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
             if (PER % 8 != 0 && j >= PER) return;
             uint32_t t, head;
             row_of(min(s * S::ROWS + piece_row[y], rows - 1), t, head);
-            const uint64_t dq_at = (uint64_t)head * qhead + place[y], do_at = (uint64_t)head * ohead + place[y];
-            BlocksDmaFrom(q0 + ((uint64_t)t * qrow + dq_at), to + j * 1024);
-            BlocksDmaFrom(o0 + ((uint64_t)t * orow + do_at), to + S::TENSOR + j * 1024);
+            const uint64_t q_at = (uint64_t)head * qhead + place[y], o_at = (uint64_t)head * ohead + place[y];
+            BlocksDmaFrom(q0 + (((uint64_t)t * qrow + q_at) << 4), to + j * 1024);
+            BlocksDmaFrom(o0 + (((uint64_t)t * orow + o_at) << 4), to + S::TENSOR + j * 1024);
         };
         auto load_info = [&](uint32_t s, uint32_t to) {
             if (wave != 7) return;
