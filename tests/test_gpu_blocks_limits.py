@@ -1,8 +1,10 @@
 """GPU: where the block operators' ranges end — values that are not numbers in rows a key is hidden from, weights and gradients at the ends of
 binary16, log-sum-exps of more keys than a call's, strides and sizes beyond the usual ones — against their definitions in binary64."""
+import numpy as np
 import pytest
 import torch
 
+import blocks_ref as ref
 from test_gpu_blocks import Problem
 
 pytestmark = pytest.mark.gpu
@@ -12,6 +14,114 @@ pytestmark = pytest.mark.gpu
 def blocks(gp):
     from pygpann import blocks
     return blocks
+
+
+def formula(p, b, t, h, heads, vis, out, lse, probes):
+    """A query row's gradients as the header's formula has them, from a given out and lse, and their bounds without the rounding of the results.
+
+    E = 2^-24, u = half a step of the type, s = half the smallest step of binary16 (2^-25) or 0.  A logit is off by (d + 4) E a, a = |scale| sum |q_i k_i| at most, and
+    a weight by w = 2 (d + 4) E a + 8 E + 4 E |lse| of itself (exponent's argument and lse * log2 e); dp and delta by (d + 2) E of the sums of their terms' sizes.
+    delta may be corrected for the rounding of out: by no more than 1.25 u sum |dout out| (+ s sum |dout|), what that rounding can have come to and a quarter more.
+    p and ds are rounded once, to u of themselves or s; sums of n terms in binary32 add n E of the terms' sizes."""
+    u, s, d = ref.U[p.dtype], 2.0 ** -25 if p.dtype == "fp16" else 0.0, p.dim
+    rows = ref.rows_of(probes[b, t, h], p.bs, p.nblk, vis)
+    q, k, v, do = p.q64[b, t, heads], p.k64[b, rows, h], p.v64[b, rows, h], p.do64[b, t, heads]
+    o, l = out[b, t, heads], lse[b, t, heads]
+    if len(rows) == 0:
+        return rows, np.zeros_like(q), None, None, np.zeros_like(q), None, None
+    a = abs(p.scale) * (np.abs(q) @ np.abs(k).T)
+    w = 2 * (d + 4) * ref.E * a + 8 * ref.E + 4 * ref.E * np.abs(l)[:, None]
+    pr = np.exp(p.scale * (q @ k.T) - l[:, None])
+    delta = (do * o).sum(1, keepdims=True)
+    ds = pr * (do @ v.T - delta)
+    off = 1.25 * u * (np.abs(do) * np.abs(o)).sum(1, keepdims=True) + s * np.abs(do).sum(1, keepdims=True)
+    dp_err = (d + 2) * ref.E * (np.abs(do) @ np.abs(v).T + (np.abs(do) * np.abs(o)).sum(1, keepdims=True)) + off
+    ds_err = pr * (1 + w) * dp_err + (w + u + 2 * ref.E) * np.abs(ds) + s
+    n = len(rows)
+    return (rows, p.scale * (ds @ k), p.scale * (ds.T @ q), pr.T @ do, abs(p.scale) * ((ds_err + n * ref.E * np.abs(ds)) @ np.abs(k)),
+            abs(p.scale) * (ds_err.T @ np.abs(q)), ((w + u) * pr).T @ np.abs(do))
+
+
+def check_gradients(p, probes=None, but=(), hidden=None):
+    """dq, dk and dv against the formula.  `but`: query rows (sequence, row) that take no part; `hidden` [batch][key][kv head]: the keys whose dk, dv are compared"""
+    u, tiny = ref.U[p.dtype], 2.0 ** -25 if p.dtype == "fp16" else 0.0
+    probes = p.probes_np if probes is None else probes
+    out, lse = p.out.double().cpu().numpy(), p.lse.double().cpu().numpy()
+    got = {x: getattr(p, x).double().cpu().numpy() for x in ("dq", "dk", "dv")}
+    want, tol = ({x: np.zeros(y.shape) for x, y in got.items()} for _ in range(2))
+    size, terms = {x: np.zeros(got[x].shape) for x in ("dk", "dv")}, np.zeros(got["dk"].shape[:3])
+    take = {"dq": np.ones(got["dq"].shape, bool), "dk": np.ones(got["dk"].shape, bool), "dv": np.ones(got["dv"].shape, bool)}
+    for b, t, h, heads, vis in p.rows():
+        if (b, t) in but:
+            take["dq"][b, t] = False
+            continue
+        rows, dq, dk, dv, eq, ek, ev = formula(p, b, t, h, heads, vis, out, lse, probes)
+        want["dq"][b, t, heads], tol["dq"][b, t, heads] = dq, eq
+        if len(rows):
+            for x, y, e in (("dk", dk, ek), ("dv", dv, ev)):
+                want[x][b, rows, h] += y
+                tol[x][b, rows, h] += e
+                size[x][b, rows, h] += np.abs(y) + e
+            terms[b, rows, h] += p.G
+    for x in ("dk", "dv"):
+        tol[x] += (terms[..., None] + 8) * ref.E * size[x]       # binary32 sums over query rows and heads
+        if hidden is not None:
+            take[x] &= hidden[..., None]
+    for x in got:
+        bound = tol[x] + u * (np.abs(want[x]) + tol[x]) + tiny
+        bad = ~(np.abs(got[x] - want[x]) <= bound) & take[x]
+        assert not bad.any(), (x, np.argwhere(bad)[:4], got[x][bad][:4], want[x][bad][:4], bound[bad][:4])
+        assert take[x].any()
+
+
+def not_seen_by(p, rows):
+    """[batch][key][kv head]: keys that none of these query rows looks at"""
+    hidden = np.ones(p.k64.shape[:3], bool)
+    for b, t, h, heads, vis in p.rows():
+        if (b, t) in rows:
+            hidden[b, ref.rows_of(p.probes_np[b, t, h], p.bs, p.nblk, vis), h] = False
+    return hidden
+
+
+# ---- gradients: rows that a key is hidden from -------------------------------------------------------------------------------------------------
+HIDDEN = [dict(), dict(dim=128, bs=64), dict(dim=96, bs=16, dtype="fp16"), dict(dim=192, dtype="fp16", bs=48), dict(dim=256, bs=128), dict(q_heads=40, kv_heads=2, bs=32, dtype="fp16"),
+          dict(q_heads=1, kv_heads=1, bs=256, scale=-0.2), dict(causal=False, bs=64), dict(q_rows=300, kv_rows=320, kv_len=[310], q_heads=32, kv_heads=1, bs=64, middle=(250, 262))]
+
+
+@pytest.mark.parametrize("kw", HIDDEN, ids=str)
+@pytest.mark.parametrize("where", ["middle", "last"])
+def test_rows_that_are_not_numbers_leave_the_keys_alone_that_they_do_not_see(blocks, kw, where):
+    """an infinity in one query row's dout and a NaN in another's q, both in the middle of a block, or an infinity in the last row of all: the keys behind them in their
+    blocks, and the cache's rows behind the sequence, have the gradients of the other query rows"""
+    kw = dict(kw)
+    middle = kw.pop("middle", (5, 9))
+    kw = {**dict(seed=81, batch=1, q_rows=40, kv_rows=160, kv_len=[150], nprobe=3), **kw}
+    bs, n = kw.get("bs", 32), kw["kv_len"][0]
+    probes = np.random.default_rng(5).integers(-1, -(-kw["kv_rows"] // bs) + 1, size=(1, kw["q_rows"], kw.get("kv_heads", 2), 3))
+    probes[..., 0], probes[..., 1] = (n - 1) // bs, max(0, (n - 1) // bs - 1)
+    for t in middle:
+        probes[0, t, :, 2] = (n - kw["q_rows"] + t) // bs          # its own block
+    p = Problem(blocks, probes=probes, **kw)
+    if where == "last":
+        rows = [(0, p.q_rows - 1)]
+        p.dout[0, -1, -1, 0] = -float("inf")
+    else:
+        rows = [(0, t) for t in middle]
+        p.dout[0, middle[0], :, 3] = float("inf")
+        p.q[0, middle[1], :, 7] = float("nan")
+    p.attend()
+    p.backward()
+    torch.cuda.synchronize()
+    check_gradients(p, but=rows, hidden=not_seen_by(p, rows))
+    assert (p.dk[0, n:] == 0).all() and (p.dv[0, n:] == 0).all()
+    if where == "middle":         # as the formula has it
+        assert torch.isnan(p.dq[0, middle[1]]).all()
+        seen = torch.from_numpy(~not_seen_by(p, rows[1:])).cuda()
+        assert torch.isnan(p.dk[seen]).all() and torch.isnan(p.dv[seen]).all()
+    first = [x.clone() for x in (p.dq, p.dk, p.dv)]
+    p.backward()
+    for x, y in zip(first, (p.dq, p.dk, p.dv)):
+        assert torch.equal(x.view(torch.int16), y.view(torch.int16))
 
 
 # ---- strides and sizes --------------------------------------------------------------------------------------------------------------------------
