@@ -41,7 +41,9 @@ __device__ __forceinline__ float BlocksDelta(const uint16_t* out, const u32x4_t 
     return BlocksSumOver4(delta);
 }
 
-// One query row's heads (columns r < heads), its probed rows straight from memory: the way out for rows whose neighbours' values are not finite.
+// One query row's heads (columns r < heads), its probed rows straight from memory: the way out for rows whose neighbours' values are not finite, and for those with
+// a ds that binary16 cannot hold (above 65504, where the gradients may well be in range): a column's ds are taken in units of a power of two that follows their
+// largest, as the sums are when it grows.
 template <bool BF16, int DC>
 __device__ __forceinline__ void BlocksQueryGradRow(const BlocksArgs& a, uint32_t b, uint32_t h, uint32_t t, uint32_t head, bool live, int visible, uint32_t lane,
                                                    uint32_t* scratch, const uint16_t* out, const uint16_t* dout, const float* lse, uint16_t* dq, BlocksRowInfo rows) {
@@ -59,6 +61,7 @@ __device__ __forceinline__ void BlocksQueryGradRow(const BlocksArgs& a, uint32_t
     f32x4_t acc[DC];
 #pragma unroll
     for (int d = 0; d < DC; ++d) acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float down = 1.f;   // units of the column's ds and sums: 1 / down
     const uint32_t tpb = a.bs / 16, units = count * tpb;
     BlocksCursor c(0, tpb);
     for (uint32_t u = 0; u < units; u += 2) {
@@ -91,17 +94,38 @@ __device__ __forceinline__ void BlocksQueryGradRow(const BlocksArgs& a, uint32_t
             if (x == 0 && second) c.Next();
         }
         c.Next();
+        if constexpr (!BF16) {
+            float most = 0.f;   // (a NaN is passed over)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(s[0][i]), fabsf(s[1][i])));
+            most = BlocksMaxOver4(most);
+            if (__ballot(most * down >= 32768.f)) {
+                const uint32_t e = __float_as_uint(most) >> 23;   // 2^(e - 127) <= most < 2^(e - 126)
+                const float to = most * down >= 32768.f && e < 255 ? __uint_as_float((268 - e) << 23) : down, f = to / down;   // most * to: 2^14 .. 2^15
+                down = to;
+#pragma unroll
+                for (int d = 0; d < DC; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[d][i] *= f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[0][i] *= down;
+                s[1][i] *= down;
+            }
+        }
         const u32x4_t ds = BlocksPackOperand<BF16>(s[0], s[1]);
 #pragma unroll
         for (int d = 0; d < DC; ++d) acc[d] = BlocksMfma<BF16>(BlocksColumn<N>(kc, d), ds, acc[d]);
     }
     if (!live) return;
     uint16_t* dst = dq + b * a.qs[0] + (int64_t)t * a.qs[1] + head * a.qs[2];
+    const float scale = a.scale / down;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         uint32_t w[N];
 #pragma unroll
-        for (int x = 0; x < N; ++x) w[x] = BlocksPack<BF16>(acc[2 * x][i] * a.scale, acc[2 * x + 1][i] * a.scale);
+        for (int x = 0; x < N; ++x) w[x] = BlocksPack<BF16>(acc[2 * x][i] * scale, acc[2 * x + 1][i] * scale);
         BlocksStoreColumns<N>(dst + (g * 4 + i) * DC, w);
     }
     if (g == 0) {
@@ -532,7 +556,7 @@ struct BlocksKeyShape {
 
 // A wavefront's sums once more, 16 keys (a lane's own: `key`, as its column of the products) and dimensions dim0 .. of the rows first .. first + 31, first + step ..:
 // in binary32, row by row, and only of rows that see the key.  In the products a row that does not is a weight 0, and 0 times a value that is not finite is none
-// that belongs there; so a wavefront whose sums are not finite comes here.  (8192 rows of 32 heads of 128 dimensions, the whole training step: 1.4 ms, with an
+// that belongs there; and a ds above 65504 is an infinity in binary16.  So a wavefront whose sums are not finite comes here.  (8192 rows of 32 heads of 128 dimensions, the whole training step: 1.4 ms, with an
 // infinity in one row's dout 3.6 ms, in every row's 12.1 ms.)
 template <bool BF16, int DC, int OD>
 __device__ __forceinline__ void BlocksKeyGradAgain(const BlocksArgs& a, uint32_t b, uint32_t h, int n, int m, const uint32_t* list, uint32_t rows, uint32_t first, uint32_t step,
