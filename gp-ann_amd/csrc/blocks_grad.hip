@@ -834,6 +834,11 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
             else
                 turned_of(stage, S::TENSOR, ot);
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (!BF16)   // a weight is at most 1 and 2^-14 is the least that binary16 holds in full: as it is, those of a few thousand rows would be lost
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[y][i] *= 32768.f;
             const u32x4_t po = BlocksPackOperand<BF16>(p[0], p[1]);
             dso = BlocksPackOperand<BF16>(ds[0], ds[1]);
             product(f1, vf, ds1);
@@ -862,6 +867,11 @@ __global__ void __launch_bounds__(512) BlocksKeyGradKernel(BlocksArgs a, uint32_
             }
         }
         if constexpr (!TIGHT) add_keys();
+        if constexpr (!BF16)
+#pragma unroll
+            for (int d = 0; d < OD; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) av[d][i] *= 1.f / 32768.f;
     }
     if (works) {
         float bad = 0.f;

@@ -158,6 +158,27 @@ def test_gradients_whose_terms_binary16_cannot_hold(blocks, kw):
     assert most > 65520          # the case is what it says
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(dim=128, bs=32), dict(dim=256, bs=128), dict(q_rows=300, kv_rows=2000, q_heads=32, kv_heads=1, bs=256, nprobe=8)], ids=str)
+def test_values_gradients_of_weights_that_binary16_cannot_hold(blocks, kw):
+    """one key has nearly all the weight of every row, the others about 2^-26 each: their dv is a sum of such"""
+    kw = {**dict(seed=83, batch=1, q_rows=64, kv_rows=1000, q_heads=4, kv_heads=2, bs=64, nprobe=16, dtype="fp16", strength=0.5), **kw}
+    p = Problem(blocks, **kw)
+    p.probes_np[...] = np.arange(p.nprobe)
+    p.probes.copy_(torch.from_numpy(p.probes_np))
+    for x, y in ((p.q, p.q64), (p.k, p.k64)):
+        x[..., 0], y[..., 0] = 0, 0
+    p.q[..., 0], p.q64[..., 0] = 16, 16
+    lift = 18.0 / (16 * p.scale)            # (e^-18 = 2^-26; the type's nearest number)
+    p.k[:, 0, :, 0] = lift
+    p.k64[:, 0, :, 0] = float(p.k[0, 0, 0, 0])
+    scaled(p, dout=2.0 ** 11)
+    p.attend()
+    p.backward()
+    torch.cuda.synchronize()
+    check_gradients(p)
+    assert (p.dv != 0).float().mean() > 0.5
+
+
 # ---- strides and sizes --------------------------------------------------------------------------------------------------------------------------
 def test_gradients_of_heads_that_lie_as_far_apart_as_a_layout_allows(blocks):
     """q, out and their gradients with a head stride of 2^31 elements"""
