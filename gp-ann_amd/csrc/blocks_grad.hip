@@ -13,6 +13,8 @@ namespace gpann {
 // delta = <dout, out> is what every dp is measured against; `out` was rounded, so it is off by e, the same for all of a row's keys.  The walk therefore sums
 // ds' = p (dp - delta'), which is e in all, and w = sum p k beside dq' = sum ds' k: the gradient at the true delta is dq' - e w (the weights sum to 1).  Taken
 // with the sum of the ds' as they were rounded for the product, that is sum ds' (k - w): the roundings then weigh k - w, not k.  The key side gets delta' + e.
+// Where ds' sums to more than rounding can have done, `out` and `lse` are not of these keys alone (attention joined over several calls, whose gradients are taken
+// from the joined ones): there is no such e, and nothing is corrected.
 // (8192 rows of 128 dimensions in bf16, relative error of dq: 0.0017 is its own rounding, 0.0023 this, 0.0025 with the sum before the rounding, 0.0032
 // uncorrected.  The products for w cost 63 of 720 us.)
 //
@@ -26,18 +28,23 @@ struct BlocksRowInfo {
     float* delta;
 };
 
+// <dout, out>, and the most that rounding `out` to its type can have moved it by: half a step of every term (1.25: of which the sums' own roundings are a part)
 template <bool BF16, int DC>
-__device__ __forceinline__ float BlocksDelta(const uint16_t* out, const u32x4_t (&go)[DC / 2]) {
+__device__ __forceinline__ float BlocksDelta(const uint16_t* out, const u32x4_t (&go)[DC / 2], float& slack) {
     u32x4_t y[DC / 2];
     BlocksLoadRows<DC / 2>(out, y);
-    float delta = 0.f;
+    float delta = 0.f, size = 0.f;
 #pragma unroll
     for (int s = 0; s < DC / 2; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            delta += BlocksToFloat((uint16_t)y[s][i], BF16) * BlocksToFloat((uint16_t)go[s][i], BF16);
-            delta += BlocksToFloat((uint16_t)(y[s][i] >> 16), BF16) * BlocksToFloat((uint16_t)(go[s][i] >> 16), BF16);
+            const float lo = BlocksToFloat((uint16_t)y[s][i], BF16) * BlocksToFloat((uint16_t)go[s][i], BF16);
+            const float hi = BlocksToFloat((uint16_t)(y[s][i] >> 16), BF16) * BlocksToFloat((uint16_t)(go[s][i] >> 16), BF16);
+            delta += lo;
+            delta += hi;
+            size += fabsf(lo) + fabsf(hi);
         }
+    slack = BlocksSumOver4(size) * (BF16 ? 1.25f / 256.f : 1.25f / 2048.f);
     return BlocksSumOver4(delta);
 }
 
@@ -55,7 +62,8 @@ __device__ __forceinline__ void BlocksQueryGradRow(const BlocksArgs& a, uint32_t
     u32x4_t q[KS], go[KS];
     BlocksLoadRows<KS>(a.q + b * a.qs[0] + t * a.qs[1] + head * a.qs[2] + g * 8, q);
     BlocksLoadRows<KS>(dout + b * a.os[0] + t * a.os[1] + head * a.os[2] + g * 8, go);
-    const float delta = BlocksDelta<BF16, DC>(out + b * a.os[0] + t * a.os[1] + head * a.os[2] + g * 8, go);
+    float slack;
+    const float delta = BlocksDelta<BF16, DC>(out + b * a.os[0] + t * a.os[1] + head * a.os[2] + g * 8, go, slack);
     const int64_t row = ((int64_t)b * a.Tq + t) * a.Hq + head;
     const float l = lse[row], lse2 = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;
     f32x4_t acc[DC];
@@ -323,6 +331,7 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
     constexpr int KS = DC / 2;
     extern __shared__ __attribute__((aligned(1024))) char s_walk[];
     __shared__ uint32_t s_count, s_scratch[8][64];
+    __shared__ float s_slack[8][16];
     const BlocksWalkTables<DC> tab(s_walk);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     uint32_t pair, tile;
@@ -356,7 +365,9 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
     if (a.scale2 <= 0.f)
 #pragma unroll
         for (int s = 0; s < KS; ++s) q[s] = a.scale2 == 0.f ? u32x4_t{0u, 0u, 0u, 0u} : q[s] ^ 0x80008000u;
-    float delta = BlocksDelta<BF16, DC>(out + at_o, go);
+    float slack;
+    float delta = BlocksDelta<BF16, DC>(out + at_o, go, slack);
+    if (g == 0) s_slack[wave][r] = slack;   // (wanted after the walk: a register less in it)
     const int64_t row = ((int64_t)w.b * a.Tq + col.Row(w, 0)) * a.Hq + col.head[0];
     const float l = lse[row], lse2 = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;   // an empty row weighs nothing
     const BlocksWalkAddresses<DC> ad(lane);
@@ -415,11 +426,14 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
     }
     off = BlocksSumOver4(off);
     float bad = off * 0.f;
+    BlocksWaveSync();
+    const bool own = fabsf(off) <= s_slack[wave][r];   // what the rounding of `out` explains; else `out` and `lse` are of more keys than these
+    const float e = own ? sds[0] : 0.f;
 #pragma unroll
     for (int d = 0; d < DC; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            acc[d][i] -= sds[0] * wk[d][i];
+            acc[d][i] -= e * wk[d][i];
             bad += acc[d][i] * 0.f;
         }
     if (__ballot(bad != 0.f)) {   // as in the forward: a value that is not finite may have met a weight 0
@@ -437,7 +451,7 @@ __global__ void __launch_bounds__(512) BlocksQueryGradKernel(BlocksArgs a, uint3
             u32x2_t{BlocksPack<BF16>(acc[d][0] * a.scale, acc[d][1] * a.scale), BlocksPack<BF16>(acc[d][2] * a.scale, acc[d][3] * a.scale)};
     if (g == 0) {
         info.lse2[row] = lse2;
-        info.delta[row] = delta + off;
+        info.delta[row] = own ? delta + off : delta;
     }
 }
 

@@ -108,7 +108,9 @@ gpann_status gpann_blocks_route(const gpann_blocks_layout* layout, const void* q
 gpann_status gpann_blocks_attend(const gpann_blocks_layout* layout, const void* q, const void* k, const void* v, const int32_t* probes, uint32_t nprobe,
                                  void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Gradients of gpann_blocks_attend, from its out and lse.  Contiguous caches only.  Every sum has one order: results repeat bit for bit. */
+/* Gradients of gpann_blocks_attend, from its out and lse, or this call's part of the gradients of attention that was joined over several calls (other probes,
+ * other rows of a longer cache), from the joined out and lse.  <dout, out> is corrected for the rounding of out where the weights' own sum tells it, by 1.25
+ * times what that rounding can have come to at most.  Contiguous caches only.  Every sum has one order: results repeat bit for bit. */
 gpann_status gpann_blocks_attend_backward(const gpann_blocks_layout* layout, const void* q, const void* k, const void* v, const int32_t* probes,
                                           uint32_t nprobe, const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv,
                                           void* workspace, size_t workspace_bytes, void* stream);

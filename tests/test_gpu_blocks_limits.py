@@ -179,6 +179,31 @@ def test_values_gradients_of_weights_that_binary16_cannot_hold(blocks, kw):
     assert (p.dv != 0).float().mean() > 0.5
 
 
+# ---- gradients from the out and lse of more keys than the call's -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("kw", [dict(), dict(dim=128, bs=64, kv_rows=400, dtype="fp16"), dict(dim=192, bs=16), dict(dim=256, q_heads=20, kv_heads=1), dict(causal=False, q_heads=2, kv_heads=2)], ids=str)
+def test_gradients_of_two_calls_whose_attention_was_joined(blocks, kw):
+    """two probe lists, their outs and log-sum-exps joined, each call's gradients from the joined ones: the header's formula for either"""
+    p = Problem(blocks, **{**dict(seed=84, batch=2, q_rows=40, kv_rows=150, nprobe=8), **kw})
+    lists = [np.full_like(p.probes_np, -1) for _ in range(2)]
+    for j in range(min(16, p.nblk)):
+        lists[j % 2][..., j // 2] = j
+    outs, lses = [], []
+    for probes in lists:
+        p.probes.copy_(torch.from_numpy(probes))
+        p.attend()
+        outs.append(p.out.double())
+        lses.append(p.lse.double())
+    lse = torch.logaddexp(*lses)
+    out = sum((l - lse).exp().nan_to_num(0.0)[..., None] * o for l, o in zip(lses, outs))
+    p.lse.copy_(lse)
+    p.out.copy_(out)
+    for probes in lists:
+        p.probes.copy_(torch.from_numpy(probes))
+        p.backward()
+        torch.cuda.synchronize()
+        check_gradients(p, probes=probes)
+
+
 # ---- strides and sizes --------------------------------------------------------------------------------------------------------------------------
 def test_gradients_of_heads_that_lie_as_far_apart_as_a_layout_allows(blocks):
     """q, out and their gradients with a head stride of 2^31 elements"""
