@@ -520,11 +520,11 @@ __global__ void __launch_bounds__(1024) BlocksEvictSelectKernel(BlocksArgs a, co
 }
 
 // 16 bytes of a kept row per thread: a copy, at a copy's rate (8 x 8192 rows x 8 heads of 128 dimensions, 537 MB moved: 93 us, 5.8 TB/s)
-__global__ void __launch_bounds__(256) BlocksEvictCopyKernel(BlocksArgs a, uint32_t chunks, uint32_t keep, const int32_t* __restrict__ rows,
+__global__ void __launch_bounds__(256) BlocksEvictCopyKernel(BlocksArgs a, uint32_t chunks, uint32_t keep, uint32_t kept, const int32_t* __restrict__ rows,
                                                              const int32_t* __restrict__ count, const float* __restrict__ mass, uint16_t* __restrict__ k_out,
                                                              uint16_t* __restrict__ v_out, int64_t os0, int64_t os1, int64_t os2, float* __restrict__ mass_out) {
     const uint32_t b = blockIdx.y;
-    const uint64_t all = (uint64_t)keep * a.Hkv * chunks;
+    const uint64_t all = (uint64_t)kept * a.Hkv * chunks;   // (slots that a sequence of this layout can fill: keep may be far more)
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
         const uint32_t c = (uint32_t)(i % chunks), h = (uint32_t)(i / chunks % a.Hkv), r = (uint32_t)(i / chunks / a.Hkv);
         const int64_t pair = (int64_t)b * a.Hkv + h;
@@ -629,7 +629,7 @@ gpann_status gpann_blocks_evict(const gpann_blocks_layout* L, const void* k, con
     const uint64_t threads = (uint64_t)kept * a.Hkv * chunks;
     int64_t zero[3] = {0, 0, 0};
     const int64_t* os = out_kv_stride ? out_kv_stride : zero;
-    hipLaunchKernelGGL(BlocksEvictCopyKernel, dim3((uint32_t)std::min<uint64_t>((threads + 255) / 256, 1u << 20), a.B), dim3(256), 0, st, a, chunks, keep, rows, count, mass,
+    hipLaunchKernelGGL(BlocksEvictCopyKernel, dim3((uint32_t)std::min<uint64_t>((threads + 255) / 256, 1u << 20), a.B), dim3(256), 0, st, a, chunks, keep, kept, rows, count, mass,
                        static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out), os[0], os[1], os[2], mass_out);
     GPANN_HIP_TRY(hipGetLastError());
     return GPANN_OK;

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import blocks_ref as ref
-from test_gpu_blocks import Problem
+from test_gpu_blocks import SENTINEL, Problem
 
 pytestmark = pytest.mark.gpu
 
@@ -227,3 +227,22 @@ def test_gradients_of_heads_that_lie_as_far_apart_as_a_layout_allows(blocks):
     p.check_attend()
     p.check_backward()
     assert torch.equal(p.q, tensors["q"]) and torch.equal(p.dout, tensors["dout"])
+
+
+def test_an_eviction_that_could_keep_far_more_than_there_is(blocks):
+    """keep = 2^24 of 64 rows: a launch's work is that of the rows"""
+    p = Problem(blocks, seed=86, batch=1, kv_rows=64, kv_heads=1, q_heads=1)
+    keep = 1 << 24
+    mass = torch.rand(1, 1, 64, device="cuda")
+    rows, mass_out = torch.full((1, 1, keep), -5, dtype=torch.int32, device="cuda"), torch.full((1, 1, keep), SENTINEL, device="cuda")
+    count = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    call = lambda: blocks.evict(p.L, None, None, mass.data_ptr(), keep, rows.data_ptr(), count.data_ptr(), mass_out=mass_out.data_ptr(), **p.space)
+    call()
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    start.record()
+    call()
+    end.record()
+    torch.cuda.synchronize()
+    assert count.item() == 64 and rows[0, 0, :64].tolist() == list(range(64)) and (rows[0, 0, 64:] == -5).all()
+    assert torch.equal(mass_out[0, 0, :64], mass[0, 0]) and (mass_out[0, 0, 64:] == SENTINEL).all()
+    assert start.elapsed_time(end) < 3.0      # ms; two launches take hundredths of one, a loop over 2^24 slots by 512 threads hundreds
