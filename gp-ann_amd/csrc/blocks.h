@@ -121,12 +121,16 @@ inline gpann_status BlocksCheckWorkspace(const void* p, size_t have, size_t need
 }
 
 // workgroups of 512 threads
-template <typename K, typename... A>
-inline gpann_status BlocksLaunch(K kernel, uint64_t grid, size_t lds, hipStream_t st, A... args) {
+inline gpann_status BlocksCheckGrid(uint64_t grid) {
     if (grid > 0x7fffffffull / 512 * 2) {   // (a launch has fewer than 2^32 threads)
         SetLastError("the call needs %llu workgroups of 512 threads", (unsigned long long)grid);
         return GPANN_ERR_UNSUPPORTED;
     }
+    return GPANN_OK;
+}
+template <typename K, typename... A>
+inline gpann_status BlocksLaunch(K kernel, uint64_t grid, size_t lds, hipStream_t st, A... args) {
+    GPANN_TRY(BlocksCheckGrid(grid));
     if (lds > 32 * 1024) GPANN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(512), lds, st, args...);
     GPANN_HIP_TRY(hipGetLastError());

@@ -999,10 +999,12 @@ BackwardSpace BackwardLayout(const BlocksArgs& a, uint32_t d) {
     return s;
 }
 
+uint32_t KeyGroups(const BlocksArgs& a) { return (a.bs / 16 + 3) / 4; }   // workgroups of 64 keys that a block has
+
 template <bool BF16, int DC, int ND, int RGS>
 gpann_status KeyGrad(const BlocksArgs& a, const BackwardSpace& s, const uint16_t* dout, BlocksRowInfo info, uint16_t* dk, uint16_t* dv, char* ws, hipStream_t st) {
     using S = BlocksKeyShape<DC, RGS>;
-    const uint32_t groups = (a.bs / 16 + 3) / 4;
+    const uint32_t groups = KeyGroups(a);
     const uint64_t per_pair = (uint64_t)s.capacity * groups;
     const size_t lds = std::max<size_t>(S::BUFFERS * S::STAGE, RGS > 1 ? (size_t)64 * S::D * 8 : 0) + (size_t)std::min(s.part_rows, a.Tq) * 4;
     return BlocksLaunch(BlocksKeyGradKernel<BF16, DC, ND, RGS>, BlocksPairGrid((uint64_t)a.B * a.Hkv, per_pair), lds, st, a, s.words, s.part_rows, s.capacity, s.slots, groups,
@@ -1077,7 +1079,9 @@ extern "C" gpann_status gpann_blocks_attend_backward(const gpann_blocks_layout* 
     GPANN_TRY(BlocksCheckMarks(L));
     GPANN_REQUIRE((uint64_t)L->batch * L->q_rows * L->q_heads < 0xFFFFFFFFull, "2^32 - 1 (query row, head) rows or more");
     const BlocksArgs a = BlocksMakeArgs(L, q, k, v, probes, nprobe);
-    GPANN_TRY(BlocksCheckWorkspace(workspace, workspace_bytes, BackwardLayout(a, L->head_dim).total));
+    const BackwardSpace space = BackwardLayout(a, L->head_dim);
+    GPANN_TRY(BlocksCheckGrid(BlocksPairGrid((uint64_t)a.B * a.Hkv, (uint64_t)space.capacity * KeyGroups(a))));   // before the query side is enqueued
+    GPANN_TRY(BlocksCheckWorkspace(workspace, workspace_bytes, space.total));
     GPANN_BLOCKS_ENTER(L, stream);
     if (a.B == 0) return GPANN_OK;
     GPANN_BLOCKS_DISPATCH(L, Backward, a, static_cast<const uint16_t*>(out), lse, static_cast<const uint16_t*>(dout), static_cast<uint16_t*>(dq),
