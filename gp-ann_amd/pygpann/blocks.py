@@ -52,6 +52,37 @@ def _u32(name, x):
     return x
 
 
+def _i32(name, x):
+    x = operator.index(x)
+    if not -1 << 31 <= x < 1 << 31:
+        raise GpannError(1, f"invalid argument: {name} = {x} is not a signed 32-bit number")
+    return x
+
+
+def _size(name, x):
+    x = operator.index(x)
+    if not 0 <= x < 1 << 64:
+        raise GpannError(1, f"invalid argument: {name} = {x} is not an unsigned 64-bit number")
+    return x
+
+
+def _strides(name, s):
+    s = tuple(operator.index(x) for x in s)
+    if len(s) != 3 or not all(-1 << 63 <= x < 1 << 63 for x in s):
+        raise GpannError(1, f"invalid argument: {name} = {s} is not three signed 64-bit numbers")
+    return (C.c_int64 * 3)(*s)
+
+
+def _address(x):
+    """a device pointer or None; 0 counts as None"""
+    if not x:
+        return None
+    x = operator.index(x)
+    if not 0 < x < 1 << 64:
+        raise GpannError(1, f"invalid argument: {x} is not a pointer")
+    return x
+
+
 class Layout:
     """The shapes of a call's tensors (gpann_blocks_layout).  Strides {batch or page, row, head} default to those of contiguous tensors; a page table's
     rows default to the blocks of a sequence."""
@@ -64,22 +95,20 @@ class Layout:
         q = (q_rows * q_heads * head_dim, q_heads * head_dim, head_dim)
         kv = ((block_rows if page_table else kv_rows) * kv_heads * head_dim, kv_heads * head_dim, head_dim)
         c = self.c = _Layout()
-        c.struct_bytes, c.device, c.dtype, c.flags = C.sizeof(_Layout), device, _DTYPES[dtype], CAUSAL if causal else 0
+        c.struct_bytes, c.device, c.dtype, c.flags = C.sizeof(_Layout), _i32("device", device), _DTYPES[dtype], CAUSAL if causal else 0
         for name, x in (("batch", batch), ("q_rows", q_rows), ("kv_rows", kv_rows), ("q_heads", q_heads), ("kv_heads", kv_heads), ("head_dim", head_dim),
                         ("block_rows", block_rows), ("page_stride", blocks if page_stride is None else page_stride), ("n_pages", n_pages)):
             setattr(c, name, _u32(name, x))
         c.scale = scale if scale is not None else head_dim ** -0.5 if head_dim > 0 else 1.0
-        c.q_len, c.kv_len, c.page_table = q_len or None, kv_len or None, page_table or None
-        q_stride = tuple(q_stride or q)
-        for name, s in (("q_stride", q_stride), ("k_stride", k_stride or kv), ("v_stride", v_stride or kv), ("out_stride", out_stride or q)):
-            if not all(-1 << 63 <= operator.index(x) < 1 << 63 for x in s):
-                raise GpannError(1, f"invalid argument: {name} = {tuple(s)} is not three signed 64-bit numbers")
-            setattr(c, name, (C.c_int64 * 3)(*s))
+        c.q_len, c.kv_len, c.page_table = _address(q_len), _address(kv_len), _address(page_table)
+        for name, s in (("q_stride", q_stride or q), ("k_stride", k_stride or kv), ("v_stride", v_stride or kv), ("out_stride", out_stride or q)):
+            setattr(c, name, _strides(name, s))
         self.blocks = blocks
 
 
 def _p(x):
-    return None if not x else C.c_void_p(x)
+    x = _address(x)
+    return None if x is None else C.c_void_p(x)
 
 
 def workspace_bytes(layout, nprobe, calls):
@@ -102,31 +131,32 @@ def summarize(layout, k, summary, new_rows=0, stream=None):
 def route(layout, q, summary, nprobe, probes, first=1, last=2, workspace=None, workspace_bytes=0, stream=None):
     """probes of every query row: the first and last visible blocks and the best-scored others, in block order, -1 behind them"""
     _check(lib().gpann_blocks_route(C.byref(layout.c), _p(q), _p(summary), _u32("nprobe", nprobe), _u32("first", first), _u32("last", last), _p(probes),
-                                    _p(workspace), workspace_bytes, _p(stream)))
+                                    _p(workspace), _size("workspace_bytes", workspace_bytes), _p(stream)))
 
 
 def attend(layout, q, k, v, probes, nprobe, out, lse=None, workspace=None, workspace_bytes=0, stream=None):
     """attention over the probed blocks"""
     _check(lib().gpann_blocks_attend(C.byref(layout.c), _p(q), _p(k), _p(v), _p(probes), _u32("nprobe", nprobe), _p(out), _p(lse), _p(workspace),
-                                     workspace_bytes, _p(stream)))
+                                     _size("workspace_bytes", workspace_bytes), _p(stream)))
 
 
 def attend_backward(layout, q, k, v, probes, nprobe, out, lse, dout, dq, dk, dv, workspace=None, workspace_bytes=0, stream=None):
     """gradients of attend"""
     _check(lib().gpann_blocks_attend_backward(C.byref(layout.c), _p(q), _p(k), _p(v), _p(probes), _u32("nprobe", nprobe), _p(out), _p(lse), _p(dout), _p(dq),
-                                              _p(dk), _p(dv), _p(workspace), workspace_bytes, _p(stream)))
+                                              _p(dk), _p(dv), _p(workspace), _size("workspace_bytes", workspace_bytes), _p(stream)))
 
 
 def weigh(layout, q, k, probes, nprobe, lse, mass_in, mass_out, workspace=None, workspace_bytes=0, stream=None):
     """mass_out = mass_in + the attention weights of this call's query rows"""
     _check(lib().gpann_blocks_weigh(C.byref(layout.c), _p(q), _p(k), _p(probes), _u32("nprobe", nprobe), _p(lse), _p(mass_in), _p(mass_out), _p(workspace),
-                                    workspace_bytes, _p(stream)))
+                                    _size("workspace_bytes", workspace_bytes), _p(stream)))
 
 
 def evict(layout, k, v, mass, keep, rows, count, k_out=None, v_out=None, mass_out=None, first=0, last=0, out_kv_stride=None, workspace=None, workspace_bytes=0,
           stream=None):
     """keeps the first, last and heaviest rows of every sequence and head; out_kv_stride defaults to contiguous [batch][keep][kv_heads][head_dim]"""
     c = layout.c
-    strides = (C.c_int64 * 3)(*(out_kv_stride or (keep * c.kv_heads * c.head_dim, c.kv_heads * c.head_dim, c.head_dim)))
-    _check(lib().gpann_blocks_evict(C.byref(c), _p(k), _p(v), _p(mass), _u32("keep", keep), _u32("first", first), _u32("last", last), _p(rows), _p(count),
-                                    _p(k_out), _p(v_out), C.byref(strides), _p(mass_out), _p(workspace), workspace_bytes, _p(stream)))
+    keep = _u32("keep", keep)
+    strides = _strides("out_kv_stride", out_kv_stride or (keep * c.kv_heads * c.head_dim, c.kv_heads * c.head_dim, c.head_dim))
+    _check(lib().gpann_blocks_evict(C.byref(c), _p(k), _p(v), _p(mass), keep, _u32("first", first), _u32("last", last), _p(rows), _p(count),
+                                    _p(k_out), _p(v_out), C.byref(strides), _p(mass_out), _p(workspace), _size("workspace_bytes", workspace_bytes), _p(stream)))
