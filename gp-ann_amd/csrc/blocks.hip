@@ -32,7 +32,7 @@ gpann_status BlocksCheckLayout(const gpann_blocks_layout* L) {
     GPANN_REQUIRE(d == 64 || d == 96 || d == 128 || d == 192 || d == 256, "head_dim must be 64, 96, 128, 192 or 256");
     GPANN_REQUIRE(L->block_rows >= 16 && L->block_rows <= 256 && L->block_rows % 16 == 0, "block_rows must be a multiple of 16 from 16 to 256");
     GPANN_REQUIRE(BlocksPerSequence(L) <= GPANN_BLOCKS_MAX_BLOCKS, "more than GPANN_BLOCKS_MAX_BLOCKS blocks per sequence");
-    GPANN_REQUIRE(std::isfinite(L->scale), "layout.scale is not finite");
+    GPANN_REQUIRE(std::isfinite(L->scale * kLog2e), "layout.scale (times log2 e) is not finite");
     const int64_t* strides[4] = {L->q_stride, L->k_stride, L->v_stride, L->out_stride};
     for (const int64_t* s : strides)
         for (int i = 0; i < 3; ++i) {

@@ -81,7 +81,7 @@ typedef struct gpann_blocks_layout {
     uint32_t q_heads, kv_heads;   /* q_heads a multiple of kv_heads */
     uint32_t head_dim;            /* 64, 96, 128, 192 or 256 */
     uint32_t block_rows;          /* a multiple of 16 up to 256 */
-    float scale;                  /* finite; of the logits, usually 1 / sqrt(head_dim) */
+    float scale;                  /* finite, below 2^127; of the logits, usually 1 / sqrt(head_dim) */
     const int32_t* q_len;         /* device [batch], clamped to [0, q_rows]; NULL: q_rows */
     const int32_t* kv_len;        /* device [batch], clamped to [0, kv_rows]; NULL: kv_rows */
     const int32_t* page_table;    /* device [batch][page_stride]: page of every block; NULL: contiguous cache */

@@ -44,3 +44,10 @@ def test_pointers_that_would_wrap_are_refused(blocks, pointer):
     _refused(blocks, lambda: blocks.attend(_layout(blocks), pointer, OK, OK, OK, 4, OK), match="pointer")
     with pytest.raises(blocks.GpannError, match="pointer"):
         _layout(blocks, kv_len=pointer)
+
+
+@pytest.mark.parametrize("scale", [3e38, -2.5e38])
+def test_scales_whose_powers_of_two_are_not_finite_are_refused(blocks, scale):
+    """the kernels' exponentials are powers of two: of the logits times log2 e = 1.44"""
+    for name, call in _calls(blocks, _layout(blocks, scale=scale)).items():
+        _refused(blocks, call, match="scale")
