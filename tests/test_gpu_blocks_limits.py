@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import blocks_ref as ref
+import test_gpu_blocks as base
 from test_gpu_blocks import SENTINEL, Problem
 
 pytestmark = pytest.mark.gpu
@@ -246,3 +247,30 @@ def test_an_eviction_that_could_keep_far_more_than_there_is(blocks):
     assert count.item() == 64 and rows[0, 0, :64].tolist() == list(range(64)) and (rows[0, 0, 64:] == -5).all()
     assert torch.equal(mass_out[0, 0, :64], mass[0, 0]) and (mass_out[0, 0, 64:] == SENTINEL).all()
     assert start.elapsed_time(end) < 3.0      # ms; two launches take hundredths of one, a loop over 2^24 slots by 512 threads hundreds
+
+
+@pytest.mark.parametrize("kw", [dict(keep=20000, kv_rows=33000, ties=True), dict(keep=500, kv_rows=70000, ties=True, first=4, last=100), dict(keep=33000, kv_rows=70000, kv_len=[70000, 32769])], ids=str)
+def test_evict_from_sequences_that_do_not_fit_lds(blocks, kw):
+    base.test_evict(blocks, kw)
+
+
+@pytest.mark.parametrize("kw", [dict(q_rows=2100), dict(q_rows=4200, dim=128, q_heads=3), dict(q_rows=2500, bs=80, paged=True, kv_len=[333])], ids=str)
+def test_weigh_of_more_query_rows_than_a_wavefront_lists_at_a_time(blocks, kw):
+    base.test_weigh(blocks, {**dict(batch=1, kv_rows=350, q_heads=2, kv_heads=1, bs=64, nprobe=3), **kw}, True)
+
+
+@pytest.mark.parametrize("kw", [dict(q_rows=1, kv_rows=20000), dict(q_rows=2, kv_rows=80000, nprobe=64), dict(q_rows=5, kv_rows=80000, dim=96, dtype="fp16", kv_len=[80000, 65600]),
+                                dict(q_rows=1, kv_rows=16 * 16384, nprobe=9, batch=1)], ids=str)
+def test_route_over_more_blocks_than_registers_hold(blocks, kw):
+    base.test_route(blocks, {**dict(bs=16, nprobe=20, q_heads=2, kv_heads=1), **kw})
+
+
+@pytest.mark.parametrize("kw", [dict(q_rows=2100, kv_rows=2100, bs=64), dict(q_rows=17000, kv_rows=400, bs=128, causal=False), dict(q_rows=17000, kv_rows=17000, bs=256, nprobe=2, dtype="fp16"),
+                                dict(q_rows=4500, kv_rows=4500, bs=16, dim=192, kv_len=[4400])], ids=str)
+def test_backward_of_more_query_rows_than_are_listed_at_a_time(blocks, kw):
+    p = Problem(blocks, **{**dict(seed=87, batch=1, q_heads=1, kv_heads=1, nprobe=3), **kw})
+    p.attend()
+    p.backward()
+    torch.cuda.synchronize()
+    p.check_attend()
+    p.check_backward()
