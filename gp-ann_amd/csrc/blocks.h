@@ -50,8 +50,8 @@ struct BlocksDevice {
     }
 };
 
+// (the layout has been checked)
 #define GPANN_BLOCKS_ENTER(L, stream)                \
-    GPANN_TRY(::gpann::BlocksCheckLayout(L));        \
     ::gpann::BlocksDevice blocks_device;             \
     GPANN_TRY(blocks_device.Enter((L)->device));     \
     GPANN_TRY(::gpann::BlocksCheckStream(L, stream))

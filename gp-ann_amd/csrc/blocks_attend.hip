@@ -88,7 +88,7 @@ __device__ __forceinline__ void BlocksAttendStep(const BlocksArgs& a, int visibl
             x[y][i] = BlocksExp2(x[y][i] - from);
             sum += x[y][i];
         }
-    // the weights enter the second product in the type of the values: 2^-9 (bf16) or 2^-12 (fp16) of each at most, as the values themselves
+    // the weights enter the second product in the type of the values: 2^-8 (bf16) or 2^-11 (fp16) of each at most, as the values themselves
     const u32x4_t p = BlocksPackOperand<BF16>(x[0], x[1]);
 #pragma unroll
     for (int d = 0; d < DC; ++d) o[d] = BlocksMfma<BF16>(BlocksColumn<DC / 2>(st.v, d), p, o[d]);
@@ -244,7 +244,7 @@ __device__ __forceinline__ void BlocksAttendTokens(const BlocksArgs& a, uint32_t
             for (int i = 0; i < 4; ++i) x[y][i] = BlocksExp2(x[y][i] - from);
             sum += (x[y][0] + x[y][1]) + (x[y][2] + x[y][3]);
         }
-        // the weights enter the second product in the type of the values: 2^-9 (bf16) or 2^-12 (fp16) of each at most, as the values themselves
+        // the weights enter the second product in the type of the values: 2^-8 (bf16) or 2^-11 (fp16) of each at most, as the values themselves
         const u32x4_t p = BlocksPackOperand<BF16>(x[0], x[1]);
         if (more)
             BlocksDmaWait<S::LOADS>();   // V has landed; the next K is on its way

@@ -86,7 +86,7 @@ struct BlocksWalkRows {
 // ... a wavefront's
 template <int CT>
 struct BlocksWalkColumns {
-    uint32_t t0, rows, full;          // first query row, how many are live, a bit for each
+    uint32_t t0, rows;                // first query row, how many are live
     int seen_by_all, seen_by_any;     // cache rows (a prefix) that its first and its last query row see
     uint32_t cols, mt;                // columns in use
     uint32_t in[CT], head[CT];        // this lane's columns: query row - t0, query head
@@ -97,7 +97,6 @@ struct BlocksWalkColumns {
         mt = w.mtiles > 1 ? (w.wt0 + wave) % w.mtiles : 0;
         cols = w.mtiles > 1 ? min(16u * CT, a.G - mt * 16 * CT) : w.tpw * a.G;
         rows = (int)t0 < w.m ? min(w.tpw, (uint32_t)w.m - t0) : 0;
-        full = rows == 32 ? ~0u : (1u << rows) - 1;
         seen_by_all = rows ? BlocksVisible(a, w.n, w.m, (int)t0) : 0;
         seen_by_any = rows ? BlocksVisible(a, w.n, w.m, (int)(t0 + rows - 1)) : 0;
 #pragma unroll
