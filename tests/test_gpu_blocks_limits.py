@@ -274,3 +274,94 @@ def test_backward_of_more_query_rows_than_are_listed_at_a_time(blocks, kw):
     torch.cuda.synchronize()
     p.check_attend()
     p.check_backward()
+
+
+# ---- layouts of other orders --------------------------------------------------------------------------------------------------------------------
+def spread(p, out_order=(0, 2, 1, 3)):
+    """q, k and v become slices of one packed tensor each with a gap behind every row, out, dout and their like [sequence][head][row][dim]; what is behind the
+    sequences' ends, and the gaps, hold NaN"""
+    def gapped(x, extra):
+        rows = torch.full((*x.shape[:2], x.shape[2] + extra, x.shape[3] + 8), float("nan"), dtype=x.dtype, device=x.device)
+        view = rows[:, :, extra:, 8:]
+        view.copy_(x)
+        return view
+    def turned(x):
+        y = torch.empty([x.shape[i] for i in out_order], dtype=x.dtype, device=x.device).permute(out_order)
+        return y.copy_(x)
+    p.q, p.k, p.v = gapped(p.q, 3), gapped(p.k, 1), gapped(p.v, 2)
+    p.out, p.dout = turned(p.out), turned(p.dout)
+    for b in range(p.batch):
+        p.dout[b, p.m[b]:] = float("nan")
+    p.L = p.blocks.Layout(p.batch, p.q_rows, p.kv_rows, p.q_heads, p.kv_heads, p.dim, p.bs, dtype=p.dtype, causal=p.causal, scale=p.scale,
+                          q_len=None if p.ql_t is None else p.ql_t.data_ptr(), kv_len=None if p.kv_t is None else p.kv_t.data_ptr(),
+                          q_stride=p.q.stride()[:3], k_stride=p.k.stride()[:3], v_stride=p.v.stride()[:3], out_stride=p.out.stride()[:3])
+
+
+LAYOUTS = [dict(), dict(q_rows=1, kv_rows=700, bs=64, dim=128), dict(q_rows=1, batch=5, bs=80, dim=256, nprobe=9), dict(bs=112, q_heads=14, dim=96, dtype="fp16"),
+           dict(bs=208, kv_rows=900, dim=192), dict(bs=240, kv_rows=900, q_rows=60, q_heads=3, kv_heads=1, kv_len=[777, 3], q_len=[60, 9]), dict(bs=80, dim=256, dtype="fp16", q_rows=30),
+           dict(batch=16, q_rows=40, q_heads=32, kv_heads=8, bs=144, kv_rows=300, dim=128, q_len=[40, 0] * 8), dict(batch=16, kv_heads=16, q_heads=256, q_rows=20, bs=176, kv_rows=400)]
+
+
+@pytest.mark.parametrize("kw", LAYOUTS, ids=str)
+def test_tensors_of_other_orders_and_strides(blocks, kw):
+    p = Problem(blocks, **{**dict(seed=91), **kw})
+    spread(p)
+    p.attend()
+    torch.cuda.synchronize()
+    p.check_attend()
+    lse = p.lse.clone()
+    p.out.fill_(SENTINEL)
+    blocks.attend(p.L, p.q.data_ptr(), p.k.data_ptr(), p.v.data_ptr(), p.probes.data_ptr(), p.nprobe, p.out.data_ptr(), **p.space)      # no lse wanted
+    torch.cuda.synchronize()
+    p.check_attend()
+    for b in range(p.batch):
+        p.lse[b, p.m[b]:] = float("nan")
+        p.out[b, p.m[b]:] = float("nan")
+    for name in ("q", "k", "v"):
+        x = getattr(p, name)
+        base_tensor = torch.full((x.shape[0] * x.stride(0),), SENTINEL, dtype=x.dtype, device="cuda")
+        setattr(p, "d" + name, torch.as_strided(base_tensor, x.shape, x.stride()))
+    p.backward_call()
+    torch.cuda.synchronize()
+    check_gradients(p)
+    p.check_backward()
+    for name in ("q", "k", "v"):           # the gaps are nobody's
+        x = getattr(p, "d" + name)
+        whole = torch.as_strided(x, (x.shape[0] * x.stride(0),), (1,), 0).clone()
+        torch.as_strided(whole, x.shape, x.stride()).fill_(SENTINEL)
+        assert (whole == SENTINEL).all()
+    assert torch.equal(lse[p.lse == p.lse], p.lse[p.lse == p.lse])
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(bs=80, dim=256, kv_rows=333, q_rows=20), dict(kv_len=[150, 61], nprobe=3, dim=96, dtype="fp16", q_rows=40)], ids=str)
+def test_routing_weights_and_eviction_of_other_orders_and_strides(blocks, kw):
+    p = Problem(blocks, **{**dict(seed=92, nprobe=3), **kw})
+    spread(p)
+    s = torch.full((p.batch, p.kv_heads, p.nblk, p.dim), SENTINEL, device="cuda")
+    blocks.summarize(p.L, p.k.data_ptr(), s.data_ptr())
+    probes = torch.full_like(p.probes, 12345)
+    blocks.route(p.L, p.q.data_ptr(), s.data_ptr(), p.nprobe, probes.data_ptr(), first=1, last=1, **p.space)
+    got, cen = probes.cpu().numpy(), s.cpu().numpy()
+    for b, t, h, heads, vis in p.rows():
+        assert np.array_equal(cen[b, h, :-(-p.n[b] // p.bs)], ref.summarize(p.k64[b, :, h], p.n[b], p.bs))
+        assert np.array_equal(got[b, t, h], ref.route(p.q64[b, t, heads], cen[b, h], p.bs, vis, p.nprobe, 1, 1)), (b, t, h)
+    p.attend()
+    mass = torch.zeros(p.batch, p.kv_heads, p.kv_rows, device="cuda")
+    blocks.weigh(p.L, p.q.data_ptr(), p.k.data_ptr(), p.probes.data_ptr(), p.nprobe, p.lse.data_ptr(), mass.data_ptr(), mass.data_ptr(), **p.space)
+    weights, sums = mass.cpu().numpy(), np.zeros((p.batch, p.kv_heads))
+    for b, t, h, heads, vis in p.rows():
+        sums[b, h] += p.G * (len(ref.rows_of(p.probes_np[b, t, h], p.bs, p.nblk, vis)) > 0)
+    assert np.allclose(weights.sum(2), sums, rtol=1e-4)          # (every head spreads a weight of 1; binary32 sums of at most 1000 terms)
+    keep = 45
+    rows, count = torch.full((p.batch, p.kv_heads, keep), -5, dtype=torch.int32, device="cuda"), torch.zeros(p.batch, p.kv_heads, dtype=torch.int32, device="cuda")
+    both = torch.full((p.batch, p.kv_heads, 2, keep, p.dim), SENTINEL, dtype=p.k.dtype, device="cuda")          # [sequence][head][k, v][row][dim]
+    k_out, v_out = (both[:, :, i].permute(0, 2, 1, 3) for i in range(2))
+    blocks.evict(p.L, p.k.data_ptr(), p.v.data_ptr(), mass.data_ptr(), keep, rows.data_ptr(), count.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), first=2, last=3,
+                 out_kv_stride=k_out.stride()[:3], **p.space)
+    for b in range(p.batch):
+        for h in range(p.kv_heads):
+            want = ref.evict(weights[b, h], p.n[b], keep, 2, 3)
+            c = len(want)
+            assert count[b, h] == c and rows[b, h, :c].tolist() == want
+            assert np.array_equal(k_out[b, :c, h].double().cpu().numpy(), p.k64[b, want, h]) and np.array_equal(v_out[b, :c, h].double().cpu().numpy(), p.v64[b, want, h])
+            assert (k_out[b, c:, h] == SENTINEL).all() and (v_out[b, c:, h] == SENTINEL).all()
