@@ -70,8 +70,8 @@ __device__ __forceinline__ void BlocksAttendStep(const BlocksArgs& a, int visibl
     }
     float best = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
     best = BlocksMaxOver4(best);
-    if (__ballot(best > top + kBlocksSlack)) {
-        best = fmaxf(top, best);
+    if (__ballot(best > top + kBlocksSlack<BF16>)) {
+        best = fmaxf(top, best - kBlocksLift<BF16>);
         const float shrink = top == best ? 1.f : BlocksExp2(top - best);   // (top = best = -inf: nothing seen yet)
         top = best;
         sum *= shrink;
@@ -88,7 +88,8 @@ __device__ __forceinline__ void BlocksAttendStep(const BlocksArgs& a, int visibl
             x[y][i] = BlocksExp2(x[y][i] - from);
             sum += x[y][i];
         }
-    // the weights enter the second product in the type of the values: 2^-8 (bf16) or 2^-11 (fp16) of each at most, as the values themselves
+    // the weights enter the second product in the type of the values: 2^-8 (bf16) or 2^-11 (fp16) of each at most, as the values themselves (fp16: of those
+    // above 2^-21 of the largest)
     const u32x4_t p = BlocksPackOperand<BF16>(x[0], x[1]);
 #pragma unroll
     for (int d = 0; d < DC; ++d) o[d] = BlocksMfma<BF16>(BlocksColumn<DC / 2>(st.v, d), p, o[d]);
@@ -227,8 +228,8 @@ __device__ __forceinline__ void BlocksAttendTokens(const BlocksArgs& a, uint32_t
             best = BlocksMaxOf4(x[y], best);
         }
         best = BlocksMaxOver4(best);
-        if (__ballot(best > top + kBlocksSlack)) {
-            best = fmaxf(top, best);
+        if (__ballot(best > top + kBlocksSlack<BF16>)) {
+            best = fmaxf(top, best - kBlocksLift<BF16>);
             const float shrink = top == best ? 1.f : BlocksExp2(top - best);   // (top = best = -inf: nothing seen yet)
             top = best;
             sum *= shrink;
@@ -244,7 +245,8 @@ __device__ __forceinline__ void BlocksAttendTokens(const BlocksArgs& a, uint32_t
             for (int i = 0; i < 4; ++i) x[y][i] = BlocksExp2(x[y][i] - from);
             sum += (x[y][0] + x[y][1]) + (x[y][2] + x[y][3]);
         }
-        // the weights enter the second product in the type of the values: 2^-8 (bf16) or 2^-11 (fp16) of each at most, as the values themselves
+        // the weights enter the second product in the type of the values: 2^-8 (bf16) or 2^-11 (fp16) of each at most, as the values themselves (fp16: of
+        // those above 2^-21 of the largest)
         const u32x4_t p = BlocksPackOperand<BF16>(x[0], x[1]);
         if (more)
             BlocksDmaWait<S::LOADS>();   // V has landed; the next K is on its way
@@ -464,12 +466,12 @@ __device__ __forceinline__ void BlocksWalkAttend(float scale2, const BlocksWalkA
             best[c] = fmaxf(best[c], member[c][e] ? most : -inf);
         }
         best[c] = BlocksMaxOver4(best[c]) * scale2;
-        raise = raise || best[c] > top[c] + kBlocksSlack;
+        raise = raise || best[c] > top[c] + kBlocksSlack<BF16>;
     }
     if (__ballot(raise)) {
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-            best[c] = fmaxf(top[c], best[c]);
+            best[c] = fmaxf(top[c], best[c] - kBlocksLift<BF16>);
             const float shrink = top[c] == best[c] ? 1.f : BlocksExp2(top[c] - best[c]);
             top[c] = best[c];
             sum[c] *= shrink;

@@ -112,9 +112,13 @@ __device__ __forceinline__ float BlocksAddLane(float x) {
     return x + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xF, 0xF, false));
 }
 __device__ __forceinline__ float BlocksSumRow16(float x) { return BlocksAddLane<0x140>(BlocksAddLane<0x141>(BlocksAddLane<0x4E>(BlocksAddLane<0xB1>(x)))); }
-// The running maximum follows the true one only when that is more than this many powers of two ahead: weights then reach 2^8 instead of 1, which 16-bit
-// floats hold as exactly, and the accumulators are hardly ever rescaled.
-constexpr float kBlocksSlack = 8.f;
+// What logits are measured against follows their running maximum only when that is more than `kBlocksSlack` powers of two ahead, and then to `kBlocksLift` below
+// it: weights reach 2^8 instead of 1 in bf16, which holds them as exactly, and the accumulators are hardly ever rescaled.  Binary16 holds up to 2^16, and in full
+// only what is above 2^-14: weights between 2^7 and 2^15 for the largest keep those of 2^-21 of it whole.
+template <bool BF16>
+constexpr float kBlocksLift = BF16 ? 0.f : 7.f;
+template <bool BF16>
+constexpr float kBlocksSlack = 8.f + kBlocksLift<BF16>;
 __device__ __forceinline__ int64_t BlocksReadLane64(int64_t x, uint32_t lane) {
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, (int)lane);
     const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)x >> 32), (int)lane);

@@ -29,7 +29,7 @@
  * reads, but for gpann_blocks_weigh in place.
  *
  * Rounding: logits, sums, softmax statistics and masses are binary32, centroids and scores as above; weights and ds are rounded once to the tensors' type
- * where they enter a matrix product, so in GPANN_BLOCKS_FP16 a weight below 2^-25 of a row's largest counts as 0 in out, one below 2^-40 in dv, and a ds
+ * where they enter a matrix product, so in GPANN_BLOCKS_FP16 a weight below 2^-32 of a row's largest counts as 0 in out, one below 2^-40 in dv, and a ds
  * below 2^-25 in dq and dk (scale a loss whose gradients are that small).  A ds that GPANN_BLOCKS_FP16 does not hold (above 65504) costs time, not the
  * result: the sums it enters are done again, row by row.  So are sums that a value which is not finite enters: it reaches the rows and keys that see it
  * and no others.

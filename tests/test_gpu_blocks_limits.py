@@ -365,3 +365,37 @@ def test_routing_weights_and_eviction_of_other_orders_and_strides(blocks, kw):
             assert count[b, h] == c and rows[b, h, :c].tolist() == want
             assert np.array_equal(k_out[b, :c, h].double().cpu().numpy(), p.k64[b, want, h]) and np.array_equal(v_out[b, :c, h].double().cpu().numpy(), p.v64[b, want, h])
             assert (k_out[b, c:, h] == SENTINEL).all() and (v_out[b, c:, h] == SENTINEL).all()
+
+
+# ---- attention whose weights binary16 holds only in part ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kw", [dict(batch=1, q_rows=1), dict(batch=1, q_rows=1, dim=256, kv_heads=2), dict(batch=64, q_rows=1, kv_rows=300), dict(batch=8, q_rows=40, q_heads=16, kv_heads=8, kv_rows=400),
+                                dict(batch=16, kv_heads=16, q_heads=256, q_rows=20, kv_rows=300, dim=128), dict(batch=8, q_rows=40, q_heads=32, kv_heads=8, kv_rows=300, dim=192, bs=16),
+                                dict(batch=8, q_rows=40, q_heads=16, kv_heads=8, kv_rows=400, beside=True)], ids=str)
+def test_attention_that_hangs_on_weights_binary16_holds_in_part(blocks, kw):
+    """one key has nearly all the weight and the value 0: out is a sum over the others, whose weights are 2^-16 to 2^-20"""
+    kw = {**dict(seed=95, kv_rows=1000, q_heads=4, kv_heads=2, bs=64, nprobe=16, dtype="fp16"), **kw}
+    beside = kw.pop("beside", False)
+    p = Problem(blocks, **kw)
+    p.probes_np[...] = np.where(np.arange(p.nprobe) < p.nblk, np.arange(p.nprobe), -1)
+    if beside:          # every second row sees values that are none: the others are done again by themselves
+        p.probes_np[:, 1::2, :, p.nblk - 1] = -1
+    p.probes.copy_(torch.from_numpy(p.probes_np))
+    bits = np.linspace(16, 20, p.q_rows * p.q_heads).reshape(p.q_rows, p.q_heads)
+    for x, y in ((p.q, p.q64), (p.k, p.k64)):
+        x.zero_()
+        y[...] = 0
+    p.q[..., 0] = torch.from_numpy(bits * np.log(2) / p.scale / 64).to(p.q)
+    p.q64[..., 0] = p.q[..., 0].double().cpu().numpy()
+    p.k[:, 0, :, 0] = p.k64[:, 0, :, 0] = 64
+    p.v.abs_().mul_(4)
+    p.v[:, 0], p.v64[...] = 0, np.abs(p.v64) * 4
+    p.v64[:, 0] = 0
+    if beside:
+        p.v[:, (p.nblk - 1) * p.bs:] = float("nan")
+    p.attend()
+    torch.cuda.synchronize()
+    out = p.out.double().cpu().numpy()
+    for b, t, h, heads, vis in p.rows():
+        if not beside or t % 2:
+            want, _, tol, _ = ref.attend(p.q64[b, t, heads], p.k64[b, :, h], p.v64[b, :, h], p.probes_np[b, t, h], p.bs, p.nblk, vis, p.scale, p.dtype)
+            assert (np.abs(out[b, t, heads] - want) <= tol).all(), (b, t, h, np.abs(out[b, t, heads] / want - 1).max())
