@@ -44,26 +44,31 @@ def lib():
     return _lib
 
 
-def _u32(name, x):
-    """a C uint32 takes any Python int modulo 2^32: refuse what would wrap"""
+def _whole(name, x, least, most, what):
     x = operator.index(x)
-    if not 0 <= x <= 0xFFFFFFFF:
-        raise GpannError(1, f"invalid argument: {name} = {x} is not an unsigned 32-bit number")
+    if not least <= x <= most:
+        raise GpannError(1, f"invalid argument: {name} = {x} is not {what}")
     return x
+
+
+# A C integer takes any Python int modulo its size: what would wrap is refused.  (A call has a dozen of them, so a plain int in range goes no further.)
+def _u32(name, x):
+    return x if x.__class__ is int and 0 <= x <= 0xFFFFFFFF else _whole(name, x, 0, 0xFFFFFFFF, "an unsigned 32-bit number")
 
 
 def _i32(name, x):
-    x = operator.index(x)
-    if not -1 << 31 <= x < 1 << 31:
-        raise GpannError(1, f"invalid argument: {name} = {x} is not a signed 32-bit number")
-    return x
+    return _whole(name, x, -0x80000000, 0x7FFFFFFF, "a signed 32-bit number")
 
 
 def _size(name, x):
-    x = operator.index(x)
-    if not 0 <= x < 1 << 64:
-        raise GpannError(1, f"invalid argument: {name} = {x} is not an unsigned 64-bit number")
-    return x
+    return x if x.__class__ is int and 0 <= x <= 0xFFFFFFFFFFFFFFFF else _whole(name, x, 0, 0xFFFFFFFFFFFFFFFF, "an unsigned 64-bit number")
+
+
+def _p(x):
+    """a device pointer or None, which 0 counts as"""
+    if x.__class__ is int and 0 < x <= 0xFFFFFFFFFFFFFFFF:
+        return x
+    return (_whole("a tensor's or stream's address", x, 1, 0xFFFFFFFFFFFFFFFF, "a pointer")) if x else None
 
 
 def _strides(name, s):
@@ -71,16 +76,6 @@ def _strides(name, s):
     if len(s) != 3 or not all(-1 << 63 <= x < 1 << 63 for x in s):
         raise GpannError(1, f"invalid argument: {name} = {s} is not three signed 64-bit numbers")
     return (C.c_int64 * 3)(*s)
-
-
-def _address(x):
-    """a device pointer or None; 0 counts as None"""
-    if not x:
-        return None
-    x = operator.index(x)
-    if not 0 < x < 1 << 64:
-        raise GpannError(1, f"invalid argument: {x} is not a pointer")
-    return x
 
 
 class Layout:
@@ -100,15 +95,10 @@ class Layout:
                         ("block_rows", block_rows), ("page_stride", blocks if page_stride is None else page_stride), ("n_pages", n_pages)):
             setattr(c, name, _u32(name, x))
         c.scale = scale if scale is not None else head_dim ** -0.5 if head_dim > 0 else 1.0
-        c.q_len, c.kv_len, c.page_table = _address(q_len), _address(kv_len), _address(page_table)
+        c.q_len, c.kv_len, c.page_table = _p(q_len), _p(kv_len), _p(page_table)
         for name, s in (("q_stride", q_stride or q), ("k_stride", k_stride or kv), ("v_stride", v_stride or kv), ("out_stride", out_stride or q)):
             setattr(c, name, _strides(name, s))
         self.blocks = blocks
-
-
-def _p(x):
-    x = _address(x)
-    return None if x is None else C.c_void_p(x)
 
 
 def workspace_bytes(layout, nprobe, calls):
