@@ -518,10 +518,12 @@ __device__ __forceinline__ void BlocksWalkAttend(float scale2, const BlocksWalkA
 
 // The walk of blocks_walk.h with the running maximum and sum of a softmax.  NT: tiles taken at a time; NM: of how many blocks they may be.
 //
-// 8192 query rows of 32 heads, 8 key/value heads of 128 dimensions, 16 probes of 64 rows (125 GFLOP of probed products): 366 us, 342 TFLOP/s.  The matrix cores
-// are busy for 28 % of the cycles, the vector units for 40 %, LDS for 14 %: a wavefront goes through reads, products and weights of a stage one after the other,
-// a SIMD has only two of them (each takes half the register file), and a barrier waits for the one with most to do.  What made it faster was fewer vector
-// instructions (493 -> 383 us), not more overlap inside a wavefront (no difference) or wavefront priorities (none).
+// 8192 query rows of 32 heads, 8 key/value heads of 128 dimensions, 16 probes of 64 rows (125 GFLOP of probed products): 355 us a call, 352 TFLOP/s.  The matrix
+// cores are busy for 28 % of the cycles, the vector units for 40 %, LDS for 14 %.  228 GFLOP are issued: a wavefront's columns are multiplied together when one of
+// their query rows looks at a block.  And a wavefront goes through reads, products and weights of a stage one after the other, a SIMD has only two of them (256
+// registers each, 3 more in scratch, and LDS has room for one workgroup), and a barrier waits for the one with most to do.  What made it faster was fewer vector
+// instructions (493 -> 383 us), not more overlap inside a wavefront (no difference) or wavefront priorities (none).  Rows of 256 dimensions keep 76 registers in
+// scratch.
 template <bool BF16, int DC, int CT, int NT, int NM>
 __global__ void __launch_bounds__(512) BlocksAttendWalkKernel(BlocksArgs a, uint32_t tpw, uint32_t mtiles, uint32_t tiles, uint16_t* __restrict__ out,
                                                               float* __restrict__ lse) {

@@ -16,11 +16,12 @@ namespace gpann {
 // Where ds' sums to more than rounding can have done, `out` and `lse` are not of these keys alone (attention joined over several calls, whose gradients are taken
 // from the joined ones): there is no such e, and nothing is corrected.
 // (8192 rows of 128 dimensions in bf16, relative error of dq: 0.0017 is its own rounding, 0.0023 this, 0.0025 with the sum before the rounding, 0.0032
-// uncorrected.  The products for w cost 63 of 720 us.)
+// uncorrected.  The products for w took 63 us when the query side took 720.)
 //
-// 8192 query rows of 32 heads, 8 key/value heads of 128 dimensions, 16 probes of 64 rows: the query side takes 549 us (three products, 188 GFLOP: 340 TFLOP/s;
-// with the one for w the matrix cores are busy for 33 % of the cycles) and the key side 470 us (four products, 250 GFLOP: 530 TFLOP/s, 26 %); joining 18,
-// counting and marking rows 8 each.  Both are bound as the forward is: two wavefronts a SIMD, whose reads, products and weights overlap little.
+// 8192 query rows of 32 heads, 8 key/value heads of 128 dimensions, 16 probes of 64 rows, by the profiler: the query side takes 563 us (three products, 188
+// GFLOP: 334 TFLOP/s; with the one for w, and the columns that look at nothing, 395 are issued and the matrix cores are busy for 32 % of the cycles) and the key
+// side 472 us (four products, 250 GFLOP: 530 TFLOP/s, 26 %); joining 18, counting and marking rows 8 each.  Both are bound as the forward is: two wavefronts a
+// SIMD, whose reads, products and weights overlap little.  In scratch: 5 to 8 registers of the query side up to 192 dimensions, 73 to 76 at 256; 2 to 6 of the key side at 256.
 
 // What the key side needs of a (query row, head) row: lse * log2 e (+inf: it weighs nothing) and delta.  Both arrays end with an entry of a row that weighs nothing.
 struct BlocksRowInfo {
@@ -220,7 +221,7 @@ __device__ __forceinline__ void BlocksWalkQueryGrad(float scale2, const BlocksWa
         }
         __builtin_amdgcn_sched_barrier(0);
         // One matrix instruction, then a step of the weights, and so on: a wavefront's vector instructions run beside its matrix instructions where they alternate
-        // (64 products and 192 additions in a loop, two wavefronts a SIMD: 1326 ticks taking turns, 2353 one block after the other; here 613 -> 601 us).
+        // (64 products and 192 additions in a loop, two wavefronts a SIMD: 1326 ticks taking turns, 2353 one block after the other; this kernel 613 -> 601 us when it was changed to it).
         constexpr int STEPS = 2 * DC > 16 ? 2 * DC : 16;   // 2 DC = 4 KS products, 16 steps of the weights
 #pragma unroll
         for (int n = 0; n < STEPS; ++n) {

@@ -90,7 +90,9 @@ typedef struct gpann_blocks_layout {
     int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
 } gpann_blocks_layout;
 
-/* Bytes of workspace that any of `calls` (GPANN_BLOCKS_ROUTE | ...) needs for this layout; 0 where a call needs none (`workspace` may be NULL then). */
+/* Bytes of workspace that any of `calls` (GPANN_BLOCKS_ROUTE | ...) needs for this layout; 0 where a call needs none (`workspace` may be NULL then; route and
+ * evict need none today).  Gradients need the most: they have room for every probe list that the layout allows (8192 rows of 32 heads, 8 key/value heads of 128
+ * dimensions, 16 probes: 131 MiB; 131072 rows, 64 probes: 8.3 GiB). */
 gpann_status gpann_blocks_workspace_bytes(const gpann_blocks_layout* layout, uint32_t nprobe, uint32_t calls, size_t* out_bytes);
 
 /* Centroids of the blocks that hold one of the last `new_rows` rows of each sequence (0: of all its blocks).  Others stay as they were.
