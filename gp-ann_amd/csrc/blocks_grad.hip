@@ -29,7 +29,7 @@ struct BlocksRowInfo {
     float* delta;
 };
 
-// <dout, out>, and the most that rounding `out` to its type can have moved it by: half a step of every term (1.25: of which the sums' own roundings are a part)
+// <dout, out>, and 1.25 times the most that rounding `out` to its type can have moved it by: half a step of every term, in binary16 at least that of its smallest numbers
 template <bool BF16, int DC>
 __device__ __forceinline__ float BlocksDelta(const uint16_t* out, const u32x4_t (&go)[DC / 2], float& slack) {
     u32x4_t y[DC / 2];
@@ -44,6 +44,7 @@ __device__ __forceinline__ float BlocksDelta(const uint16_t* out, const u32x4_t 
             delta += lo;
             delta += hi;
             size += fabsf(lo) + fabsf(hi);
+            if (!BF16) size += (fabsf(BlocksToFloat((uint16_t)go[s][i], BF16)) + fabsf(BlocksToFloat((uint16_t)(go[s][i] >> 16), BF16))) * 0x1p-14f;   // 2^-25 / 2^-11
         }
     slack = BlocksSumOver4(size) * (BF16 ? 1.25f / 256.f : 1.25f / 2048.f);
     return BlocksSumOver4(delta);

@@ -22,7 +22,7 @@ def formula(p, b, t, h, heads, vis, out, lse, probes):
 
     E = 2^-24, u = half a step of the type, s = half the smallest step of binary16 (2^-25) or 0.  A logit is off by (d + 4) E a, a = |scale| sum |q_i k_i| at most, and
     a weight by w = 2 (d + 4) E a + 8 E + 4 E |lse| of itself (exponent's argument and lse * log2 e); dp and delta by (d + 2) E of the sums of their terms' sizes.
-    delta may be corrected for the rounding of out: by no more than 1.25 u sum |dout out| (+ s sum |dout|), what that rounding can have come to and a quarter more.
+    delta may be corrected for the rounding of out: by no more than 1.25 (u sum |dout out| + s sum |dout|), what that rounding can have come to and a quarter more.
     p and ds are rounded once, to u of themselves or s; sums of n terms in binary32 add n E of the terms' sizes."""
     u, s, d = ref.U[p.dtype], 2.0 ** -25 if p.dtype == "fp16" else 0.0, p.dim
     rows = ref.rows_of(probes[b, t, h], p.bs, p.nblk, vis)
@@ -35,7 +35,7 @@ def formula(p, b, t, h, heads, vis, out, lse, probes):
     pr = np.exp(p.scale * (q @ k.T) - l[:, None])
     delta = (do * o).sum(1, keepdims=True)
     ds = pr * (do @ v.T - delta)
-    off = 1.25 * u * (np.abs(do) * np.abs(o)).sum(1, keepdims=True) + s * np.abs(do).sum(1, keepdims=True)
+    off = 1.25 * (u * (np.abs(do) * np.abs(o)).sum(1, keepdims=True) + s * np.abs(do).sum(1, keepdims=True))
     dp_err = (d + 2) * ref.E * (np.abs(do) @ np.abs(v).T + (np.abs(do) * np.abs(o)).sum(1, keepdims=True)) + off
     ds_err = pr * (1 + w) * dp_err + (w + u + 2 * ref.E) * np.abs(ds) + s
     n = len(rows)
@@ -399,3 +399,35 @@ def test_attention_that_hangs_on_weights_binary16_holds_in_part(blocks, kw):
         if not beside or t % 2:
             want, _, tol, _ = ref.attend(p.q64[b, t, heads], p.k64[b, :, h], p.v64[b, :, h], p.probes_np[b, t, h], p.bs, p.nblk, vis, p.scale, p.dtype)
             assert (np.abs(out[b, t, heads] - want) <= tol).all(), (b, t, h, np.abs(out[b, t, heads] / want - 1).max())
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(dim=192, bs=64), dict(q_rows=70, kv_rows=300, q_heads=16, kv_heads=1)], ids=str)
+def test_gradients_of_values_near_the_smallest_of_binary16(blocks, kw):
+    """values of 2^-16: the steps of out are a hundredth of it, and delta's error is told from the weights' own sum all the same.  Against the gradient at the unrounded out:
+    what is left of delta's error is the sum of the ds' own rounding, u sum |ds|, the weights' in out (u sum p |dp|) and binary32's"""
+    p = Problem(blocks, **{**dict(seed=96, batch=1, q_rows=40, kv_rows=150, nprobe=5, dtype="fp16"), **kw})
+    p.probes_np[...] = np.arange(p.nprobe)
+    p.probes.copy_(torch.from_numpy(p.probes_np))
+    scaled(p, dout=2.0 ** 8)
+    p.v.mul_(2.0 ** -16)
+    p.v64 = p.v.double().cpu().numpy()
+    p.v64[np.isnan(p.v64)] = 0
+    p.attend()
+    p.backward()
+    torch.cuda.synchronize()
+    u, got, s = ref.U["fp16"], p.dq.double().cpu().numpy(), 2.0 ** -25
+    for b, t, h, heads, vis in p.rows():
+        rows = ref.rows_of(p.probes_np[b, t, h], p.bs, p.nblk, vis)
+        if len(rows) == 0:
+            continue
+        k, v, do = p.k64[b, rows, h], p.v64[b, rows, h], p.do64[b, t, heads]
+        lse, pr, w = ref.softmax_rows(p.q64[b, t, heads], k, p.scale)
+        dp = do @ v.T
+        ds = pr * (dp - (pr * dp).sum(1, keepdims=True))
+        n, away = len(rows), np.abs(k)
+        each = (u + 3 * w + n * ref.E) * np.abs(ds) + (p.dim + 2) * ref.E * pr * (np.abs(do) @ np.abs(v).T) + s                  # a ds' own error
+        left = each.sum(1, keepdims=True) + (u + w) * (pr * np.abs(dp)).sum(1, keepdims=True)                                  # delta's
+        bound = abs(p.scale) * ((each + pr * left) @ away)
+        want = p.scale * (ds @ k)
+        bound += u * (np.abs(want) + bound) + s
+        assert (np.abs(got[b, t, heads] - want) <= bound).all(), (b, t, h, (np.abs(got[b, t, heads] - want) / bound).max())
